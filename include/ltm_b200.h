@@ -262,6 +262,110 @@ LTM_API ltm_status ltm_memory_store_noalloc(void* memory, const void* keys, int6
                                             int use_attention_scores, ltm_dtype dtype,
                                             void* stream);
 
+/* -------------------------------------------------------------- KV cache -- */
+/* The cache as a store of its own, and what serving does with it beyond one
+ * greedy token: int8 caches, attention of several drafted tokens, beam search.
+ * No callable counterpart in the reference, whose cache manager is a stub
+ * (python_bindings/src/main.cpp:101-135).
+ *
+ * Caches are those of the decode step: contiguous, head-major
+ * [B, kv_heads, max_positions, head_dim], 16-byte aligned, head_dim 64 or 128.
+ * With scales (fp32 [B, kv_heads, max_positions]) they hold int8 codes, without
+ * (NULL) values of `dtype` (f16 / bf16).  Strides are in elements.  Sequence b
+ * is skipped, and the device error word set to 5, where cache_lens[b] or
+ * num_tokens[b] is negative, num_tokens[b] > T, or cache_lens[b] + num_tokens[b]
+ * passes max_positions.  Nothing here allocates or keeps state; calls on
+ * different streams are independent as long as their buffers are. */
+
+/* Writes T new tokens of every sequence at positions cache_lens[b] .. + T
+ * (device int32 [B]; num_tokens, device int32 [B] or NULL: only the first
+ * num_tokens[b] of them).  k, v: token t of batch b, head h starts at
+ * k + b * k_strides[0] + t * k_strides[1] + h * k_strides[2] (host arrays of
+ * three; 16-byte aligned rows).  int8 caches take dtype f32, f16 or bf16:
+ *   s = max_d |x_d| / 127 ;  q_d = clamp(round_half_away(x_d / s), -127, 127)
+ *   per token and head (s == 0 => q = 0); a row with an infinity or a NaN gets
+ *   s = NaN and q = 0, so that whatever reads it gets NaN.
+ * Positions outside the written ones keep their bytes. */
+LTM_API ltm_status ltm_kv_cache_append(const void* k, const int64_t* k_strides, const void* v,
+                                       const int64_t* v_strides, ltm_dtype dtype, void* k_cache,
+                                       void* v_cache, float* k_scale, float* v_scale,
+                                       int64_t max_positions, const int32_t* cache_lens,
+                                       const int32_t* num_tokens, int B, int T, int kv_heads,
+                                       int head_dim, void* stream);
+
+/* Reads n positions of every sequence from first[b] on (device int32 [B];
+ * NULL: 0) into out, contiguous [B, kv_heads, n, head_dim] of out_dtype:
+ * q * s of an int8 cache (one fp32 product, rounded to out_dtype), or a copy of a
+ * 16-bit cache of out_dtype (scale NULL).  Positions outside
+ * [0, min(max_positions, cache_lens[b])) (cache_lens: device int32 [B] or NULL)
+ * give zeros. */
+LTM_API ltm_status ltm_kv_cache_read(const void* cache, const float* scale, ltm_dtype out_dtype,
+                                     int64_t max_positions, const int32_t* first,
+                                     const int32_t* cache_lens, int B, int kv_heads, int head_dim,
+                                     int n, void* out, void* stream);
+
+/* Attention of T drafted tokens per sequence (T <= 64; T = 1: a decode step)
+ * over the cache:
+ *   o_t = softmax_j(q_t . k_j / sqrt(head_dim)) v_j
+ * over j in [0, cache_lens[b]) and, at positions cache_lens[b] + a, the token
+ * itself (a = t) and its ancestors: parents (device int32 [B, T]) holds a
+ * token's parent, an earlier token of the draft, or -1 for a root; NULL is a
+ * chain (every token sees those before it).  The drafted tokens' keys and values
+ * have been appended at cache_lens[b] .. + T.  A parent that does not come before
+ * its token counts as -1 and sets the device error word to 7.
+ * num_heads is a multiple of kv_heads: query head h reads cached head
+ * h / (num_heads / kv_heads).  q and o: token t of batch b, head h at
+ * b * s[0] + t * s[1] + h * s[2] (multiples of 8 elements), f16 / bf16; int8
+ * caches serve both.  Tokens t >= num_tokens[b], and those of a skipped
+ * sequence, get zeros.  What the cache holds at positions that a token does not
+ * see never reaches its output, NaN and infinities included.
+ * workspace: device memory of ltm_tree_attention_workspace bytes, 16-byte
+ * aligned, that nothing else uses until the call's work is done. */
+LTM_API ltm_status ltm_tree_attention_workspace(int B, int T, int num_heads, int kv_heads,
+                                                int head_dim, size_t* bytes);
+LTM_API ltm_status ltm_tree_attention(const void* q, const int64_t* q_strides, const void* k_cache,
+                                      const void* v_cache, const float* k_scale,
+                                      const float* v_scale, int64_t max_positions,
+                                      const int32_t* cache_lens, const int32_t* num_tokens,
+                                      const int32_t* parents, void* o, const int64_t* o_strides,
+                                      int B, int T, int num_heads, int kv_heads, int head_dim,
+                                      ltm_dtype dtype, void* workspace, size_t workspace_bytes,
+                                      void* stream);
+
+/* One selection step of a beam search: the K best of the W * V continuations
+ * of every request, in descending order, equal ones by the lowest w * V + x:
+ *   total[w, x] = scores[b, w] + logits[b, w, x] - log sum_y exp(logits[b, w, y])
+ * logits: row w of request b at b * batch_stride + w * beam_stride (elements),
+ * V of them contiguous, any alignment; scores: fp32 [B, W], finite or -inf (a
+ * beam that does not exist).  done (uint8 [B, W] or NULL): a finished beam
+ * continues as itself only, its end_token keeping its score and every other
+ * token -inf.  A NaN logit or score counts as -inf, a logit +inf as the largest
+ * float.  Outputs [B, K]: totals (evaluated in 64 bits, stored as fp32), the beam
+ * and the token of each, and with done whether the continuation is finished (its
+ * beam was, or the token is end_token).  W <= 32, K <= 64.
+ * workspace: device memory of ltm_beam_select_workspace bytes, 8-byte aligned. */
+LTM_API ltm_status ltm_beam_select_workspace(int B, int W, int V, int K, size_t* bytes);
+LTM_API ltm_status ltm_beam_select(const void* logits, ltm_dtype dtype, int64_t batch_stride,
+                                   int64_t beam_stride, const float* scores, const uint8_t* done,
+                                   int end_token, int B, int W, int V, int K, float* out_scores,
+                                   int32_t* out_beams, int32_t* out_tokens, uint8_t* out_done,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* Makes the caches of every request's beams follow a selection, in place:
+ *   cache[b * W + w, :, p] <- cache[b * W + beams[b, w], :, p]
+ * for all w at once and p in [first[b], cache_lens[b]) (device int32 [B]; NULL: 0
+ * and max_positions).  Any map is allowed (copies, swaps, cycles); beams that keep
+ * their slot are not touched.  caches: host array of n_caches device pointers to
+ * [B * W, kv_heads, max_positions, row] tensors, row_bytes[i] bytes per row
+ * (a multiple of 4: K or V rows of any type, or an int8 cache's scales),
+ * each listed once.  W <= 32.  A request whose beams hold an index outside
+ * [0, W), or whose range is not inside the cache, is left as it is and the device
+ * error word set to 6. */
+LTM_API ltm_status ltm_kv_cache_reorder(void* const* caches, const int64_t* row_bytes,
+                                        int n_caches, const int32_t* beams, const int32_t* first,
+                                        const int32_t* cache_lens, int B, int W, int kv_heads,
+                                        int64_t max_positions, void* stream);
+
 /* ----------------------------------------------------------------- block -- */
 /* Field-for-field mirror of ltm::transformer::TitanBlockConfig
  * (include/core/transformer/titan_inspired_block.cuh:19-50): same names, same

@@ -36,6 +36,8 @@ enum DeviceErrorCode : int {
   kErrWaitAccum = 3,    // epilogue waited too long for the accumulator
   kErrWaitOther = 4,
   kErrBadCacheLen = 5,  // a per-sequence cache length outside [0, max_positions)
+  kErrBadBeam = 6,      // a beam index outside [0, beams), or a bad range, in a cache reorder
+  kErrBadParent = 7,    // a draft token whose parent does not come before it
 };
 
 #define LTM_CUDA_TRY(expr)                                                              \

@@ -93,6 +93,16 @@ def _declare(L):
         "ltm_memory_store": ([vp, vp, i64, vp, i64, i64, vp, ci, ci, ci, C.c_float, ci, ci, vp], ci),
         "ltm_memory_store_noalloc": ([vp, vp, i64, vp, i64, i64, vp, ci, ci, ci, C.c_float, ci,
                                       ci, vp], ci),
+        "ltm_kv_cache_append": ([vp, vp, vp, vp, ci, vp, vp, vp, vp, i64, vp, vp, ci, ci, ci, ci, vp],
+                                ci),
+        "ltm_kv_cache_read": ([vp, vp, ci, i64, vp, vp, ci, ci, ci, ci, vp, vp], ci),
+        "ltm_tree_attention_workspace": ([ci, ci, ci, ci, ci, C.POINTER(C.c_size_t)], ci),
+        "ltm_tree_attention": ([vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci,
+                                ci, vp, C.c_size_t, vp], ci),
+        "ltm_beam_select_workspace": ([ci, ci, ci, ci, C.POINTER(C.c_size_t)], ci),
+        "ltm_beam_select": ([vp, ci, i64, i64, vp, vp, ci, ci, ci, ci, ci, vp, vp, vp, vp, vp,
+                             C.c_size_t, vp], ci),
+        "ltm_kv_cache_reorder": ([vp, vp, ci, vp, vp, vp, ci, ci, ci, i64, vp], ci),
         "ltm_block_config_default": ([C.POINTER(BlockConfigC)], None),
         "ltm_block_create": ([C.POINTER(BlockConfigC), C.POINTER(QuantConfigC), ci,
                               C.POINTER(vp)], ci),
@@ -459,6 +469,245 @@ def memory_store_noalloc(memory, keys, queries, state, num_heads: int, update_ra
                                           num_heads, update_rate, int(use_attention_scores),
                                           dtype_code(memory.dtype), _stream(stream)))
     return memory
+
+
+# ------------------------------------------------- KV cache, beam search --
+class _Call:
+    """Device and stream of one call: its tensors' device is the current one
+    inside the `with` block, and memory made there for the call is safe on a
+    stream that is not the current one."""
+
+    def __init__(self, t, stream):
+        torch = _torch()
+        self.device = t.device
+        cur = torch.cuda.current_stream(t.device)
+        self.other = stream if stream is not None and stream != cur else None
+        self.stream = C.c_void_p((stream if self.other is not None else cur).cuda_stream)
+        self._guard = None
+
+    def __enter__(self):
+        torch = _torch()
+        if torch.cuda.current_device() != self.device.index:
+            self._guard = torch.cuda.device(self.device)
+            self._guard.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+        return False
+
+    def empty(self, shape, dtype):
+        t = _torch().empty(shape, dtype=dtype, device=self.device)
+        if self.other is not None:
+            t.record_stream(self.other)
+        return t
+
+
+def _bad(msg: str):
+    raise LtmError(ERR_INVALID_ARG, msg)
+
+
+def _check_op(first, tensors, index=(), index_shape=None):
+    """Tensors (None allowed) on `first`'s CUDA device; `index`: contiguous int32
+    tensors of index_shape."""
+    if not first.is_cuda:
+        raise ValueError("ltm_b200 operates on CUDA tensors only")
+    for t in tensors:
+        if t is not None and t.device != first.device:
+            _bad("all tensors must be on one device")
+    for t in index:
+        if t is None:
+            continue
+        if t.device != first.device:
+            _bad("all tensors must be on one device")
+        if t.dtype != _torch().int32 or t.shape != index_shape or not t.is_contiguous():
+            _bad(f"lengths and indices must be contiguous int32 {list(index_shape)}")
+
+
+def _check_cache(cache, scale, what: str):
+    if cache.dim() != 4 or not cache.is_contiguous():
+        _bad(f"{what} must be contiguous [B, kv_heads, max_positions, head_dim]")
+    torch = _torch()
+    if (scale is not None) != (cache.dtype == torch.int8):
+        _bad(f"{what}: int8 caches need scales, others take none")
+    if scale is not None and (scale.dtype != torch.float32 or scale.shape != cache.shape[:3]
+                              or not scale.is_contiguous()):
+        _bad(f"{what}: scales must be contiguous fp32 [B, kv_heads, max_positions]")
+
+
+def _check_pair(k_cache, v_cache, k_scale, v_scale):
+    _check_cache(k_cache, k_scale, "k_cache")
+    _check_cache(v_cache, v_scale, "v_cache")
+    if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+        _bad("k_cache and v_cache must have one shape and type")
+
+
+def _strides3(t, what: str):
+    """Batch, token and head strides of a [B, T, heads, head_dim] view."""
+    s = t.stride()
+    if s[3] != 1:
+        _bad(f"{what} must have unit stride in head_dim")
+    return (C.c_int64 * 3)(s[0], s[1], s[2])
+
+
+def _dp(t):
+    return None if t is None else t.data_ptr()
+
+
+def kv_cache_append(k, v, k_cache, v_cache, cache_lens, k_scale=None, v_scale=None,
+                    num_tokens=None, stream=None) -> None:
+    """Writes T new tokens per sequence into the caches at positions
+    cache_lens[b] .. + T (ltm_kv_cache_append).
+
+    k, v: [B, T, kv_heads, head_dim] (any strides with 16-byte aligned rows, e.g.
+    slices of the fused projection); caches [B, kv_heads, max_positions,
+    head_dim]: int8 with fp32 scales [B, kv_heads, max_positions] (k, v f32, f16
+    or bf16), or of k's type (f16 / bf16).  cache_lens, num_tokens (how many of the
+    T tokens a sequence has): int32 [B].  The lengths are not advanced."""
+    _check_op(k, (v, k_cache, v_cache, k_scale, v_scale), (cache_lens, num_tokens), k.shape[:1])
+    _check_pair(k_cache, v_cache, k_scale, v_scale)
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+        _bad("k and v must both be [B, T, kv_heads, head_dim]")
+    B, T, h, d = k.shape
+    if k_cache.shape[0] != B or k_cache.shape[1] != h or k_cache.shape[3] != d:
+        _bad("the caches do not fit k and v")
+    if k_scale is None and k_cache.dtype != k.dtype:
+        _bad("the caches must be int8 or have k's type")
+    with _Call(k, stream) as c:
+        _check(lib().ltm_kv_cache_append(
+            k.data_ptr(), _strides3(k, "k"), v.data_ptr(), _strides3(v, "v"), dtype_code(k.dtype),
+            k_cache.data_ptr(), v_cache.data_ptr(), _dp(k_scale), _dp(v_scale), k_cache.shape[2],
+            cache_lens.data_ptr(), _dp(num_tokens), B, T, h, d, c.stream))
+
+
+def kv_cache_read(cache, scale, length: int, first=None, cache_lens=None, dtype=None, out=None,
+                  stream=None):
+    """`length` positions of every sequence and head from first[b] (int32 [B];
+    0 when None) on: [B, kv_heads, length, head_dim] (ltm_kv_cache_read).  int8
+    caches give code * scale in `dtype` (f32, f16 or bf16; f32 when None), other caches
+    (scale None) their values.  Positions outside [0, cache_lens[b]) (int32 [B];
+    max_positions when None) give zeros."""
+    _check_op(cache, (scale, out), (first, cache_lens), cache.shape[:1])
+    _check_cache(cache, scale, "cache")
+    if length < 0:
+        _bad("length must not be negative")
+    if dtype is None:
+        dtype = cache.dtype if scale is None else _torch().float32
+    if scale is None and dtype != cache.dtype:
+        _bad("a 16-bit cache is read in its own type")
+    B, h, P, d = cache.shape
+    shape = (B, h, length, d)
+    with _Call(cache, stream) as c:
+        if out is None:
+            out = c.empty(shape, dtype)
+        elif out.shape != shape or out.dtype != dtype or not out.is_contiguous():
+            _bad(f"out must be contiguous {list(shape)} of the read type")
+        _check(lib().ltm_kv_cache_read(cache.data_ptr(), _dp(scale), dtype_code(dtype), P,
+                                       _dp(first), _dp(cache_lens), B, h, d, length,
+                                       out.data_ptr(), c.stream))
+    return out
+
+
+def tree_attention(q, k_cache, v_cache, cache_lens, parents=None, k_scale=None, v_scale=None,
+                   num_tokens=None, out=None, stream=None):
+    """Attention of T <= 64 drafted tokens per sequence (T = 1: a decode step)
+    over a KV cache (ltm_tree_attention): token t of sequence b sees positions
+    [0, cache_lens[b]) and, at cache_lens[b] + a, itself and its ancestors a.
+
+    q: [B, T, heads, head_dim] f16 / bf16 (heads a multiple of the caches'
+    kv_heads); caches of q's type, or int8 with fp32 scales; the drafted tokens
+    have been appended (kv_cache_append).  parents: int32 [B, T], -1 for a root;
+    None for a chain.  num_tokens: int32 [B], how many of the T tokens a sequence
+    has (the others get zeros).  Returns [B, T, heads, head_dim]."""
+    _check_op(q, (k_cache, v_cache, k_scale, v_scale, out), (cache_lens, num_tokens), q.shape[:1])
+    _check_op(q, (), (parents,), q.shape[:2])
+    _check_pair(k_cache, v_cache, k_scale, v_scale)
+    if q.dim() != 4 or k_cache.shape[0] != q.shape[0] or k_cache.shape[3] != q.shape[3]:
+        _bad("q must be [B, T, heads, head_dim] for the caches' B and head_dim")
+    if k_scale is None and k_cache.dtype != q.dtype:
+        _bad("the caches must be int8 or have q's type")
+    B, T, heads, d = q.shape
+    kvh, P = k_cache.shape[1], k_cache.shape[2]
+    L = lib()
+    nbytes = C.c_size_t()
+    _check(L.ltm_tree_attention_workspace(B, T, heads, kvh, d, C.byref(nbytes)))
+    with _Call(q, stream) as c:
+        if out is None:
+            out = c.empty(q.shape, q.dtype)
+        elif out.shape != q.shape or out.dtype != q.dtype:
+            _bad("out must have q's shape and type")
+        ws = c.empty(nbytes.value, _torch().uint8)
+        _check(L.ltm_tree_attention(
+            q.data_ptr(), _strides3(q, "q"), k_cache.data_ptr(), v_cache.data_ptr(), _dp(k_scale),
+            _dp(v_scale), P, cache_lens.data_ptr(), _dp(num_tokens), _dp(parents), out.data_ptr(),
+            _strides3(out, "out"), B, T, heads, kvh, d, dtype_code(q.dtype), ws.data_ptr(),
+            nbytes.value, c.stream))
+    return out
+
+
+def beam_select(logits, scores, num_out: int | None = None, done=None, end_token: int = -1,
+                stream=None):
+    """One selection step of a beam search (ltm_beam_select): logits [B, W, V]
+    (f32 / f16 / bf16, V contiguous), scores fp32 [B, W] (finite, or -inf for a beam
+    that does not exist) -> (scores [B, K] fp32, beams [B, K] int32, tokens [B, K]
+    int32) of the K = num_out (W when None) best continuations, best first.  With
+    `done` (bool [B, W]) finished beams continue as themselves with `end_token`
+    and a fourth output [B, K] bool says which continuations are finished."""
+    torch = _torch()
+    _check_op(logits, (scores, done))
+    if logits.dim() != 3 or logits.stride(2) != 1:
+        _bad("logits must be [B, W, V] with unit stride in V")
+    B, W, V = logits.shape
+    if scores.dtype != torch.float32 or scores.shape != (B, W) or not scores.is_contiguous():
+        _bad("scores must be contiguous fp32 [B, W]")
+    if done is not None and (done.dtype != torch.bool or done.shape != (B, W)
+                             or not done.is_contiguous()):
+        _bad("done must be contiguous bool [B, W]")
+    K = W if num_out is None else num_out
+    L = lib()
+    nbytes = C.c_size_t()
+    _check(L.ltm_beam_select_workspace(B, W, V, K, C.byref(nbytes)))
+    with _Call(logits, stream) as c:
+        s = c.empty((B, K), torch.float32)
+        bt = c.empty((2, B, K), torch.int32)
+        d = c.empty((B, K), torch.bool) if done is not None else None
+        ws = c.empty(nbytes.value, torch.uint8)
+        _check(L.ltm_beam_select(
+            logits.data_ptr(), dtype_code(logits.dtype), logits.stride(0), logits.stride(1),
+            scores.data_ptr(), _dp(done), end_token, B, W, V, K, s.data_ptr(), bt[0].data_ptr(),
+            bt[1].data_ptr(), _dp(d), ws.data_ptr(), nbytes.value, c.stream))
+    return (s, bt[0], bt[1]) if d is None else (s, bt[0], bt[1], d)
+
+
+def kv_cache_reorder(caches, beams, cache_lens=None, first=None, stream=None) -> None:
+    """Makes beams' caches follow a selection, in place (ltm_kv_cache_reorder):
+    cache[b * W + w] <- cache[b * W + beams[b, w]] at positions [first[b],
+    cache_lens[b]).  caches: a list of contiguous [B * W, kv_heads,
+    max_positions, head_dim] tensors (K and V of all layers) and [B * W, kv_heads,
+    max_positions] tensors (int8 caches' scales), each once; beams int32 [B, W];
+    cache_lens, first: int32 [B] (max_positions and 0 when None)."""
+    caches = list(caches)
+    _check_op(beams, caches, (beams,), beams.shape)
+    if beams.dim() != 2:
+        _bad("beams must be int32 [B, W]")
+    B, W = beams.shape
+    _check_op(beams, (), (cache_lens, first), beams.shape[:1])
+    n = len(caches)
+    if n == 0:
+        return
+    lead = caches[0].shape[:3]
+    for t in caches:
+        if t.dim() not in (3, 4) or t.shape[:3] != lead or not t.is_contiguous():
+            _bad("caches must be contiguous [B * W, kv_heads, max_positions(, head_dim)]")
+    if lead[0] != B * W:
+        _bad("caches must have B * W sequences")
+    ptrs = (C.c_void_p * n)(*[t.data_ptr() for t in caches])
+    rows = (C.c_int64 * n)(*[t.element_size() * (t.shape[3] if t.dim() == 4 else 1)
+                             for t in caches])
+    with _Call(beams, stream) as c:
+        _check(lib().ltm_kv_cache_reorder(ptrs, rows, n, beams.data_ptr(), _dp(first),
+                                          _dp(cache_lens), B, W, lead[1], lead[2], c.stream))
 
 
 # --------------------------------------------------------------------- block --
