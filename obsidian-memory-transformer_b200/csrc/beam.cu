@@ -9,15 +9,15 @@
 // is NaN counts as -inf.
 //
 // Every logit is read once (the bound): beam_chunk_kernel gives each CTA up to
-// 8192 logits of one row, held in registers as order-preserving integers.  It
-// takes the chunk's maximum, the sum of exponentials, and its K best by
-// filtering: the smallest of n >= K group maxima is a value that at least K
-// logits reach, and usually few more do (about n * H_n for n groups, 22 for 8
-// beams), so only those are compacted and ranked.  Where too many pass (long
-// runs of equal or masked logits) the K best are taken one by one instead.
-// beam_merge_kernel (one warp per request) merges the chunks' sorted lists by
-// their totals, evaluated in 64 bits because nearly equal totals of different
-// beams decide the order; within a row the order is that of the logits.
+// 8192 logits of one row, held in registers.  It takes the chunk's maximum, the
+// sum of exponentials, and its K best by filtering: the smallest of n >= K group
+// maxima is a value that at least K logits reach, and usually few more do (about
+// n * H_n for n groups, 22 for 8 beams), so only those are compacted and ranked.
+// Where too many pass (long runs of equal or masked logits) the K best are
+// taken one by one instead.  beam_merge_kernel (one CTA per request) evaluates the
+// totals of the chunks' sorted lists in 64 bits, because nearly equal totals of
+// different beams decide the order, and filters and ranks them the same way;
+// within a row the order is that of the logits.
 //
 // The reference's generation loop samples on the host
 // (python_bindings/ltm/inference.py:131-260).
@@ -34,21 +34,22 @@ constexpr int kChunk = kBThreads * kPer;     // logits per CTA
 constexpr int kMaxCand = 1024;               // candidates ranked in shared memory
 constexpr int kMaxK = 64;
 constexpr int kMaxW = 32;
-constexpr uint32_t kNone = 0u;               // not a logit (past the row's end)
 constexpr uint32_t kNegInf = 0x007fffffu;    // ordered(-inf)
 
 // Order-preserving bits of a float: larger float <=> larger integer.
 __device__ __forceinline__ uint32_t ordered(float x) {
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(x + 0.0f);  // -0 -> +0: equal values have equal keys
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float unordered(uint32_t u) {
   return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
-__device__ __forceinline__ uint32_t logit_key(float x) {
-  if (!(x == x)) return kNegInf;
-  x = fminf(x, 3.402823466e38f) + 0.0f;  // -0 -> +0: equal values have equal keys
-  return ordered(x);
+// fmaxf gives the other operand for a NaN.
+__device__ __forceinline__ float logit_value(float x) {
+  return fminf(fmaxf(x, -INFINITY), 3.402823466e38f);
+}
+__device__ __forceinline__ uint64_t list_key(float x, int token) {
+  return (static_cast<uint64_t>(ordered(x)) << 32) | ~static_cast<uint32_t>(token);
 }
 
 struct BeamPartial {
@@ -58,109 +59,130 @@ struct BeamPartial {
 // Workspace: [rows, nchunk] BeamPartial, then [rows, nchunk, K] sorted keys
 // (ordered logit << 32 | ~token; 0 = none).
 template <class T>
-__global__ void __launch_bounds__(kBThreads)
+__global__ void __launch_bounds__(kBThreads, 3)
     beam_chunk_kernel(const T* __restrict__ logits, int64_t ldb, int64_t ldw,
                       const float* __restrict__ scores, const uint8_t* __restrict__ done, int end,
                       int W, int V, int K, int nchunk, int groups, BeamPartial* __restrict__ stats,
                       uint64_t* __restrict__ lists) {
-  __shared__ uint32_t s_group[kMaxK];
+  __shared__ float s_group[kBThreads];
   __shared__ float s_sum[kBThreads / 32];
   __shared__ uint64_t s_cand[kMaxCand];
   __shared__ uint64_t s_best[kBThreads / 32];
   __shared__ int s_count;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x / nchunk, chunk = blockIdx.x % nchunk;
-  const int b = row / W, w = row % W;
+  const int row = blockIdx.x / nchunk, chunk = blockIdx.x - row * nchunk;
+  const int b = row / W, w = row - b * W;
   const int c0 = chunk * kChunk, c1 = min(V, c0 + kChunk);
   const int64_t item = blockIdx.x;
   uint64_t* list = lists + item * K;
-  const bool is_done = done != nullptr && done[row] != 0;
-  const float score = scores[row];
 
+  // ---- load: 16-byte vectors of the row's aligned span, all in flight at once; then the
+  // vectors that the chunk's ends cut, element by element
+  constexpr int N = 16 / sizeof(T);  // logits per vector
+  constexpr int NV = kPer / N;       // vectors per thread
+  const T* r = logits + b * ldb + w * ldw;
+  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
+  // token of element j of vector i: t0 + i * 256 * N + j
+  const int t0 = c0 - shift + tid * N;
+  uint4 raw[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int x = t0 + i * kBThreads * N;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (x >= c0 && x + N <= c1) raw[i] = __ldg(reinterpret_cast<const uint4*>(r + x));
+  }
+  const float score = scores[row];
+  const bool is_done = done != nullptr && done[row] != 0;
   if (is_done || !(score > -INFINITY)) {
     // no logit matters: the end token (if this chunk has it), then the lowest tokens
     const bool has = is_done && score > -INFINITY && end >= c0 && end < c1;
     if (tid < K) {
-      int x = tid;
-      uint32_t u = kNegInf;
+      int x = c0 + tid;
+      float y = -INFINITY;
       if (has) {
         if (tid == 0) {
-          x = end - c0;
-          u = ordered(0.0f);
-        } else {
-          x = tid - 1 < end - c0 ? tid - 1 : tid;
+          x = end;
+          y = 0.0f;
+        } else if (x - 1 < end) {
+          x -= 1;
         }
       }
-      list[tid] = c0 + x < c1
-                      ? (static_cast<uint64_t>(u) << 32) | ~static_cast<uint32_t>(c0 + x)
-                      : 0ull;
+      list[tid] = x < c1 ? list_key(y, x) : 0ull;
     }
     if (tid == 0) stats[item] = BeamPartial{0.0f, 1.0f};
     return;
   }
-
-  // ---- load: 16-byte vectors of the row's aligned span, the ragged ends one by one
-  constexpr int N = 16 / sizeof(T);       // logits per vector
-  constexpr int NV = kPer / N;            // vectors per thread
-  const T* r = logits + b * ldb + w * ldw;
-  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
-  uint32_t u[kPer];
-  // token of element j of vector i: c0 - shift + (i * 256 + tid) * N + j
-  const int t0 = c0 - shift + tid * N;
+  if (tid == 0) s_count = 0;
+  // elements that are not there are -inf here and left out by their index below
+  float v[kPer];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const T* e = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[i * N + j] = logit_value(to_f32(e[j]));
+  }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int x = t0 + i * kBThreads * N;
-    if (x >= c0 && x + N <= c1) {
-      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(r + x));
-      const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-      for (int j = 0; j < N; ++j) u[i * N + j] = logit_key(to_f32(e[j]));
-    } else {
+    if (!(x >= c0 && x + N <= c1)) {
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        u[i * N + j] = (x + j >= c0 && x + j < c1) ? logit_key(to_f32(r[x + j])) : kNone;
+        v[i * N + j] = (x + j >= c0 && x + j < c1) ? logit_value(to_f32(r[x + j])) : -INFINITY;
     }
   }
   // a misaligned row's last `shift` logits lie past the vectors: one per thread
-  uint32_t extra = kNone;
   const int xe = c0 - shift + kChunk + tid;
-  if (tid < shift && xe < c1) extra = logit_key(to_f32(r[xe]));
+  const bool has_extra = tid < shift && xe < c1;
+  const float extra = has_extra ? logit_value(to_f32(r[xe])) : -INFINITY;
 
-  uint32_t um = extra;
+  float vm[NV];  // maximum of each vector
+  float tm = extra;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) um = max(um, u[i]);
-  // maxima of `groups` groups of consecutive lanes (8 warps down to 4 lanes each)
-  const int gl = kBThreads / groups;
-  for (int o = gl >> 1; o > 0; o >>= 1) um = max(um, __shfl_xor_sync(0xffffffffu, um, o));
-  if (tid % gl == 0) s_group[tid / gl] = um;
-  if (tid == 0) s_count = 0;
-  __syncthreads();
-  uint32_t hi = kNone, tau = 0xffffffffu;
-  for (int i = 0; i < groups; ++i) {
-    const uint32_t g = s_group[i];
-    hi = max(hi, g);
-    tau = min(tau, g);
+  for (int i = 0; i < NV; ++i) {
+    vm[i] = v[i * N];
+#pragma unroll
+    for (int j = 1; j < N; ++j) vm[i] = fmaxf(vm[i], v[i * N + j]);
+    tm = fmaxf(tm, vm[i]);
   }
-  if (tau == kNone) tau = 1u;
-  const float m = unordered(hi);
-  const float ref = hi <= kNegInf ? 0.0f : m;
-  float sum = 0.0f;
-  auto visit = [&](uint32_t key, int x) {
-    if (key > kNegInf) sum += __expf(unordered(key) - ref);
-    if (key >= tau) {
+  // maxima of the groups of equal tid % groups (so that a short chunk fills them all)
+  float gm = tm;
+  for (int o = 16; o >= groups; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+  s_group[tid] = gm;
+  __syncthreads();
+  float g0 = -INFINITY, g1 = -INFINITY;  // groups lane and lane + 32 (mod groups)
+#pragma unroll
+  for (int i = 0; i < kBThreads / 32; i += 2) {
+    g0 = fmaxf(g0, s_group[i * 32 + lane]);
+    g1 = fmaxf(g1, s_group[i * 32 + 32 + lane]);
+  }
+  if (groups <= 32) g0 = g1 = fmaxf(g0, g1);
+  const float m = unordered(__reduce_max_sync(0xffffffffu, ordered(fmaxf(g0, g1))));
+  const float tau = unordered(__reduce_min_sync(0xffffffffu, ordered(fminf(g0, g1))));
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float sum = __expf(extra - ref);
+  auto offer = [&](float y, int x) {
+    if (y >= tau && x >= c0 && x < c1) {
       const int at = atomicAdd(&s_count, 1);
-      if (at < kMaxCand) s_cand[at] = (static_cast<uint64_t>(key) << 32) | ~static_cast<uint32_t>(x);
+      if (at < kMaxCand) s_cand[at] = list_key(y, x);
     }
   };
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) visit(u[i], t0 + (i / N) * kBThreads * N + i % N);
-  visit(extra, xe);
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum += __expf(v[i * N + j] - ref);
+    if (vm[i] >= tau) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) offer(v[i * N + j], t0 + i * kBThreads * N + j);
+    }
+  }
+  if (has_extra) offer(extra, xe);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) s_sum[warp] = sum;
   __syncthreads();
   if (tid == 0) {
     float t = 0.0f;
+#pragma unroll
     for (int i = 0; i < kBThreads / 32; ++i) t += s_sum[i];
     stats[item] = BeamPartial{m, t};
   }
@@ -169,6 +191,7 @@ __global__ void __launch_bounds__(kBThreads)
     for (int i = tid; i < n; i += kBThreads) {
       const uint64_t mine = s_cand[i];
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < n; ++j) rank += s_cand[j] > mine;
       if (rank < K) list[rank] = mine;
     }
@@ -179,18 +202,19 @@ __global__ void __launch_bounds__(kBThreads)
   uint64_t last = ~0ull;
   for (int kk = 0; kk < K; ++kk) {
     uint64_t best = 0ull;
-    auto look = [&](uint32_t key, int x) {
-      const uint64_t full = (static_cast<uint64_t>(key) << 32) | ~static_cast<uint32_t>(x);
-      if (key != kNone && full < last && full > best) best = full;
+    auto look = [&](float y, int x) {
+      const uint64_t full = list_key(y, x);
+      if (x >= c0 && x < c1 && full < last && full > best) best = full;
     };
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) look(u[i], t0 + (i / N) * kBThreads * N + i % N);
-    look(extra, xe);
+    for (int i = 0; i < kPer; ++i) look(v[i], t0 + (i / N) * kBThreads * N + i % N);
+    if (has_extra) look(extra, xe);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
     __syncthreads();
     if (lane == 0) s_best[warp] = best;
     __syncthreads();
+#pragma unroll
     for (int i = 0; i < kBThreads / 32; ++i) best = max(best, s_best[i]);
     if (tid == 0) list[kk] = best;
     last = best;
@@ -207,95 +231,150 @@ __device__ __forceinline__ double unordered64(uint64_t u) {
       static_cast<long long>((u >> 63) ? (u & 0x7fffffffffffffffull) : ~u));
 }
 
-__device__ __forceinline__ uint64_t warp_max64(uint64_t v) {
-  const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(v >> 32));
-  const uint32_t lo = __reduce_max_sync(
-      0xffffffffu, static_cast<uint32_t>(v >> 32) == hi ? static_cast<uint32_t>(v) : 0u);
-  return (static_cast<uint64_t>(hi) << 32) | lo;
+// A continuation: larger total first, then the lower flat index.
+struct Total {
+  uint64_t t;  // ordered bits of the total; 0 = none
+  uint64_t f;  // beam * V + token
+};
+__device__ __forceinline__ bool before(const Total& a, const Total& b) {
+  return a.t > b.t || (a.t == b.t && a.f < b.f);
 }
 
-// One warp per request: lane l owns the lists l, l + 32, ... (row-major over
-// beams and chunks) and keeps the best head among them.
-__global__ void __launch_bounds__(32)
+constexpr int kMergeCand = 512;  // continuations ranked in shared memory
+
+// One CTA per request.  Its W * nchunk lists are sorted, so the best d entries
+// of every list, d = ceil(K / lists), hold K continuations: the least of those
+// d-th entries bounds the K-th best from below, more sharply by the K-th of
+// the lists' heads where there are K of them.  What reaches the bound is ranked;
+// where that is more than shared memory takes, the K best are taken one by one.
+__global__ void __launch_bounds__(kBThreads)
     beam_merge_kernel(const float* __restrict__ scores, const uint8_t* __restrict__ done, int end,
                       int W, int V, int K, int nchunk, const BeamPartial* __restrict__ stats,
                       const uint64_t* __restrict__ lists, float* __restrict__ out_scores,
                       int* __restrict__ out_beams, int* __restrict__ out_tokens,
                       uint8_t* __restrict__ out_done) {
-  extern __shared__ int s_pos[];  // next entry of every list
   __shared__ double s_m[kMaxW], s_ls[kMaxW], s_score[kMaxW];
   __shared__ uint8_t s_done[kMaxW];
-  const int b = blockIdx.x, lane = threadIdx.x;
+  __shared__ Total s_cand[kMergeCand];
+  __shared__ Total s_best[kBThreads / 32];
+  __shared__ uint64_t s_low[kBThreads / 32];
+  __shared__ int s_count;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int nlists = W * nchunk;
-  for (int i = lane; i < nlists; i += 32) s_pos[i] = 0;
-  // a row's maximum and sum over its chunks
-  if (lane < W) {
-    const int row = b * W + lane;
-    const BeamPartial* st = stats + static_cast<int64_t>(row) * nchunk;
-    float m = -INFINITY;
-    for (int c = 0; c < nchunk; ++c) m = fmaxf(m, st[c].m);
-    double sum = 0.0;
-    for (int c = 0; c < nchunk; ++c)
-      if (st[c].m > -INFINITY)
-        sum += static_cast<double>(st[c].sum) * exp(static_cast<double>(st[c].m) - m);
-    const float sc = scores[row];
-    s_m[lane] = m;
-    s_ls[lane] = log(sum);
-    s_score[lane] = sc == sc ? sc : -INFINITY;
-    s_done[lane] = done != nullptr && done[row] != 0;
-  }
-  __syncwarp();
   const uint64_t* mine = lists + static_cast<int64_t>(b) * nlists * K;
-  // total of a list's entry as ordered bits; 0 = the list is used up
-  auto total_of = [&](int l, int pos) -> uint64_t {
-    if (pos >= K) return 0ull;
+  if (tid == 0) s_count = 0;
+  // a row's maximum and sum over its chunks: one warp per row
+  for (int w = warp; w < W; w += kBThreads / 32) {
+    const int row = b * W + w;
+    const float sc = scores[row];
+    float m = -INFINITY;
+    double sum = 0.0;
+    for (int c0 = 0; c0 < nchunk; c0 += 32) {
+      BeamPartial st{-INFINITY, 0.0f};
+      if (c0 + lane < nchunk) st = stats[static_cast<int64_t>(row) * nchunk + c0 + lane];
+      float mm = st.m;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+      mm = fmaxf(mm, m);
+      double part = st.m == -INFINITY ? 0.0 : static_cast<double>(st.sum * expf(st.m - mm));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+      sum = (m == -INFINITY ? 0.0 : sum * static_cast<double>(expf(m - mm))) + part;
+      m = mm;
+    }
+    if (lane == 0) {
+      s_m[w] = m;
+      s_ls[w] = log(sum);
+      s_score[w] = sc == sc ? sc : -INFINITY;
+      s_done[w] = done != nullptr && done[row] != 0;
+    }
+  }
+  __syncthreads();
+  auto entry = [&](int l, int pos) -> Total {
     const uint64_t key = mine[static_cast<int64_t>(l) * K + pos];
-    if (key == 0ull) return 0ull;
+    if (key == 0ull) return Total{0ull, ~0ull};
     const uint32_t u = static_cast<uint32_t>(key >> 32);
     const int w = l / nchunk;
     double t = -INFINITY;
     if (u > kNegInf && s_score[w] > -INFINITY)
       t = s_done[w] ? s_score[w]
                     : s_score[w] + ((static_cast<double>(unordered(u)) - s_m[w]) - s_ls[w]);
-    return ordered64(t);
+    return Total{ordered64(t), static_cast<uint64_t>(w) * V + ~static_cast<uint32_t>(key)};
   };
-  auto flat_of = [&](int l, int pos) -> uint64_t {
-    const uint64_t key = mine[static_cast<int64_t>(l) * K + pos];
-    return static_cast<uint64_t>(l / nchunk) * V + static_cast<uint32_t>(~static_cast<uint32_t>(key));
+  auto put = [&](int k, const Total& x) {
+    const int w = static_cast<int>(x.f / V), tok = static_cast<int>(x.f - static_cast<uint64_t>(w) * V);
+    const int64_t o = static_cast<int64_t>(b) * K + k;
+    out_scores[o] = static_cast<float>(unordered64(x.t));
+    out_beams[o] = w;
+    out_tokens[o] = tok;
+    if (out_done) out_done[o] = s_done[w] || tok == end;
   };
-  uint64_t best = 0ull, flat = ~0ull;
-  int from = -1;
-  auto rescan = [&] {
-    best = 0ull;
-    flat = ~0ull;
-    from = -1;
-    for (int l = lane; l < nlists; l += 32) {
-      const uint64_t t = total_of(l, s_pos[l]);
-      if (t == 0ull) continue;
-      const uint64_t f = flat_of(l, s_pos[l]);
-      if (t > best || (t == best && f < flat)) {
-        best = t;
-        flat = f;
-        from = l;
-      }
+  // ---- the bound (ordered bits of a total that at least K continuations reach)
+  uint64_t low = ~0ull;
+  if (nlists >= K && nlists <= kMergeCand) {
+    for (int l = tid; l < nlists; l += kBThreads) s_cand[l] = entry(l, 0);
+    __syncthreads();
+    for (int l = tid; l < nlists; l += kBThreads) {
+      const Total x = s_cand[l];
+      int rank = 0;
+#pragma unroll 4
+      for (int j = 0; j < nlists; ++j) rank += before(s_cand[j], x);
+      if (rank == K - 1) s_low[0] = x.t;
     }
-  };
-  rescan();
+    __syncthreads();
+    low = s_low[0];
+    __syncthreads();  // s_cand is written again below
+  } else {
+    const int d = min(K, (K + nlists - 1) / nlists) - 1;
+    for (int l = tid; l < nlists; l += kBThreads) low = min(low, entry(l, d).t);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+    if (lane == 0) s_low[warp] = low;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kBThreads / 32; ++i) low = min(low, s_low[i]);
+  }
+  low = max(low, static_cast<uint64_t>(1));  // a list without that many entries bounds nothing
+  const int entries = nlists * K;
+  for (int i = tid; i < entries; i += kBThreads) {
+    const Total x = entry(i / K, i % K);
+    if (x.t >= low) {
+      const int at = atomicAdd(&s_count, 1);
+      if (at < kMergeCand) s_cand[at] = x;
+    }
+  }
+  __syncthreads();
+  const int n = s_count;
+  if (n <= kMergeCand) {
+    for (int i = tid; i < n; i += kBThreads) {
+      const Total x = s_cand[i];
+      int rank = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) rank += before(s_cand[j], x);
+      if (rank < K) put(rank, x);
+    }
+    return;
+  }
+  Total last{~0ull, 0ull};
   for (int k = 0; k < K; ++k) {
-    const uint64_t top = warp_max64(best);
-    // of the lanes that hold it, the lowest flat index
-    const uint64_t inv = (best == top && from >= 0) ? ~flat : 0ull;
-    const uint64_t win = warp_max64(inv);
-    if (inv == win && win != 0ull) {
-      const int w = static_cast<int>(flat / V), x = static_cast<int>(flat - static_cast<uint64_t>(w) * V);
-      const int64_t o = static_cast<int64_t>(b) * K + k;
-      out_scores[o] = static_cast<float>(unordered64(best));
-      out_beams[o] = w;
-      out_tokens[o] = x;
-      if (out_done) out_done[o] = s_done[w] || x == end;
-      s_pos[from] += 1;
-      rescan();
+    Total best{0ull, ~0ull};
+    for (int i = tid; i < entries; i += kBThreads) {
+      const Total x = entry(i / K, i % K);
+      if (before(last, x) && before(x, best)) best = x;
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const Total y{__shfl_xor_sync(0xffffffffu, best.t, o), __shfl_xor_sync(0xffffffffu, best.f, o)};
+      if (before(y, best)) best = y;
+    }
+    __syncthreads();
+    if (lane == 0) s_best[warp] = best;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kBThreads / 32; ++i)
+      if (before(s_best[i], best)) best = s_best[i];
+    if (tid == 0) put(k, best);
+    last = best;
   }
 }
 
@@ -355,7 +434,7 @@ extern "C" ltm_status ltm_beam_select(const void* logits, ltm_dtype dtype, int64
           K, nchunk, groups, stats, lists);
     });
     check_launch("beam_chunk_kernel", st);
-    beam_merge_kernel<<<B, 32, static_cast<size_t>(W) * nchunk * sizeof(int), st>>>(
+    beam_merge_kernel<<<B, kBThreads, 0, st>>>(
         scores, done, end_token, W, V, K, nchunk, stats, lists, out_scores, out_beams, out_tokens,
         out_done);
     check_launch("beam_merge_kernel", st);

@@ -24,8 +24,10 @@
 namespace ltm_b200 {
 namespace {
 
-constexpr int kWarps = 8;   // warps per CTA of the write and read kernels
-constexpr int kRowsFly = 4;  // rows in flight per lane group
+constexpr int kWarps = 8;    // warps per CTA of the write and read kernels
+constexpr int kVals = 16;    // values of a row per lane
+constexpr int kRowsFly = 2;  // rows in flight per lane group (write)
+constexpr int kReadFly = 4;  // rows in flight per lane group (read)
 
 struct RowStrides {
   int64_t b, t, h;  // elements between batches, tokens, heads
@@ -43,67 +45,128 @@ __device__ __forceinline__ bool seq_span(const int* lens, const int* num_tokens,
   return ok;
 }
 
-// One row of a lane group: codes and scale of V values per lane.  All 32 lanes
-// call it (lanes without a row pass zeros).  abs_bits: the largest |x| of the
-// row as bits, where an infinity or a NaN compares above every finite value.
-template <int V>
-__device__ __forceinline__ float quant_row(const float (&v)[V], uint32_t abs_bits,
-                                           int8_t (&out)[V]) {
-  const bool bad = abs_bits >= 0x7f800000u;
-  const float amax = bad ? 0.0f : __uint_as_float(abs_bits);
-  const float s = __fdiv_rn(amax, 127.0f);
-  // a reciprocal of a scale this small overflows: such rows take the division
-  const bool tiny = s < 1e-37f;
-  float w[V];
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Scale and codes of one row: 16 values per lane, packed to four words.  All 32
+// lanes call it (lanes without a row pass zeros).  abs_bits: the row's largest
+// |x| as bits, where an infinity or a NaN compares above every finite value.
+//
+// The scale is the IEEE quotient amax / 127, by Markstein's correction of the
+// product with the rounded reciprocal (q = a y, q + (a - 127 q) y with fused
+// multiply-adds; compared with the division for every mantissa on the CPU); amax
+// below 2^-100, where the correction could underflow, is divided.
+// The quotients are estimated with an approximate reciprocal (relative error
+// 2^-23, another 2^-24 by the product) and rounded by adding 1.5 * 2^23: an
+// estimate of |t| <= 127.5 is off by at most 2.3e-5, the IEEE quotient by 0.8e-5,
+// so both round alike unless the estimate is within 2^-14 of a tie; such values
+// (6% of the warps' rows have one) take the division and round half away from zero.
+__device__ __forceinline__ float quant_row16(const float (&v)[kVals], uint32_t abs_bits,
+                                             uint32_t (&code)[kVals / 4]) {
+  constexpr float kShift = 12582912.0f;            // 1.5 * 2^23
+  constexpr float kTie = 0.5f - 6.103515625e-5f;   // 0.5 - 2^-14
+  constexpr float kY = 1.0f / 127.0f;
+  const float amax = __uint_as_float(abs_bits);
+  const bool bad = abs_bits >= 0x7f800000u, tiny = amax < 7.9e-31f;
+  float s = amax * kY;
+  s = fmaf(fmaf(-s, 127.0f, amax), kY, s);
+  if (tiny) s = __fdiv_rn(amax, 127.0f);
+  const float inv = (bad || tiny) ? 0.0f : rcp_approx(s);
+  const uint64_t inv2 = f2_pack(inv, inv), shift2 = f2_pack(kShift, kShift);
+  float big[kVals], off[kVals];
+  bool near_tie = false;
 #pragma unroll
-  for (int i = 0; i < V; ++i) w[i] = (bad || tiny) ? 0.0f : v[i];
-  quant_i8_exact_warp<V>(w, tiny ? 0.0f : s, tiny ? 0.0f : recip_or_zero(s), out);
-  if (tiny && s > 0.0f && !bad) {
+  for (int i = 0; i < kVals; i += 2) {
+    const uint64_t t = f2_mul(f2_pack(v[i], v[i + 1]), inv2);
+    const uint64_t b = f2_add(t, shift2);
+    f2_unpack(f2_sub(t, f2_sub(b, shift2)), off[i], off[i + 1]);
+    f2_unpack(b, big[i], big[i + 1]);
+    near_tie |= (fabsf(off[i]) >= kTie) | (fabsf(off[i + 1]) >= kTie);
+  }
+  const bool divide = tiny && s > 0.0f;
+  if ((near_tie || divide) && !bad) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float r = roundf(__fdiv_rn(v[i], s));
-      out[i] = static_cast<int8_t>(static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f)));
-    }
+    for (int i = 0; i < kVals; ++i)
+      if (divide || fabsf(off[i]) >= kTie) {
+        const float r = fminf(fmaxf(roundf(__fdiv_rn(v[i], s)), -127.0f), 127.0f);
+        big[i] = r + kShift;
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < kVals / 4; ++i) {  // the low byte holds the code
+    const uint32_t lo = __byte_perm(__float_as_uint(big[4 * i]), __float_as_uint(big[4 * i + 1]), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(big[4 * i + 2]), __float_as_uint(big[4 * i + 3]), 0x0040);
+    code[i] = bad ? 0u : __byte_perm(lo, hi, 0x5410);
   }
   return bad ? __int_as_float(0x7fc00000) : s;
 }
 
-// New tokens into the caches.  A warp takes kRowsFly * (32 / group) consecutive
-// tokens of one head, K or V: its int8 rows are then one contiguous block and
-// its scales whole 32-byte sectors; neighbouring warps take neighbouring heads
-// of the same tokens, so that the reads cover whole projection rows.
+// Bits of the largest |x| of a 16-byte vector.
+template <class T>
+__device__ __forceinline__ uint32_t abs_max_bits(const uint4& raw) {
+  if constexpr (sizeof(T) == 4) {
+    return max(max(raw.x & 0x7fffffffu, raw.y & 0x7fffffffu),
+               max(raw.z & 0x7fffffffu, raw.w & 0x7fffffffu));
+  } else {  // two 16-bit patterns a word: without the sign they compare as integers
+    return __vmaxu2(__vmaxu2(raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu),
+                         __vmaxu2(raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu));
+  }
+}
+// The larger half of a pair, as the bits of its fp32 value.
+template <class T>
+__device__ __forceinline__ uint32_t widen_bits(uint32_t m) {
+  if constexpr (sizeof(T) == 4) {
+    return m;
+  } else {
+    const uint32_t h = max(m & 0xffffu, m >> 16);
+    const uint16_t u = static_cast<uint16_t>(h);
+    return __float_as_uint(to_f32(*reinterpret_cast<const T*>(&u)));
+  }
+}
+
+// New tokens into the caches.  Bound by memory (input read once, codes and scales
+// written once).  A lane holds 16 values of a row (two or four 16-byte pieces a
+// group's width apart, so that loads and stores are contiguous over the group),
+// a group of D / 16 lanes a row; a warp takes kRowsFly * 32 / group
+// consecutive tokens of one head, K or V, so that its int8 rows are one
+// contiguous block and its scales whole 32-byte sectors; neighbouring warps take
+// neighbouring heads of the same tokens: the reads cover whole projection rows.
 template <class T, int D, bool Q8>
 __global__ void __launch_bounds__(kWarps * 32)
     cache_append_kernel(const T* __restrict__ k, RowStrides sk, const T* __restrict__ v,
                         RowStrides sv, void* __restrict__ kc, void* __restrict__ vc,
                         float* __restrict__ ks, float* __restrict__ vs, int64_t P,
-                        const int* __restrict__ lens, const int* __restrict__ num_tokens, int B,
-                        int Tn, int heads, int tgroups, int64_t tasks, int* err) {
-  constexpr int V = 16 / sizeof(T);   // values per lane and row
-  constexpr int G = D / V;            // lanes per row
+                        const int* __restrict__ lens, const int* __restrict__ num_tokens, int Tn,
+                        int heads, int tgroups, int* err) {
+  constexpr int N = 16 / sizeof(T);   // values per piece
+  constexpr int NP = kVals / N;       // pieces per lane
+  constexpr int G = D / kVals;        // lanes per row
   constexpr int RP = 32 / G;          // rows per warp and step
-  constexpr int TOK = RP * kRowsFly;  // tokens per warp task
+  constexpr int TOK = RP * kRowsFly;  // tokens per warp
   const int lane = threadIdx.x & 31;
-  const int64_t task = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  if (task >= tasks) return;
-  const int h = static_cast<int>(task % heads);
-  int64_t rest = task / heads;
-  const bool is_v = rest & 1;
-  rest >>= 1;
-  const int tg = static_cast<int>(rest % tgroups), b = static_cast<int>(rest / tgroups);
+  const int hv = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);  // K heads, then V heads
+  if (hv >= 2 * heads) return;
+  const bool is_v = hv >= heads;
+  const int h = is_v ? hv - heads : hv;
+  const int b = blockIdx.x / tgroups, tg = blockIdx.x - b * tgroups;
   int len, n;
   const bool ok = seq_span(lens, num_tokens, b, Tn, P, len, n,
-                           (tg == 0 && h == 0 && !is_v && lane == 0) ? err : nullptr);
+                           (tg == 0 && hv == 0 && lane == 0) ? err : nullptr);
   if (!ok) return;
   const T* src = (is_v ? v + b * sv.b + h * sv.h : k + b * sk.b + h * sk.h);
   const int64_t st = is_v ? sv.t : sk.t;
   const int sub = lane / G, gl = lane % G;
-  uint4 raw[kRowsFly];
+  uint4 raw[kRowsFly][NP];
 #pragma unroll
   for (int j = 0; j < kRowsFly; ++j) {
     const int t = tg * TOK + j * RP + sub;
-    raw[j] = make_uint4(0, 0, 0, 0);
-    if (t < n) raw[j] = __ldg(reinterpret_cast<const uint4*>(src + t * st) + gl);
+    const uint4* at = reinterpret_cast<const uint4*>(src + t * st) + gl;
+#pragma unroll
+    for (int q = 0; q < NP; ++q)
+      raw[j][q] = t < n ? __ldg(at + q * G) : make_uint4(0, 0, 0, 0);
   }
   const int64_t row0 = (static_cast<int64_t>(b) * heads + h) * P + len;
 #pragma unroll
@@ -111,75 +174,84 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int t = tg * TOK + j * RP + sub;
     if (tg * TOK + j * RP >= n) break;  // uniform over the warp
     if constexpr (Q8) {
-      const T* e = reinterpret_cast<const T*>(&raw[j]);
-      float x[V];
+      float x[kVals];
       uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        x[i] = to_f32(e[i]);
-        m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+      for (int q = 0; q < NP; ++q) {
+        const uint32_t a = abs_max_bits<T>(raw[j][q]);
+        if constexpr (sizeof(T) == 4) m = max(m, a);
+        else m = __vmaxu2(m, a);
+        const T* e = reinterpret_cast<const T*>(&raw[j][q]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[q * N + i] = to_f32(e[i]);
       }
 #pragma unroll
-      for (int o = G / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      int8_t out[V];
-      const float s = quant_row<V>(x, m, out);
+      for (int o = G / 2; o > 0; o >>= 1) {
+        const uint32_t a = __shfl_xor_sync(0xffffffffu, m, o);
+        if constexpr (sizeof(T) == 4) m = max(m, a);
+        else m = __vmaxu2(m, a);
+      }
+      uint32_t code[kVals / 4];
+      const float s = quant_row16(x, widen_bits<T>(m), code);
       if (t < n) {
-        int8_t* dst = static_cast<int8_t*>(is_v ? vc : kc) + (row0 + t) * D + gl * V;
-        if constexpr (V == 8)
-          *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(out);
-        else
-          *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(out);
+        int8_t* dst = static_cast<int8_t*>(is_v ? vc : kc) + (row0 + t) * D + gl * N;
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+          if constexpr (N == 8)
+            *reinterpret_cast<uint2*>(dst + q * G * N) = make_uint2(code[2 * q], code[2 * q + 1]);
+          else
+            *reinterpret_cast<uint32_t*>(dst + q * G * N) = code[q];
+        }
         if (gl == 0) (is_v ? vs : ks)[row0 + t] = s;
       }
     } else {
-      if (t < n)
-        reinterpret_cast<uint4*>(static_cast<T*>(is_v ? vc : kc) + (row0 + t) * D)[gl] = raw[j];
+      if (t < n) {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(is_v ? vc : kc) + (row0 + t) * D) + gl;
+#pragma unroll
+        for (int q = 0; q < NP; ++q) dst[q * G] = raw[j][q];
+      }
     }
   }
 }
 
 // Rows [first_b, first_b + n) of every head back as O values; positions
-// outside [0, min(P, len_b)) give zeros.  A lane holds 16 codes (or 8 values of
-// a 16-bit cache, copied).
+// outside [0, min(P, len_b)) give zeros.  Bound by memory.  A lane holds 16 codes
+// (or 8 values of a 16-bit cache, copied).
 template <class O, int D, bool Q8>
 __global__ void __launch_bounds__(kWarps * 32)
     cache_read_kernel(const void* __restrict__ cache, const float* __restrict__ scale, int64_t P,
                       const int* __restrict__ first, const int* __restrict__ lens, int heads,
-                      int n, int groups, int64_t tasks, O* __restrict__ out) {
+                      int n, O* __restrict__ out) {
   constexpr int V = Q8 ? 16 : 8;
   constexpr int G = D / V;
   constexpr int RP = 32 / G;
-  constexpr int ROWS = RP * kRowsFly;
+  constexpr int ROWS = RP * kReadFly;
   const int lane = threadIdx.x & 31;
-  const int64_t task = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  if (task >= tasks) return;
-  const int g = static_cast<int>(task % groups);
-  const int64_t bh = task / groups;
-  const int b = static_cast<int>(bh / heads);
+  const int bh = blockIdx.x;
+  const int i0 = (blockIdx.y * kWarps + (threadIdx.x >> 5)) * ROWS;
+  if (i0 >= n) return;
+  const int b = bh / heads;
   const int64_t p0 = first ? first[b] : 0;
   const int64_t end = lens ? min(P, static_cast<int64_t>(lens[b])) : P;
   const int sub = lane / G, gl = lane % G;
-  uint4 raw[kRowsFly];
-  float s[kRowsFly];
+  uint4 raw[kReadFly];
+  float s[kReadFly];
 #pragma unroll
-  for (int j = 0; j < kRowsFly; ++j) {
-    const int i = g * ROWS + j * RP + sub;
+  for (int j = 0; j < kReadFly; ++j) {
+    const int i = i0 + j * RP + sub;
     const int64_t p = p0 + i;
-    raw[j] = make_uint4(0, 0, 0, 0);
-    s[j] = 0.0f;
-    if (i < n && p >= 0 && p < end) {
-      const int64_t row = bh * P + p;
-      raw[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) +
-                                                    row * D * (Q8 ? 1 : 2)) +
-                     gl);
-      if constexpr (Q8) s[j] = __ldg(scale + row);
-    }
+    const bool live = i < n && p >= 0 && p < end;
+    const int64_t row = bh * P + p;
+    raw[j] = live ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) +
+                                                         row * D * (Q8 ? 1 : 2)) + gl)
+                  : make_uint4(0, 0, 0, 0);
+    s[j] = Q8 && live ? __ldg(scale + row) : 0.0f;
   }
 #pragma unroll
-  for (int j = 0; j < kRowsFly; ++j) {
-    const int i = g * ROWS + j * RP + sub;
+  for (int j = 0; j < kReadFly; ++j) {
+    const int i = i0 + j * RP + sub;
     if (i >= n) continue;
-    O* dst = out + (bh * n + i) * D + gl * V;
+    O* dst = out + (static_cast<int64_t>(bh) * n + i) * D + gl * V;
     if constexpr (Q8) {
       const int8_t* q = reinterpret_cast<const int8_t*>(&raw[j]);
       constexpr int W = 16 / sizeof(O);  // values per 16-byte store
@@ -277,12 +349,6 @@ void check_dims(int B, int heads, int head_dim, int64_t P) {
   LTM_REQUIRE(P < (1ll << 31), "max_positions exceeds int32");
 }
 
-unsigned grid_of(int64_t tasks) {
-  const int64_t g = (tasks + kWarps - 1) / kWarps;
-  LTM_REQUIRE(g < (1ll << 31), "too many rows");
-  return static_cast<unsigned>(g);
-}
-
 template <class F>
 void by_head_dim(int D, F&& f) {
   if (D == 64) f(std::integral_constant<int, 64>{});
@@ -317,21 +383,23 @@ extern "C" ltm_status ltm_kv_cache_append(const void* k, const int64_t* k_stride
                  15) == 0, "the caches must be 16-byte aligned");
     const RowStrides sk{k_strides[0], k_strides[1], k_strides[2]};
     const RowStrides sv{v_strides[0], v_strides[1], v_strides[2]};
-    const int per = static_cast<int>(16 / dtype_size(dtype));
-    const int tok = 32 / (head_dim / per) * kRowsFly;
+    const int tok = 32 / (head_dim / kVals) * kRowsFly;
     const int tgroups = (T + tok - 1) / tok;
-    const int64_t tasks = static_cast<int64_t>(B) * tgroups * 2 * kv_heads;
-    const unsigned grid = grid_of(tasks);
+    LTM_REQUIRE(static_cast<int64_t>(B) * tgroups < (1ll << 31), "too many tokens");
+    const int warps = 2 * kv_heads < kWarps ? 2 * kv_heads : kWarps;
+    const int gy = (2 * kv_heads + warps - 1) / warps;
+    LTM_REQUIRE(gy < (1 << 16), "too many heads");
+    const dim3 grid(static_cast<unsigned>(B) * tgroups, static_cast<unsigned>(gy));
     const cudaStream_t st = as_stream(stream);
     dispatch_dtype(dtype, [&](auto tag) {
       using E = decltype(tag);
       by_head_dim(head_dim, [&](auto d_c) {
         constexpr int D = decltype(d_c)::value;
         auto go = [&](auto q_c) {
-          cache_append_kernel<E, D, decltype(q_c)::value><<<grid, kWarps * 32, 0, st>>>(
+          cache_append_kernel<E, D, decltype(q_c)::value><<<grid, warps * 32, 0, st>>>(
               static_cast<const E*>(k), sk, static_cast<const E*>(v), sv, k_cache, v_cache,
-              k_scale, v_scale, max_positions, cache_lens, num_tokens, B, T, kv_heads, tgroups,
-              tasks, device_error_ptr());
+              k_scale, v_scale, max_positions, cache_lens, num_tokens, T, kv_heads, tgroups,
+              device_error_ptr());
         };
         if constexpr (std::is_same<E, float>::value) {
           go(std::true_type{});
@@ -359,10 +427,10 @@ extern "C" ltm_status ltm_kv_cache_read(const void* cache, const float* scale, l
     if (!scale && out_dtype == LTM_DTYPE_F32) LTM_UNSUPPORTED("fp32 caches (int8, f16 or bf16)");
     LTM_REQUIRE(((reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
                 "the cache and the output must be 16-byte aligned");
-    const int rows = 32 / (head_dim / (scale ? 16 : 8)) * kRowsFly;
-    const int groups = (n + rows - 1) / rows;
-    const int64_t tasks = static_cast<int64_t>(B) * kv_heads * groups;
-    const unsigned grid = grid_of(tasks);
+    const int rows = 32 / (head_dim / (scale ? 16 : 8)) * kReadFly * kWarps;  // per CTA
+    const int gy = (n + rows - 1) / rows;
+    LTM_REQUIRE(static_cast<int64_t>(B) * kv_heads < (1ll << 31) && gy < (1 << 16), "too many rows");
+    const dim3 grid(static_cast<unsigned>(B) * kv_heads, static_cast<unsigned>(gy));
     const cudaStream_t st = as_stream(stream);
     dispatch_dtype(out_dtype, [&](auto tag) {
       using O = decltype(tag);
@@ -370,7 +438,7 @@ extern "C" ltm_status ltm_kv_cache_read(const void* cache, const float* scale, l
         constexpr int D = decltype(d_c)::value;
         auto go = [&](auto q_c) {
           cache_read_kernel<O, D, decltype(q_c)::value><<<grid, kWarps * 32, 0, st>>>(
-              cache, scale, max_positions, first, cache_lens, kv_heads, n, groups, tasks,
+              cache, scale, max_positions, first, cache_lens, kv_heads, n,
               static_cast<O*>(out));
         };
         if constexpr (std::is_same<O, float>::value) {

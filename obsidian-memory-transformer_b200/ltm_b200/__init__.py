@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import dataclasses
+import functools
 from pathlib import Path
 
 import numpy as np
@@ -273,14 +274,26 @@ class KernelTimer:
 
 
 # ---------------------------------------------------------------- torch glue --
+_torch_module = None
+
+
 def _torch():
-    import torch  # noqa: WPS433
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch  # noqa: WPS433
+        _torch_module = torch
+    return _torch_module
+
+
+_dtype_codes: dict = {}
 
 
 def dtype_code(t) -> int:
-    torch = _torch()
-    return {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}[t]
+    if not _dtype_codes:
+        torch = _torch()
+        _dtype_codes.update({torch.float32: DTYPE_F32, torch.float16: DTYPE_F16,
+                             torch.bfloat16: DTYPE_BF16})
+    return _dtype_codes[t]
 
 
 def torch_dtype(code: int):
@@ -473,29 +486,31 @@ def memory_store_noalloc(memory, keys, queries, state, num_heads: int, update_ra
 
 # ------------------------------------------------- KV cache, beam search --
 class _Call:
-    """Device and stream of one call: its tensors' device is the current one
-    inside the `with` block, and memory made there for the call is safe on a
+    """Device and stream of one call: its tensors' device is made the current
+    one (done() puts the old one back), and memory made for the call is safe on a
     stream that is not the current one."""
+
+    __slots__ = ("device", "other", "stream", "_back")
 
     def __init__(self, t, stream):
         torch = _torch()
         self.device = t.device
-        cur = torch.cuda.current_stream(t.device)
-        self.other = stream if stream is not None and stream != cur else None
-        self.stream = C.c_void_p((stream if self.other is not None else cur).cuda_stream)
-        self._guard = None
+        index = self.device.index
+        self.other = self._back = None
+        if torch.cuda.current_device() != index:
+            self._back = torch.cuda.current_device()
+            torch.cuda.set_device(index)
+        raw = torch._C._cuda_getCurrentRawStream(index)
+        if stream is not None and stream.cuda_stream != raw:
+            self.other = stream
+            raw = stream.cuda_stream
+        self.stream = raw
 
-    def __enter__(self):
-        torch = _torch()
-        if torch.cuda.current_device() != self.device.index:
-            self._guard = torch.cuda.device(self.device)
-            self._guard.__enter__()
-        return self
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
-        return False
+    def done(self, status: int) -> None:
+        if self._back is not None:
+            _torch().cuda.set_device(self._back)
+        if status != OK:
+            _check(status)
 
     def empty(self, shape, dtype):
         t = _torch().empty(shape, dtype=dtype, device=self.device)
@@ -508,21 +523,20 @@ def _bad(msg: str):
     raise LtmError(ERR_INVALID_ARG, msg)
 
 
-def _check_op(first, tensors, index=(), index_shape=None):
-    """Tensors (None allowed) on `first`'s CUDA device; `index`: contiguous int32
-    tensors of index_shape."""
+def _check_device(first, *tensors):
+    """Tensors (None allowed) on `first`'s CUDA device."""
     if not first.is_cuda:
         raise ValueError("ltm_b200 operates on CUDA tensors only")
+    device = first.device
     for t in tensors:
-        if t is not None and t.device != first.device:
+        if t is not None and t.device != device:
             _bad("all tensors must be on one device")
-    for t in index:
-        if t is None:
-            continue
-        if t.device != first.device:
-            _bad("all tensors must be on one device")
-        if t.dtype != _torch().int32 or t.shape != index_shape or not t.is_contiguous():
-            _bad(f"lengths and indices must be contiguous int32 {list(index_shape)}")
+
+
+def _check_index(t, shape):
+    """A contiguous int32 tensor of `shape` (or None)."""
+    if t is not None and (t.dtype != _torch().int32 or t.shape != shape or not t.is_contiguous()):
+        _bad(f"lengths and indices must be contiguous int32 {list(shape)}")
 
 
 def _check_cache(cache, scale, what: str):
@@ -543,12 +557,24 @@ def _check_pair(k_cache, v_cache, k_scale, v_scale):
         _bad("k_cache and v_cache must have one shape and type")
 
 
+@functools.lru_cache(maxsize=256)
+def _int64s(*v):
+    return (C.c_int64 * len(v))(*v)
+
+
 def _strides3(t, what: str):
     """Batch, token and head strides of a [B, T, heads, head_dim] view."""
     s = t.stride()
     if s[3] != 1:
         _bad(f"{what} must have unit stride in head_dim")
-    return (C.c_int64 * 3)(s[0], s[1], s[2])
+    return _int64s(s[0], s[1], s[2])
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(name: str, *sizes) -> int:
+    n = C.c_size_t()
+    _check(getattr(lib(), name)(*sizes, C.byref(n)))
+    return n.value
 
 
 def _dp(t):
@@ -565,7 +591,7 @@ def kv_cache_append(k, v, k_cache, v_cache, cache_lens, k_scale=None, v_scale=No
     head_dim]: int8 with fp32 scales [B, kv_heads, max_positions] (k, v f32, f16
     or bf16), or of k's type (f16 / bf16).  cache_lens, num_tokens (how many of the
     T tokens a sequence has): int32 [B].  The lengths are not advanced."""
-    _check_op(k, (v, k_cache, v_cache, k_scale, v_scale), (cache_lens, num_tokens), k.shape[:1])
+    _check_device(k, v, k_cache, v_cache, cache_lens, k_scale, v_scale, num_tokens)
     _check_pair(k_cache, v_cache, k_scale, v_scale)
     if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
         _bad("k and v must both be [B, T, kv_heads, head_dim]")
@@ -574,11 +600,14 @@ def kv_cache_append(k, v, k_cache, v_cache, cache_lens, k_scale=None, v_scale=No
         _bad("the caches do not fit k and v")
     if k_scale is None and k_cache.dtype != k.dtype:
         _bad("the caches must be int8 or have k's type")
-    with _Call(k, stream) as c:
-        _check(lib().ltm_kv_cache_append(
-            k.data_ptr(), _strides3(k, "k"), v.data_ptr(), _strides3(v, "v"), dtype_code(k.dtype),
-            k_cache.data_ptr(), v_cache.data_ptr(), _dp(k_scale), _dp(v_scale), k_cache.shape[2],
-            cache_lens.data_ptr(), _dp(num_tokens), B, T, h, d, c.stream))
+    _check_index(cache_lens, (B,))
+    _check_index(num_tokens, (B,))
+    sk, sv, dt = _strides3(k, "k"), _strides3(v, "v"), dtype_code(k.dtype)
+    c = _Call(k, stream)
+    c.done(lib().ltm_kv_cache_append(
+        k.data_ptr(), sk, v.data_ptr(), sv, dt, k_cache.data_ptr(), v_cache.data_ptr(),
+        _dp(k_scale), _dp(v_scale), k_cache.shape[2], cache_lens.data_ptr(), _dp(num_tokens), B, T,
+        h, d, c.stream))
 
 
 def kv_cache_read(cache, scale, length: int, first=None, cache_lens=None, dtype=None, out=None,
@@ -588,7 +617,7 @@ def kv_cache_read(cache, scale, length: int, first=None, cache_lens=None, dtype=
     caches give code * scale in `dtype` (f32, f16 or bf16; f32 when None), other caches
     (scale None) their values.  Positions outside [0, cache_lens[b]) (int32 [B];
     max_positions when None) give zeros."""
-    _check_op(cache, (scale, out), (first, cache_lens), cache.shape[:1])
+    _check_device(cache, scale, first, cache_lens, out)
     _check_cache(cache, scale, "cache")
     if length < 0:
         _bad("length must not be negative")
@@ -597,15 +626,16 @@ def kv_cache_read(cache, scale, length: int, first=None, cache_lens=None, dtype=
     if scale is None and dtype != cache.dtype:
         _bad("a 16-bit cache is read in its own type")
     B, h, P, d = cache.shape
-    shape = (B, h, length, d)
-    with _Call(cache, stream) as c:
-        if out is None:
-            out = c.empty(shape, dtype)
-        elif out.shape != shape or out.dtype != dtype or not out.is_contiguous():
-            _bad(f"out must be contiguous {list(shape)} of the read type")
-        _check(lib().ltm_kv_cache_read(cache.data_ptr(), _dp(scale), dtype_code(dtype), P,
-                                       _dp(first), _dp(cache_lens), B, h, d, length,
-                                       out.data_ptr(), c.stream))
+    _check_index(first, (B,))
+    _check_index(cache_lens, (B,))
+    shape, dt = (B, h, length, d), dtype_code(dtype)
+    if out is not None and (out.shape != shape or out.dtype != dtype or not out.is_contiguous()):
+        _bad(f"out must be contiguous {list(shape)} of the read type")
+    c = _Call(cache, stream)
+    if out is None:
+        out = c.empty(shape, dtype)
+    c.done(lib().ltm_kv_cache_read(cache.data_ptr(), _dp(scale), dt, P, _dp(first),
+                                   _dp(cache_lens), B, h, d, length, out.data_ptr(), c.stream))
     return out
 
 
@@ -620,29 +650,31 @@ def tree_attention(q, k_cache, v_cache, cache_lens, parents=None, k_scale=None, 
     have been appended (kv_cache_append).  parents: int32 [B, T], -1 for a root;
     None for a chain.  num_tokens: int32 [B], how many of the T tokens a sequence
     has (the others get zeros).  Returns [B, T, heads, head_dim]."""
-    _check_op(q, (k_cache, v_cache, k_scale, v_scale, out), (cache_lens, num_tokens), q.shape[:1])
-    _check_op(q, (), (parents,), q.shape[:2])
+    _check_device(q, k_cache, v_cache, cache_lens, parents, k_scale, v_scale, num_tokens, out)
     _check_pair(k_cache, v_cache, k_scale, v_scale)
     if q.dim() != 4 or k_cache.shape[0] != q.shape[0] or k_cache.shape[3] != q.shape[3]:
         _bad("q must be [B, T, heads, head_dim] for the caches' B and head_dim")
     if k_scale is None and k_cache.dtype != q.dtype:
         _bad("the caches must be int8 or have q's type")
-    B, T, heads, d = q.shape
+    shape = q.shape
+    B, T, heads, d = shape
     kvh, P = k_cache.shape[1], k_cache.shape[2]
-    L = lib()
-    nbytes = C.c_size_t()
-    _check(L.ltm_tree_attention_workspace(B, T, heads, kvh, d, C.byref(nbytes)))
-    with _Call(q, stream) as c:
-        if out is None:
-            out = c.empty(q.shape, q.dtype)
-        elif out.shape != q.shape or out.dtype != q.dtype:
-            _bad("out must have q's shape and type")
-        ws = c.empty(nbytes.value, _torch().uint8)
-        _check(L.ltm_tree_attention(
-            q.data_ptr(), _strides3(q, "q"), k_cache.data_ptr(), v_cache.data_ptr(), _dp(k_scale),
-            _dp(v_scale), P, cache_lens.data_ptr(), _dp(num_tokens), _dp(parents), out.data_ptr(),
-            _strides3(out, "out"), B, T, heads, kvh, d, dtype_code(q.dtype), ws.data_ptr(),
-            nbytes.value, c.stream))
+    _check_index(cache_lens, (B,))
+    _check_index(num_tokens, (B,))
+    _check_index(parents, (B, T))
+    if out is not None and (out.shape != shape or out.dtype != q.dtype):
+        _bad("out must have q's shape and type")
+    sq, dt = _strides3(q, "q"), dtype_code(q.dtype)
+    so = (_int64s(T * heads * d, heads * d, d) if out is None else _strides3(out, "out"))
+    nbytes = _workspace_bytes("ltm_tree_attention_workspace", B, T, heads, kvh, d)
+    c = _Call(q, stream)
+    if out is None:
+        out = c.empty(shape, q.dtype)
+    ws = c.empty(nbytes, _torch().uint8)
+    c.done(lib().ltm_tree_attention(
+        q.data_ptr(), sq, k_cache.data_ptr(), v_cache.data_ptr(), _dp(k_scale), _dp(v_scale), P,
+        cache_lens.data_ptr(), _dp(num_tokens), _dp(parents), out.data_ptr(), so, B, T, heads, kvh,
+        d, dt, ws.data_ptr(), nbytes, c.stream))
     return out
 
 
@@ -655,7 +687,7 @@ def beam_select(logits, scores, num_out: int | None = None, done=None, end_token
     `done` (bool [B, W]) finished beams continue as themselves with `end_token`
     and a fourth output [B, K] bool says which continuations are finished."""
     torch = _torch()
-    _check_op(logits, (scores, done))
+    _check_device(logits, scores, done)
     if logits.dim() != 3 or logits.stride(2) != 1:
         _bad("logits must be [B, W, V] with unit stride in V")
     B, W, V = logits.shape
@@ -665,19 +697,19 @@ def beam_select(logits, scores, num_out: int | None = None, done=None, end_token
                              or not done.is_contiguous()):
         _bad("done must be contiguous bool [B, W]")
     K = W if num_out is None else num_out
-    L = lib()
-    nbytes = C.c_size_t()
-    _check(L.ltm_beam_select_workspace(B, W, V, K, C.byref(nbytes)))
-    with _Call(logits, stream) as c:
-        s = c.empty((B, K), torch.float32)
-        bt = c.empty((2, B, K), torch.int32)
-        d = c.empty((B, K), torch.bool) if done is not None else None
-        ws = c.empty(nbytes.value, torch.uint8)
-        _check(L.ltm_beam_select(
-            logits.data_ptr(), dtype_code(logits.dtype), logits.stride(0), logits.stride(1),
-            scores.data_ptr(), _dp(done), end_token, B, W, V, K, s.data_ptr(), bt[0].data_ptr(),
-            bt[1].data_ptr(), _dp(d), ws.data_ptr(), nbytes.value, c.stream))
-    return (s, bt[0], bt[1]) if d is None else (s, bt[0], bt[1], d)
+    sb, sw, _ = logits.stride()
+    dt = dtype_code(logits.dtype)
+    nbytes = _workspace_bytes("ltm_beam_select_workspace", B, W, V, K)
+    c = _Call(logits, stream)
+    best = c.empty((B, K), torch.float32)
+    beams, tokens = c.empty((2, B, K), torch.int32).unbind(0)
+    fin = c.empty((B, K), torch.bool) if done is not None else None
+    ws = c.empty(nbytes, torch.uint8)
+    c.done(lib().ltm_beam_select(
+        logits.data_ptr(), dt, sb, sw, scores.data_ptr(), _dp(done), end_token, B, W, V, K,
+        best.data_ptr(), beams.data_ptr(), tokens.data_ptr(), _dp(fin), ws.data_ptr(), nbytes,
+        c.stream))
+    return (best, beams, tokens) if fin is None else (best, beams, tokens, fin)
 
 
 def kv_cache_reorder(caches, beams, cache_lens=None, first=None, stream=None) -> None:
@@ -688,11 +720,13 @@ def kv_cache_reorder(caches, beams, cache_lens=None, first=None, stream=None) ->
     max_positions] tensors (int8 caches' scales), each once; beams int32 [B, W];
     cache_lens, first: int32 [B] (max_positions and 0 when None)."""
     caches = list(caches)
-    _check_op(beams, caches, (beams,), beams.shape)
+    _check_device(beams, cache_lens, first, *caches)
     if beams.dim() != 2:
         _bad("beams must be int32 [B, W]")
     B, W = beams.shape
-    _check_op(beams, (), (cache_lens, first), beams.shape[:1])
+    _check_index(beams, (B, W))
+    _check_index(cache_lens, (B,))
+    _check_index(first, (B,))
     n = len(caches)
     if n == 0:
         return
@@ -703,11 +737,10 @@ def kv_cache_reorder(caches, beams, cache_lens=None, first=None, stream=None) ->
     if lead[0] != B * W:
         _bad("caches must have B * W sequences")
     ptrs = (C.c_void_p * n)(*[t.data_ptr() for t in caches])
-    rows = (C.c_int64 * n)(*[t.element_size() * (t.shape[3] if t.dim() == 4 else 1)
-                             for t in caches])
-    with _Call(beams, stream) as c:
-        _check(lib().ltm_kv_cache_reorder(ptrs, rows, n, beams.data_ptr(), _dp(first),
-                                          _dp(cache_lens), B, W, lead[1], lead[2], c.stream))
+    rows = _int64s(*[t.element_size() * (t.shape[3] if t.dim() == 4 else 1) for t in caches])
+    c = _Call(beams, stream)
+    c.done(lib().ltm_kv_cache_reorder(ptrs, rows, n, beams.data_ptr(), _dp(first),
+                                      _dp(cache_lens), B, W, lead[1], lead[2], c.stream))
 
 
 # --------------------------------------------------------------------- block --
