@@ -339,8 +339,8 @@ LTM_API ltm_status ltm_tree_attention(const void* q, const int64_t* q_strides, c
  * V of them contiguous, any alignment; scores: fp32 [B, W], finite or -inf (a
  * beam that does not exist).  done (uint8 [B, W] or NULL): a finished beam
  * continues as itself only, its end_token keeping its score and every other
- * token -inf.  A NaN logit or score counts as -inf, a logit +inf as the largest
- * float.  Outputs [B, K]: totals (evaluated in 64 bits, stored as fp32), the beam
+ * token -inf.  A NaN logit or score counts as -inf, a logit +inf as its type's
+ * largest value.  Outputs [B, K]: totals (evaluated in 64 bits, stored as fp32), the beam
  * and the token of each, and with done whether the continuation is finished (its
  * beam was, or the token is end_token).  W <= 32, K <= 64.
  * workspace: device memory of ltm_beam_select_workspace bytes, 8-byte aligned. */

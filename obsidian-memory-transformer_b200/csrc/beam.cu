@@ -5,7 +5,7 @@
 //   K largest totals, descending; equal totals: the lowest w * V + x first.
 //   A finished beam (done) continues as itself only: its end token keeps
 //   score_w, every other token has -inf.
-// A logit NaN counts as -inf and +inf as the largest finite float; a score that
+// A logit NaN counts as -inf and +inf as its type's largest value; a score that
 // is NaN counts as -inf.
 //
 // Every logit is read once (the bound): beam_chunk_kernel gives each CTA up to
@@ -44,9 +44,13 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 __device__ __forceinline__ float unordered(uint32_t u) {
   return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
-// fmaxf gives the other operand for a NaN.
+// NaN -> -inf (fmaxf gives the other operand for a NaN), +inf -> the type's largest value.
+template <class T>
 __device__ __forceinline__ float logit_value(float x) {
-  return fminf(fmaxf(x, -INFINITY), 3.402823466e38f);
+  constexpr float kMost = std::is_same<T, float>::value    ? 3.402823466e38f
+                          : std::is_same<T, __half>::value ? 65504.0f
+                                                           : 3.389531390e38f;
+  return fminf(fmaxf(x, -INFINITY), kMost);
 }
 __device__ __forceinline__ uint64_t list_key(float x, int token) {
   return (static_cast<uint64_t>(ordered(x)) << 32) | ~static_cast<uint32_t>(token);
@@ -59,27 +63,31 @@ struct BeamPartial {
 // Workspace: [rows, nchunk] BeamPartial, then [rows, nchunk, K] sorted keys
 // (ordered logit << 32 | ~token; 0 = none).
 template <class T>
-__global__ void __launch_bounds__(kBThreads, 3)
+__global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 5 : 3)
     beam_chunk_kernel(const T* __restrict__ logits, int64_t ldb, int64_t ldw,
                       const float* __restrict__ scores, const uint8_t* __restrict__ done, int end,
                       int W, int V, int K, int nchunk, int groups, BeamPartial* __restrict__ stats,
                       uint64_t* __restrict__ lists) {
+  constexpr int N = 16 / sizeof(T);  // logits per vector
+  constexpr int NV = kPer / N;       // vectors per thread
   __shared__ float s_group[kBThreads];
   __shared__ float s_sum[kBThreads / 32];
   __shared__ uint64_t s_cand[kMaxCand];
   __shared__ uint64_t s_best[kBThreads / 32];
-  __shared__ int s_count;
+  __shared__ uint4 s_slot[kBThreads * NV];  // vectors of the threads that hold candidates
+  __shared__ int s_owner[kBThreads];
+  __shared__ int s_count, s_slots;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / nchunk, chunk = blockIdx.x - row * nchunk;
   const int b = row / W, w = row - b * W;
   const int c0 = chunk * kChunk, c1 = min(V, c0 + kChunk);
   const int64_t item = blockIdx.x;
   uint64_t* list = lists + item * K;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- load: 16-byte vectors of the row's aligned span, all in flight at once; then the
-  // vectors that the chunk's ends cut, element by element
-  constexpr int N = 16 / sizeof(T);  // logits per vector
-  constexpr int NV = kPer / N;       // vectors per thread
+  // vectors that the chunk's ends cut, element by element (-inf where there is none:
+  // such elements are left out by their index below)
   const T* r = logits + b * ldb + w * ldw;
   const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
   // token of element j of vector i: t0 + i * 256 * N + j
@@ -88,7 +96,6 @@ __global__ void __launch_bounds__(kBThreads, 3)
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int x = t0 + i * kBThreads * N;
-    raw[i] = make_uint4(0, 0, 0, 0);
     if (x >= c0 && x + N <= c1) raw[i] = __ldg(reinterpret_cast<const uint4*>(r + x));
   }
   const float score = scores[row];
@@ -112,80 +119,96 @@ __global__ void __launch_bounds__(kBThreads, 3)
     if (tid == 0) stats[item] = BeamPartial{0.0f, 1.0f};
     return;
   }
-  if (tid == 0) s_count = 0;
-  // elements that are not there are -inf here and left out by their index below
-  float v[kPer];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const T* e = reinterpret_cast<const T*>(&raw[i]);
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[i * N + j] = logit_value(to_f32(e[j]));
-  }
+  if (tid == 0) s_count = s_slots = 0;
+  const T none = from_f32<T>(-INFINITY);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int x = t0 + i * kBThreads * N;
     if (!(x >= c0 && x + N <= c1)) {
+      T e[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        v[i * N + j] = (x + j >= c0 && x + j < c1) ? logit_value(to_f32(r[x + j])) : -INFINITY;
+      for (int j = 0; j < N; ++j) e[j] = (x + j >= c0 && x + j < c1) ? r[x + j] : none;
+      raw[i] = *reinterpret_cast<const uint4*>(e);
     }
   }
   // a misaligned row's last `shift` logits lie past the vectors: one per thread
   const int xe = c0 - shift + kChunk + tid;
   const bool has_extra = tid < shift && xe < c1;
-  const float extra = has_extra ? logit_value(to_f32(r[xe])) : -INFINITY;
+  float extra = has_extra ? to_f32(r[xe]) : -INFINITY;
 
-  float vm[NV];  // maximum of each vector
-  float tm = extra;
+  // Maximum, bound and sum.  The first pass takes the logits as they are; a NaN
+  // or +inf among them makes the sum a NaN, and they are replaced before a second.
+  float m, tau, tm;
+  while (true) {
+    tm = extra;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    vm[i] = v[i * N];
+    for (int i = 0; i < NV; ++i) {
+      const T* e = reinterpret_cast<const T*>(&raw[i]);
 #pragma unroll
-    for (int j = 1; j < N; ++j) vm[i] = fmaxf(vm[i], v[i * N + j]);
-    tm = fmaxf(tm, vm[i]);
+      for (int j = 0; j < N; ++j) tm = fmaxf(tm, to_f32(e[j]));
+    }
+    // maxima of the groups of equal tid % groups (so that a short chunk fills them all)
+    float gm = tm;
+    for (int o = 16; o >= groups; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+    s_group[tid] = gm;
+    __syncthreads();
+    float g0 = -INFINITY, g1 = -INFINITY;  // groups lane and lane + 32 (mod groups)
+#pragma unroll
+    for (int i = 0; i < kBThreads / 32; i += 2) {
+      g0 = fmaxf(g0, s_group[i * 32 + lane]);
+      g1 = fmaxf(g1, s_group[i * 32 + 32 + lane]);
+    }
+    if (groups <= 32) g0 = g1 = fmaxf(g0, g1);
+    m = unordered(__reduce_max_sync(0xffffffffu, ordered(fmaxf(g0, g1))));
+    tau = unordered(__reduce_min_sync(0xffffffffu, ordered(fminf(g0, g1))));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float sum = __expf(extra - ref);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const T* e = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+      for (int j = 0; j < N; ++j) sum += __expf(to_f32(e[j]) - ref);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) s_sum[warp] = sum;
+    if (!__syncthreads_or(sum != sum)) break;
+    extra = logit_value<T>(extra);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      T* e = reinterpret_cast<T*>(&raw[i]);
+#pragma unroll
+      for (int j = 0; j < N; ++j) e[j] = from_f32<T>(logit_value<T>(to_f32(e[j])));
+    }
   }
-  // maxima of the groups of equal tid % groups (so that a short chunk fills them all)
-  float gm = tm;
-  for (int o = 16; o >= groups; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
-  s_group[tid] = gm;
-  __syncthreads();
-  float g0 = -INFINITY, g1 = -INFINITY;  // groups lane and lane + 32 (mod groups)
-#pragma unroll
-  for (int i = 0; i < kBThreads / 32; i += 2) {
-    g0 = fmaxf(g0, s_group[i * 32 + lane]);
-    g1 = fmaxf(g1, s_group[i * 32 + 32 + lane]);
-  }
-  if (groups <= 32) g0 = g1 = fmaxf(g0, g1);
-  const float m = unordered(__reduce_max_sync(0xffffffffu, ordered(fmaxf(g0, g1))));
-  const float tau = unordered(__reduce_min_sync(0xffffffffu, ordered(fminf(g0, g1))));
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float sum = __expf(extra - ref);
+  // ---- the threads that hold a value at the bound hand theirs to the whole CTA
   auto offer = [&](float y, int x) {
     if (y >= tau && x >= c0 && x < c1) {
       const int at = atomicAdd(&s_count, 1);
       if (at < kMaxCand) s_cand[at] = list_key(y, x);
     }
   };
+  if (tm >= tau) {
+    const int at = atomicAdd(&s_slots, 1);
+    s_owner[at] = t0;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) sum += __expf(v[i * N + j] - ref);
-    if (vm[i] >= tau) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) offer(v[i * N + j], t0 + i * kBThreads * N + j);
-    }
+    for (int i = 0; i < NV; ++i) s_slot[at * NV + i] = raw[i];
+    if (has_extra) offer(extra, xe);
   }
-  if (has_extra) offer(extra, xe);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) s_sum[warp] = sum;
-  __syncthreads();
   if (tid == 0) {
     float t = 0.0f;
 #pragma unroll
     for (int i = 0; i < kBThreads / 32; ++i) t += s_sum[i];
     stats[item] = BeamPartial{m, t};
   }
+  __syncthreads();
+  const int nval = s_slots * kPer;
+  for (int i = tid; i < nval; i += kBThreads) {
+    const float y = to_f32(reinterpret_cast<const T*>(s_slot)[i]);
+    const int e = i % kPer;
+    offer(y, s_owner[i / kPer] + (e / N) * kBThreads * N + e % N);
+  }
+  __syncthreads();
   const int n = s_count;
   if (n <= kMaxCand) {
     for (int i = tid; i < n; i += kBThreads) {
@@ -207,7 +230,11 @@ __global__ void __launch_bounds__(kBThreads, 3)
       if (x >= c0 && x < c1 && full < last && full > best) best = full;
     };
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) look(v[i], t0 + (i / N) * kBThreads * N + i % N);
+    for (int i = 0; i < NV; ++i) {
+      const T* e = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+      for (int j = 0; j < N; ++j) look(to_f32(e[j]), t0 + i * kBThreads * N + j);
+    }
     if (has_extra) look(extra, xe);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
@@ -232,145 +259,183 @@ __device__ __forceinline__ double unordered64(uint64_t u) {
 }
 
 // A continuation: larger total first, then the lower flat index.
-struct Total {
+struct __align__(16) Total {
   uint64_t t;  // ordered bits of the total; 0 = none
-  uint64_t f;  // beam * V + token
+  uint32_t f;  // beam * V + token (below 2^29)
+  uint32_t pad;
 };
 __device__ __forceinline__ bool before(const Total& a, const Total& b) {
   return a.t > b.t || (a.t == b.t && a.f < b.f);
 }
 
-constexpr int kMergeCand = 512;  // continuations ranked in shared memory
+constexpr int kMergeCand = 512;   // continuations ranked in shared memory
+constexpr int kMergeKeys = 8192;  // entries whose keys fit in shared memory
+constexpr int kMergeSlack = 24;   // continuations past K that are ranked rather than sorted out
 
-// One CTA per request.  Its W * nchunk lists are sorted, so the best d entries
-// of every list, d = ceil(K / lists), hold K continuations: the least of those
-// d-th entries bounds the K-th best from below, more sharply by the K-th of
-// the lists' heads where there are K of them.  What reaches the bound is ranked;
-// where that is more than shared memory takes, the K best are taken one by one.
+// One CTA per request.  Its W * nchunk lists are sorted, so the best
+// d = ceil(K / lists) entries of every list hold K continuations, and the least of
+// those d-th entries is a total that at least K reach.  From there a bisection on
+// the upper 32 bits of the totals (one count per step) raises the bound until
+// few more than K are left, whatever the beams' scores; those are ranked.  Where
+// shared memory does not take them (equal totals), the K best are taken one by
+// one.  Loops stay rolled: for one request the code's own fetch is most of the time.
 __global__ void __launch_bounds__(kBThreads)
     beam_merge_kernel(const float* __restrict__ scores, const uint8_t* __restrict__ done, int end,
-                      int W, int V, int K, int nchunk, const BeamPartial* __restrict__ stats,
-                      const uint64_t* __restrict__ lists, float* __restrict__ out_scores,
+                      int W, int V, int K, int nchunk, const BeamPartial* stats,
+                      const uint64_t* lists, float* __restrict__ out_scores,
                       int* __restrict__ out_beams, int* __restrict__ out_tokens,
                       uint8_t* __restrict__ out_done) {
-  __shared__ double s_m[kMaxW], s_ls[kMaxW], s_score[kMaxW];
+  __shared__ double s_base[kMaxW], s_score[kMaxW];  // score - max - log(sum), score
+  __shared__ float s_max[kMaxW];
   __shared__ uint8_t s_done[kMaxW];
   __shared__ Total s_cand[kMergeCand];
   __shared__ Total s_best[kBThreads / 32];
-  __shared__ uint64_t s_low[kBThreads / 32];
-  __shared__ int s_count;
+  __shared__ uint32_t s_key[kMergeKeys];
+  __shared__ uint32_t s_lim[2 * kBThreads / 32];
+  __shared__ int s_count[2];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int nlists = W * nchunk;
-  const uint64_t* mine = lists + static_cast<int64_t>(b) * nlists * K;
-  if (tid == 0) s_count = 0;
+  const int nlists = W * nchunk, entries = nlists * K;
+  const uint64_t* mine = lists + static_cast<int64_t>(b) * entries;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the chunks' kernel has completed
   // a row's maximum and sum over its chunks: one warp per row
+#pragma unroll 1
   for (int w = warp; w < W; w += kBThreads / 32) {
     const int row = b * W + w;
     const float sc = scores[row];
-    float m = -INFINITY;
-    double sum = 0.0;
+    float m = -INFINITY, sum = 0.0f;
+#pragma unroll 1
     for (int c0 = 0; c0 < nchunk; c0 += 32) {
       BeamPartial st{-INFINITY, 0.0f};
       if (c0 + lane < nchunk) st = stats[static_cast<int64_t>(row) * nchunk + c0 + lane];
-      float mm = st.m;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-      mm = fmaxf(mm, m);
-      double part = st.m == -INFINITY ? 0.0 : static_cast<double>(st.sum * expf(st.m - mm));
+      const float mm =
+          fmaxf(m, unordered(__reduce_max_sync(0xffffffffu, ordered(st.m))));
+      float part = st.m == -INFINITY ? 0.0f : st.sum * expf(st.m - mm);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-      sum = (m == -INFINITY ? 0.0 : sum * static_cast<double>(expf(m - mm))) + part;
+      sum = (m == -INFINITY ? 0.0f : sum * expf(m - mm)) + part;
       m = mm;
     }
     if (lane == 0) {
-      s_m[w] = m;
-      s_ls[w] = log(sum);
-      s_score[w] = sc == sc ? sc : -INFINITY;
+      const float s = sc == sc ? sc : -INFINITY;
+      s_max[w] = m;
+      s_base[w] = static_cast<double>(s) - log(static_cast<double>(sum));
+      s_score[w] = s;
       s_done[w] = done != nullptr && done[row] != 0;
     }
   }
   __syncthreads();
-  auto entry = [&](int l, int pos) -> Total {
-    const uint64_t key = mine[static_cast<int64_t>(l) * K + pos];
-    if (key == 0ull) return Total{0ull, ~0ull};
+  auto entry = [&](int l, int i) -> Total {  // list l, entry i of all
+    const uint64_t key = mine[i];
+    if (key == 0ull) return Total{0ull, ~0u, 0u};
     const uint32_t u = static_cast<uint32_t>(key >> 32);
     const int w = l / nchunk;
     double t = -INFINITY;
     if (u > kNegInf && s_score[w] > -INFINITY)
-      t = s_done[w] ? s_score[w]
-                    : s_score[w] + ((static_cast<double>(unordered(u)) - s_m[w]) - s_ls[w]);
-    return Total{ordered64(t), static_cast<uint64_t>(w) * V + ~static_cast<uint32_t>(key)};
+      t = s_done[w] ? s_score[w] : s_base[w] + (static_cast<double>(unordered(u)) - s_max[w]);
+    return Total{ordered64(t), static_cast<uint32_t>(w) * V + ~static_cast<uint32_t>(key), 0u};
   };
   auto put = [&](int k, const Total& x) {
-    const int w = static_cast<int>(x.f / V), tok = static_cast<int>(x.f - static_cast<uint64_t>(w) * V);
+    const int w = static_cast<int>(x.f / static_cast<uint32_t>(V));
+    const int tok = static_cast<int>(x.f) - w * V;
     const int64_t o = static_cast<int64_t>(b) * K + k;
     out_scores[o] = static_cast<float>(unordered64(x.t));
     out_beams[o] = w;
     out_tokens[o] = tok;
     if (out_done) out_done[o] = s_done[w] || tok == end;
   };
-  // ---- the bound (ordered bits of a total that at least K continuations reach)
-  uint64_t low = ~0ull;
-  if (nlists >= K && nlists <= kMergeCand) {
-    for (int l = tid; l < nlists; l += kBThreads) s_cand[l] = entry(l, 0);
-    __syncthreads();
-    for (int l = tid; l < nlists; l += kBThreads) {
-      const Total x = s_cand[l];
-      int rank = 0;
-#pragma unroll 4
-      for (int j = 0; j < nlists; ++j) rank += before(s_cand[j], x);
-      if (rank == K - 1) s_low[0] = x.t;
-    }
-    __syncthreads();
-    low = s_low[0];
-    __syncthreads();  // s_cand is written again below
-  } else {
-    const int d = min(K, (K + nlists - 1) / nlists) - 1;
-    for (int l = tid; l < nlists; l += kBThreads) low = min(low, entry(l, d).t);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
-    if (lane == 0) s_low[warp] = low;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kBThreads / 32; ++i) low = min(low, s_low[i]);
+  // ---- the bound: `low` is reached by at least K continuations
+  const bool staged = entries <= kMergeKeys;
+  auto key_of = [&](int i) -> uint32_t {
+    return staged ? s_key[i] : static_cast<uint32_t>(entry(i / K, i).t >> 32);
+  };
+  if (staged)
+#pragma unroll 1
+    for (int i = tid; i < entries; i += kBThreads)
+      s_key[i] = static_cast<uint32_t>(entry(i / K, i).t >> 32);
+  __syncthreads();
+  const int d = min(K, (K + nlists - 1) / nlists) - 1;
+  uint32_t low = ~0u, high = 0u;
+#pragma unroll 1
+  for (int l = tid; l < nlists; l += kBThreads) {
+    low = min(low, key_of(l * K + d));
+    high = max(high, key_of(l * K));
   }
-  low = max(low, static_cast<uint64_t>(1));  // a list without that many entries bounds nothing
-  const int entries = nlists * K;
-  for (int i = tid; i < entries; i += kBThreads) {
-    const Total x = entry(i / K, i % K);
-    if (x.t >= low) {
-      const int at = atomicAdd(&s_count, 1);
-      if (at < kMergeCand) s_cand[at] = x;
+  low = __reduce_min_sync(0xffffffffu, low);
+  high = __reduce_max_sync(0xffffffffu, high);
+  if (lane == 0) {
+    s_lim[warp] = low;
+    s_lim[8 + warp] = high;
+  }
+  __syncthreads();
+  for (int i = 0; i < kBThreads / 32; ++i) {
+    low = min(low, s_lim[i]);
+    high = max(high, s_lim[8 + i]);
+  }
+  low = max(low, 1u);  // a list without that many entries bounds nothing
+  if (tid < 2) s_count[tid] = 0;
+  __syncthreads();
+  // how many reach x; the two counters take turns
+  int turn = 0;
+  auto reach = [&](uint32_t x) -> int {
+    int c = 0;
+#pragma unroll 1
+    for (int i = tid; i < entries; i += kBThreads) c += key_of(i) >= x;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0 && c) atomicAdd(&s_count[turn], c);
+    __syncthreads();
+    c = s_count[turn];
+    turn ^= 1;
+    __syncthreads();
+    if (tid == 0) s_count[turn ^ 1] = 0;
+    return c;
+  };
+  int n = reach(low);
+  while (n > K + kMergeSlack && low < high) {
+    const uint32_t mid = low + (high - low + 1) / 2;
+    const int c = reach(mid);
+    if (c >= K) {
+      low = mid;
+      n = c;
+    } else {
+      high = mid - 1;
     }
   }
   __syncthreads();
-  const int n = s_count;
   if (n <= kMergeCand) {
+    if (tid == 0) s_count[0] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < entries; i += kBThreads)
+      if (key_of(i) >= low) s_cand[atomicAdd(&s_count[0], 1)] = entry(i / K, i);
+    __syncthreads();
+#pragma unroll 1
     for (int i = tid; i < n; i += kBThreads) {
       const Total x = s_cand[i];
       int rank = 0;
-#pragma unroll 4
+#pragma unroll 2
       for (int j = 0; j < n; ++j) rank += before(s_cand[j], x);
       if (rank < K) put(rank, x);
     }
     return;
   }
-  Total last{~0ull, 0ull};
+  Total last{~0ull, 0u, 0u};
+#pragma unroll 1
   for (int k = 0; k < K; ++k) {
-    Total best{0ull, ~0ull};
+    Total best{0ull, ~0u, 0u};
+#pragma unroll 1
     for (int i = tid; i < entries; i += kBThreads) {
-      const Total x = entry(i / K, i % K);
+      const Total x = entry(i / K, i);
       if (before(last, x) && before(x, best)) best = x;
     }
-#pragma unroll
+#pragma unroll 1
     for (int o = 16; o > 0; o >>= 1) {
-      const Total y{__shfl_xor_sync(0xffffffffu, best.t, o), __shfl_xor_sync(0xffffffffu, best.f, o)};
+      const Total y{__shfl_xor_sync(0xffffffffu, best.t, o), __shfl_xor_sync(0xffffffffu, best.f, o), 0u};
       if (before(y, best)) best = y;
     }
     __syncthreads();
     if (lane == 0) s_best[warp] = best;
     __syncthreads();
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < kBThreads / 32; ++i)
       if (before(s_best[i], best)) best = s_best[i];
     if (tid == 0) put(k, best);
@@ -434,9 +499,11 @@ extern "C" ltm_status ltm_beam_select(const void* logits, ltm_dtype dtype, int64
           K, nchunk, groups, stats, lists);
     });
     check_launch("beam_chunk_kernel", st);
-    beam_merge_kernel<<<B, kBThreads, 0, st>>>(
-        scores, done, end_token, W, V, K, nchunk, stats, lists, out_scores, out_beams, out_tokens,
-        out_done);
+    // launched while the chunks still run; it waits for their completion on the device
+    launch_dependent(beam_merge_kernel, dim3(static_cast<unsigned>(B)), kBThreads, 0, st, scores,
+                     done, end_token, W, V, K, nchunk, static_cast<const BeamPartial*>(stats),
+                     static_cast<const uint64_t*>(lists), out_scores, out_beams, out_tokens,
+                     out_done);
     check_launch("beam_merge_kernel", st);
   });
 }

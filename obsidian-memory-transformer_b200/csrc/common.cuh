@@ -251,6 +251,25 @@ int persistent_grid(K kernel, int block, size_t smem, int64_t want) {
   return static_cast<int>(want < cap ? (want < 1 ? 1 : want) : cap);
 }
 
+// Launches a kernel that starts by waiting (griddepcontrol.wait) for the kernel
+// before it on the stream: its CTAs may be scheduled once every CTA of that
+// kernel has executed griddepcontrol.launch_dependents or ended.
+template <class... P, class... A>
+void launch_dependent(void (*kernel)(P...), dim3 grid, int block, size_t smem, cudaStream_t stream,
+                      A... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(block));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  LTM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+}
+
 // ------------------------------------------------------- PTX: sync/timing --
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

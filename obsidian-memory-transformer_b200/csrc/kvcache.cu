@@ -77,17 +77,17 @@ __device__ __forceinline__ float quant_row16(const float (&v)[kVals], uint32_t a
   const float inv = (bad || tiny) ? 0.0f : rcp_approx(s);
   const uint64_t inv2 = f2_pack(inv, inv), shift2 = f2_pack(kShift, kShift);
   float big[kVals], off[kVals];
-  bool near_tie = false;
+  float far = 0.0f;  // the largest distance from the rounded value
 #pragma unroll
   for (int i = 0; i < kVals; i += 2) {
     const uint64_t t = f2_mul(f2_pack(v[i], v[i + 1]), inv2);
     const uint64_t b = f2_add(t, shift2);
     f2_unpack(f2_sub(t, f2_sub(b, shift2)), off[i], off[i + 1]);
     f2_unpack(b, big[i], big[i + 1]);
-    near_tie |= (fabsf(off[i]) >= kTie) | (fabsf(off[i + 1]) >= kTie);
+    far = fmaxf(far, fmaxf(fabsf(off[i]), fabsf(off[i + 1])));
   }
   const bool divide = tiny && s > 0.0f;
-  if ((near_tie || divide) && !bad) {
+  if ((far >= kTie || divide) && !bad) {
 #pragma unroll
     for (int i = 0; i < kVals; ++i)
       if (divide || fabsf(off[i]) >= kTie) {
