@@ -8,26 +8,34 @@
 // the token itself and its ancestors (parents).  G = heads / kv_heads query
 // heads share a cached head.
 //
-// The mask only concerns the T newest positions, so the work is split there:
+// The keys of a (sequence, head) -- context, then draft -- are cut into tiles of
+// 128 positions.  The tiles of the whole batch, whatever the lengths, form one
+// list that the persistent CTAs (one per SM) share out evenly; a CTA that ends or
+// starts inside a head leaves a partial (max, sum, output) there, and
+// tree_combine_kernel merges them, one warp per query row.  Every cached byte is
+// read once for a block of rows; that read is the bound.  Only tiles that reach
+// past the context look at the mask: a 64-bit ancestor set per token, found by
+// pointer doubling.
 //
-// * tree_context_kernel: all G * T rows of a (sequence, head) against the
-//   context.  No mask but the context's end.  Every cached byte is read once;
-//   that read is the bound.  The tiles (128 positions of one head) of the whole
-//   batch, whatever the lengths, form one list that the persistent CTAs (one
-//   per SM) share out evenly; a CTA that ends or starts inside a head leaves a
-//   partial (max, sum, output) there.
-//   Warp 0 streams K and V tiles by TMA into a ring of swizzled stages; eight
-//   consumer warps contract them on mma.sync m16n8k16 (the rows of a decode
-//   step fill a fraction of a 128-row tcgen05 tile): each warp scores 16 of the
-//   tile's keys, writes its probabilities to shared memory, and accumulates
-//   its D / 8 output dims over all 128 keys.  The rows' reference maximum is
-//   shared and only raised when a score exceeds it by more than 2^8.
-//   int8 codes become f16 in registers (exact), with the row's scale applied
-//   to the fp32 score (K) and to the probability (V).
-// * tree_combine_kernel: one warp per query row walks the row's ancestors in
-//   fp32 (a few rows of shared memory, no mask arithmetic, so a non-finite
-//   value of one branch cannot reach another), merges the context's partials
-//   and writes the output.
+// Two kernels contract the tiles, by the rows G * T that share a cached head:
+//
+// * tree_mma_kernel, up to 16 rows (and int8 caches): warp 0 streams K and V
+//   tiles by TMA into a ring of swizzled stages; eight consumer warps contract them
+//   on mma.sync m16n8k16 (the rows of a decode step fill a fraction of a 128-row
+//   tcgen05 tile): each warp scores 16 of the tile's keys, writes its
+//   probabilities to shared memory, and accumulates its D / 8 output dims over all
+//   128 keys.  int8 codes become f16 in registers (exact), with the row's scale
+//   applied to the fp32 score (K) and to the probability (V).
+// * tree_tc_kernel, more rows of a 16-bit cache: tcgen05, keys as the 128 lanes:
+//   S^T [128 keys x N rows] = K Q^T and O^T [D x N] += V^T P, N = 32, 64 or 128 rows.
+//   K and V tiles are used as they lie (K-major and M-major operands), the
+//   softmax work grows with the rows, and a thread owns a key: its mask test and
+//   the clean-up of rows past the end are its own.
+//
+// In both, the rows' reference maximum is shared and only raised when a score
+// exceeds it by more than 2^8.  A non-finite value of a drafted token must not
+// reach the tokens that do not see it (0 * inf): it is taken out of the tile, and
+// the combine kernel adds it to the rows that do.
 //
 // The reference has no counterpart: its cache manager is a stub
 // (python_bindings/src/main.cpp:101-135).
@@ -41,6 +49,7 @@ namespace {
 constexpr int kTTile = 128;       // cache positions per tile
 constexpr int kTCons = 8;         // consumer warps
 constexpr int kTBatch = 512;      // sequences per launch
+constexpr int kTMaxGrid = 256;    // CTAs that share the tiles, whatever the device
 constexpr int kTMaxTokens = 64;   // drafted tokens (one 64-bit ancestor mask)
 constexpr float kTRaise = 8.0f;   // log2 of the largest probability before the reference is raised
 
@@ -56,18 +65,18 @@ struct TreeParams {
   const int* lens;
   const int* ntok;
   const int* parents;
-  int B, T, G, kvh, nrb;  // nrb: row blocks per cached head
+  int B, T, G, kvh, nrb, rb;  // nrb: row blocks per cached head, of rb rows
   int64_t P;
   float sl2;
   float* part;
-  int grid;  // CTAs of the context kernel
+  int grid;  // CTAs that share the tiles
   int* err;
 };
 
 template <int D>
-constexpr int part_stride() { return D + 4; }  // output, max, sum (16-byte rows)
+constexpr int part_stride() { return D + 4; }  // output, max, sum, "values were taken out"
 
-// Context length (0: nothing to do) and tokens of sequence b.
+// Context length and tokens (0: nothing to do) of sequence b.
 __device__ __forceinline__ bool tree_seq(const TreeParams& p, int b, int& len, int& n) {
   len = p.lens[b];
   n = p.ntok ? p.ntok[b] : p.T;
@@ -76,14 +85,14 @@ __device__ __forceinline__ bool tree_seq(const TreeParams& p, int b, int& len, i
   return ok;
 }
 
-__device__ __forceinline__ int tiles_of(int len) { return (len + kTTile - 1) / kTTile; }
-template <int RB>
+__device__ __forceinline__ int tiles_of(int len, int n) {
+  return n > 0 ? (len + n - 1) / kTTile + 1 : 0;
+}
 __device__ __forceinline__ int row_blocks(const TreeParams& p, int n) {
-  return (p.G * n + RB - 1) / RB;
+  return (p.G * n + p.rb - 1) / p.rb;
 }
 
 // First tile of every sequence in the batch's list (one warp).
-template <int RB>
 __device__ __forceinline__ void tree_scan(const TreeParams& p, uint32_t* base, int lane) {
   uint32_t carry = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
@@ -92,7 +101,7 @@ __device__ __forceinline__ void tree_scan(const TreeParams& p, uint32_t* base, i
     if (b < p.B) {
       int len, n;
       tree_seq(p, b, len, n);
-      w = static_cast<uint32_t>(p.kvh) * row_blocks<RB>(p, n) * tiles_of(len);
+      w = static_cast<uint32_t>(p.kvh) * row_blocks(p, n) * tiles_of(len, n);
     }
     uint32_t s = w;
 #pragma unroll
@@ -117,9 +126,8 @@ __device__ __forceinline__ uint32_t share_of(uint32_t tile, uint32_t total, uint
 
 // Where tile w of the list lies.
 struct TreeSpan {
-  int b, h, rb, len, rows, tile, tiles;  // tile: index within the head's context
+  int b, h, rb, len, n, rows, tile, tiles;  // tile: index within the head's keys
 };
-template <int RB>
 __device__ __forceinline__ TreeSpan tree_find(const TreeParams& p, const uint32_t* base, uint32_t w) {
   int lo = 0, hi = p.B;  // base[lo] <= w < base[hi]
   while (hi - lo > 1) {
@@ -129,17 +137,100 @@ __device__ __forceinline__ TreeSpan tree_find(const TreeParams& p, const uint32_
   }
   TreeSpan s;
   s.b = lo;
-  int n;
-  tree_seq(p, lo, s.len, n);
-  s.tiles = tiles_of(s.len);
-  const int nrb = row_blocks<RB>(p, n);
+  tree_seq(p, lo, s.len, s.n);
+  s.tiles = tiles_of(s.len, s.n);
+  const int nrb = row_blocks(p, s.n);
   const uint32_t at = w - base[lo];
   const uint32_t item = at / s.tiles;
   s.tile = static_cast<int>(at - item * s.tiles);
   s.h = static_cast<int>(item / nrb);
   s.rb = static_cast<int>(item - s.h * nrb);
-  s.rows = min(RB, p.G * n - s.rb * RB);
+  s.rows = min(p.rb, p.G * s.n - s.rb * p.rb);
   return s;
+}
+
+// Ancestor sets (the token itself included) of the drafted tokens that the rows
+// row0 .. row0 + rows (at most 64) of a sequence belong to, into mask[0 .. rows), by
+// one warp: log2(n) rounds of pointer doubling over the n tokens.  A parent that
+// does not come before its token counts as none and sets the device error word.
+__device__ __forceinline__ void tree_masks(const TreeParams& p, int b, int n, int row0, int rows,
+                                           unsigned long long* mask, int lane) {
+  unsigned long long m[2];
+  int up[2];
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int t = lane + 32 * i;
+    m[i] = 1ull << t;
+    up[i] = t - 1;
+    if (p.parents != nullptr) {
+      up[i] = t < n ? p.parents[static_cast<int64_t>(b) * p.T + t] : -1;
+      if (up[i] >= t || up[i] < -1) {
+        bad = true;
+        up[i] = -1;
+      }
+    }
+  }
+  if (bad) atomicExch(p.err, kErrBadParent);
+#pragma unroll 1
+  for (int reach = 1; reach < n; reach *= 2) {
+    unsigned long long a[2];
+    int nx[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // set and parent of this token's farthest known ancestor
+      const int from = up[i] & 31;
+      const unsigned long long m0 = __shfl_sync(0xffffffffu, m[0], from);
+      const unsigned long long m1 = __shfl_sync(0xffffffffu, m[1], from);
+      const int u0 = __shfl_sync(0xffffffffu, up[0], from);
+      const int u1 = __shfl_sync(0xffffffffu, up[1], from);
+      a[i] = up[i] < 0 ? 0ull : up[i] < 32 ? m0 : m1;
+      nx[i] = up[i] < 0 ? -1 : up[i] < 32 ? u0 : u1;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      m[i] |= a[i];
+      up[i] = nx[i];
+    }
+  }
+  __syncwarp();  // the sets of the segment before have been read
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = lane + 32 * i, tok = (row0 + r) / p.G;
+    const unsigned long long m0 = __shfl_sync(0xffffffffu, m[0], tok & 31);
+    const unsigned long long m1 = __shfl_sync(0xffffffffu, m[1], tok & 31);
+    if (r < rows) mask[r] = tok >= n ? 0ull : tok < 32 ? m0 : m1;
+  }
+  __syncwarp();
+}
+
+// Whether a 16-bit value of a word is not finite: exponent bits all ones.
+template <class T>
+__device__ __forceinline__ uint32_t non_finite_halves(uint32_t w) {
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  uint32_t keep = 0xffffffffu;
+  if ((w & kExp) == kExp) keep &= 0xffff0000u;
+  if (((w >> 16) & kExp) == kExp) keep &= 0x0000ffffu;
+  return keep;
+}
+// One 16-byte unit of a tile's V row: zeroed (`drop`: nothing is there), or
+// without its non-finite values (a drafted token); returns whether any was found.
+template <class T>
+__device__ __forceinline__ bool clean_unit(uint8_t* at, bool drop) {
+  uint4 x = *reinterpret_cast<const uint4*>(at);
+  uint32_t keep[4] = {0u, 0u, 0u, 0u};
+  if (!drop) {
+    keep[0] = non_finite_halves<T>(x.x);
+    keep[1] = non_finite_halves<T>(x.y);
+    keep[2] = non_finite_halves<T>(x.z);
+    keep[3] = non_finite_halves<T>(x.w);
+    if ((keep[0] & keep[1] & keep[2] & keep[3]) == 0xffffffffu) return false;
+  }
+  x.x &= keep[0];
+  x.y &= keep[1];
+  x.z &= keep[2];
+  x.w &= keep[3];
+  *reinterpret_cast<uint4*>(at) = x;
+  return !drop;
 }
 
 // -------------------------------------------------------------- mma helpers --
@@ -210,6 +301,9 @@ __device__ __forceinline__ bool cons_any(bool pred) {
       : "memory");
   return r != 0;
 }
+__device__ __forceinline__ void launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 __device__ __forceinline__ void cons_sync() {
   asm volatile("barrier.cta.sync 1, %0;" ::"n"(kTCons * 32) : "memory");
 }
@@ -227,7 +321,8 @@ struct TreeSmem {
   static constexpr int kOffP = kStages * kStage;                // probabilities [RB][128] 16-bit
   static constexpr int kOffMax = kOffP + RB * kTTile * 2;       // [8][RB] x 2 row maxima, sums
   static constexpr int kOffBase = kOffMax + 2 * kTCons * RB * 4;
-  static constexpr int kOffBar = kOffBase + (kTBatch + 2) * 4;
+  static constexpr int kOffMask = kOffBase + (kTBatch + 2) * 4;  // [8][64] ancestor sets
+  static constexpr int kOffBar = kOffMask + kTCons * kTMaxTokens * 8;
   static constexpr int kOffFlag = kOffBar + 2 * kStages * 8;
   static constexpr int kBytes = kOffFlag + 64 + 1024;
 };
@@ -243,7 +338,7 @@ __device__ __forceinline__ uint32_t tile_unit(int r, int c) {
 
 template <class T, int D, bool Q8, int MT>
 __global__ void __launch_bounds__(32 * (kTCons + 1), 1)
-    tree_context_kernel(const __grid_constant__ CUtensorMap tmK,
+    tree_mma_kernel(const __grid_constant__ CUtensorMap tmK,
                         const __grid_constant__ CUtensorMap tmV, const TreeParams p) {
   using S = TreeSmem<D, Q8, MT>;
   constexpr int NS = S::kStages, KS = D / 16, RB = S::RB;
@@ -259,6 +354,7 @@ __global__ void __launch_bounds__(32 * (kTCons + 1), 1)
   uint64_t* empty = full + NS;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kOffFlag);
   int* wait_ok = reinterpret_cast<int*>(smem + S::kOffFlag) + 1;  // [kTCons]
+  int* taken = wait_ok + kTCons;                                  // by segment parity
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 32) {
@@ -267,12 +363,14 @@ __global__ void __launch_bounds__(32 * (kTCons + 1), 1)
       mbar_init(empty + i, kTCons);
     }
     *abort_flag = 0;
+    taken[0] = taken[1] = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
-  if (warp == 0) tree_scan<RB>(p, base, lane);
+  if (warp == 0) tree_scan(p, base, lane);
   __syncthreads();
+  launch_dependents();
   const uint32_t total = base[p.B];
   if (total == 0) return;
   const uint32_t shares = min(total, gridDim.x);
@@ -286,7 +384,7 @@ __global__ void __launch_bounds__(32 * (kTCons + 1), 1)
       int it = 0;
       bool ok = true;
       for (uint32_t w = w0; ok && w < w1;) {
-        const TreeSpan s = tree_find<RB>(p, base, w);
+        const TreeSpan s = tree_find(p, base, w);
         const int nt = min(static_cast<int>(w1 - w), s.tiles - s.tile);
         const int row = static_cast<int>((static_cast<int64_t>(s.b) * p.kvh + s.h) * p.P) +
                         s.tile * kTTile;
@@ -320,11 +418,16 @@ __global__ void __launch_bounds__(32 * (kTCons + 1), 1)
   // ---- consumers: this warp's keys of a tile are cw * 16 .. + 15
   const int cw = warp - 1, g = lane >> 2, c = lane & 3;
   const uint32_t sP = smem_u32(smem + S::kOffP);
-  int it = 0;
-  for (uint32_t w = w0; w < w1;) {
-    const TreeSpan sp = tree_find<RB>(p, base, w);
+  unsigned long long* mask =
+      reinterpret_cast<unsigned long long*>(smem + S::kOffMask) + cw * kTMaxTokens;
+  int it = 0, seg = 0;
+  for (uint32_t w = w0; w < w1; seg ^= 1) {
+    const TreeSpan sp = tree_find(p, base, w);
     const int nt = min(static_cast<int>(w1 - w), sp.tiles - sp.tile);
     const int64_t head = static_cast<int64_t>(sp.b) * p.kvh + sp.h;
+    const int keys = sp.len + sp.n;
+    if ((sp.tile + nt) * kTTile > sp.len)
+      tree_masks(p, sp.b, sp.n, sp.rb * RB, RB, mask, lane);
     // Q as A fragments.  int8 codes: lane c of a quad holds dims c * D/4 ..
     // (the codes' own order, any order of the dims gives the same products) in
     // f16, each row scaled by a power of two so that its largest value is
@@ -394,7 +497,7 @@ __global__ void __launch_bounds__(32 * (kTCons + 1), 1)
     if constexpr (Q8) {
       scp = (lane < 16 ? p.ks : p.vs) + head * p.P + cw * 16 + (lane & 15);
       const int key = sp.tile * kTTile + cw * 16 + (lane & 15);
-      sc_next = key < sp.len ? __ldg(scp + sp.tile * kTTile) : 0.0f;
+      sc_next = key < keys ? __ldg(scp + sp.tile * kTTile) : 0.0f;
     }
 
     for (int t = 0; t < nt; ++t, ++it) {
@@ -403,8 +506,8 @@ __global__ void __launch_bounds__(32 * (kTCons + 1), 1)
       const float sc = sc_next;
       if constexpr (Q8) {
         if (t + 1 < nt)
-          sc_next = key0 + kTTile + cw * 16 + (lane & 15) < sp.len ? __ldg(scp + key0 + kTTile)
-                                                                   : 0.0f;
+          sc_next = key0 + kTTile + cw * 16 + (lane & 15) < keys ? __ldg(scp + key0 + kTTile)
+                                                                 : 0.0f;
       }
       const bool got = __all_sync(
           0xffffffffu,
@@ -476,19 +579,22 @@ __global__ void __launch_bounds__(32 * (kTCons + 1), 1)
           for (int i = 0; i < 4; ++i) {
             float s = acc[mt][n][i] * qinv[mt][i >> 1];
             if constexpr (Q8) s *= ksc[n][i & 1];
-            if (tail && key0 + cw * 16 + n * 8 + 2 * c + (i & 1) >= sp.len) s = -INFINITY;
+            if (tail) {
+              const int at = key0 + cw * 16 + n * 8 + 2 * c + (i & 1) - sp.len;  // in the draft
+              if (at >= 0 && !(at < sp.n && (mask[mt * 16 + (i >> 1) * 8 + g] >> at & 1ull)))
+                s = -INFINITY;
+            }
             acc[mt][n][i] = s;
             need |= s > mref[mt][i >> 1] + kTRaise;
             if constexpr (Q8) need |= s + lvs[n][i & 1] > eref[mt][i >> 1] + kTRaise;
           }
       if constexpr (!Q8) {
-        // rows past the context may hold anything: 0 * NaN must not reach the sums
-        if (tail) {
+        if (tail && got) {  // rows past the end may hold anything, and drafted ones infinities
           for (int u = lane; u < 16 * (S::kRow / 16); u += 32) {
             const int r = cw * 16 + u / (S::kRow / 16);
-            if (key0 + r >= sp.len)
-              *reinterpret_cast<uint4*>(tv + tile_unit<S>(r, u % (S::kRow / 16))) =
-                  make_uint4(0, 0, 0, 0);
+            if (key0 + r >= sp.len &&
+                clean_unit<T>(tv + tile_unit<S>(r, u % (S::kRow / 16)), key0 + r >= keys))
+              taken[seg] = 1;
           }
         }
       }
@@ -567,7 +673,8 @@ __global__ void __launch_bounds__(32 * (kTCons + 1), 1)
                 // factor only overflows where p is 0.
                 float f = vsc[n][i] * frow[mt][hf];
                 f = f > 3.0e38f ? 3.0e38f : f;
-                x[i] *= f;
+                // a key that the row does not see may have the scale NaN
+                x[i] = acc[mt][n][2 * hf + i] == -INFINITY ? 0.0f : x[i] * f;
               }
             }
             const uint32_t at = sP + r * 256 + (((2 * cw + n) ^ (r & 7)) << 4) + 4 * c;
@@ -676,198 +783,585 @@ __global__ void __launch_bounds__(32 * (kTCons + 1), 1)
             for (int k = 0; k < kTCons; ++k) sum += smax[k * RB + r];
             row[D] = mref[mt][hf];
             row[D + 1] = sum;
+            row[D + 2] = Q8 ? 0.0f : static_cast<float>(taken[seg]);
           }
         }
       }
+    if (cw == 0) {
+      __syncwarp();
+      if (lane == 0) taken[seg] = 0;  // next used two segments on
+    }
     w += nt;
   }
 }
 
-// ----------------------------------------------------------------- combine --
-constexpr int kCRows = 32;  // query rows per CTA of the combine kernel
+// ------------------------------------------------------------ tcgen05 kernel --
+// Shared memory: Q [N rows x D] (K-major), P [128 keys x N] (N contiguous), a ring
+// of 128-position K and V tiles, all in 128-byte-swizzled chunks of 64 columns.
+template <int D, int N>
+struct TcSmem {
+  static constexpr int kTile = kTTile * D * 2;        // K or V tile
+  static constexpr int kQChunk = N * 128;             // N rows x 64 dims
+  static constexpr int kQ = (D / 64) * kQChunk;
+  static constexpr int kPChunk = kTTile * 128;        // 128 keys x 64 rows
+  static constexpr int kP = ((N + 63) / 64) * kPChunk;
+  static constexpr int kOffP = kQ;
+  static constexpr int kOffRing = kOffP + kP;
+  static constexpr int kLeft = 222 * 1024 - kOffRing;
+  static constexpr int kSlots = kLeft / kTile > 8 ? 8 : kLeft / kTile;
+  static constexpr int kOffMax = kOffRing + kSlots * kTile;  // [4][N] maxima / sums
+  static constexpr int kOffRef = kOffMax + 4 * N * 4;        // [N] -reference, [N] factor
+  static constexpr int kOffMask = kOffRef + 2 * N * 4;       // [8][64] ancestor sets
+  static constexpr int kOffBase = kOffMask + 8 * kTMaxTokens * 8;
+  static constexpr int kOffBar = (kOffBase + (kTBatch + 2) * 4 + 7) / 8 * 8;
+  static constexpr int kBars = 2 * kSlots + 8;
+  static constexpr int kOffFlag = kOffBar + kBars * 8;
+  static constexpr int kBytes = kOffFlag + 48 + 1024;
+  // softmax: groups of four warps, each with up to 64 of the block's rows
+  static constexpr int kRows = N < 64 ? N : 64, kGroups = N / kRows;
+  static_assert(kBytes <= 232448, "shared memory of one CTA");
+};
 
-// D / 32 values of a lane from a row in shared memory.
-template <class T, bool Q8, int DL>
-__device__ __forceinline__ void draft_part(const uint8_t* row, int lane, float scale,
-                                           float (&x)[DL]) {
-  if constexpr (Q8) {
-    const int8_t* e = reinterpret_cast<const int8_t*>(row) + lane * DL;
+// Maxima (or sums) over the warp's 32 lanes of v[0 .. 31]; lane i gets that of v[i].
+template <bool SUM>
+__device__ __forceinline__ float across_lanes(float (&v)[32], int lane) {
 #pragma unroll
-    for (int i = 0; i < DL; ++i) x[i] = static_cast<float>(e[i]) * scale;
-  } else {
-    const T* e = reinterpret_cast<const T*>(row) + lane * DL;
+  for (int o = 16; o >= 1; o >>= 1)
 #pragma unroll
-    for (int i = 0; i < DL; ++i) x[i] = to_f32(e[i]);
+    for (int i = 0; i < o; ++i) {
+      const bool up = lane & o;
+      const float give = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+      const float got = __shfl_xor_sync(0xffffffffu, give, o);
+      v[i] = SUM ? keep + got : fmaxf(keep, got);
+    }
+  return v[0];
+}
+
+// Barrier of the softmax warps (THREADS of them); true where any predicate holds.
+template <int THREADS>
+__device__ __forceinline__ bool soft_any(bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(pred)), "n"(THREADS)
+      : "memory");
+  return r != 0;
+}
+template <int THREADS>
+__device__ __forceinline__ void soft_sync() {
+  asm volatile("barrier.cta.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
+
+// warp 0: TMA producer (K(0), V(0), K(1), ... into the ring); warp 1: TMEM and
+// the MMAs, in the order S(0), S(1), O(0), S(2), O(1), ... within a head's
+// segment; warps 4-7 (and 8-11 for the upper 64 of 128 rows): softmax, thread =
+// key = TMEM lane.  TMEM: S^T twice, O^T.  The softmax reads a row block of S twice,
+// 32 rows at a time (for the vote, then for the exponentials), instead of holding it.
+template <class T, int D, int N>
+__global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
+    tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const TreeParams p) {
+  using S = TcSmem<D, N>;
+  constexpr int NS = S::kSlots;
+  constexpr int RW = S::kRows, NC = RW / 32, kSoft = 128 * S::kGroups;
+  constexpr uint32_t kCols = N <= 32 ? 128 : N <= 64 ? 256 : 512;  // 3 N columns
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  float* smax = reinterpret_cast<float*>(smem + S::kOffMax);
+  float* nref = reinterpret_cast<float*>(smem + S::kOffRef);  // -reference (0: none yet)
+  float* fact = nref + N;
+  uint32_t* base = reinterpret_cast<uint32_t*>(smem + S::kOffBase);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kOffBar);
+  uint64_t* empty = full + NS;
+  uint64_t* q_full = empty + NS;  // an arrival per softmax warp: q_full, s_free, p_full
+  uint64_t* s_full = q_full + 1;  // [2]
+  uint64_t* s_free = s_full + 2;  // [2]
+  uint64_t* p_full = s_free + 2;
+  uint64_t* pv_done = p_full + 1;
+  uint64_t* drained = pv_done + 1;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kOffFlag);
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + S::kOffFlag) + 1;
+  int* wait_ok = reinterpret_cast<int*>(tslot) + 1;  // [softmax warps]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < S::kBars; ++i) {
+      const bool per_warp = full + i == q_full || full + i == s_free || full + i == s_free + 1 ||
+                            full + i == p_full;
+      mbar_init(full + i, per_warp ? kSoft / 32 : 1);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tmem_alloc(tslot, kCols);
+  }
+  if (warp == 0) tree_scan(p, base, lane);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  launch_dependents();
+  const uint32_t tmem = *tslot, tO = tmem + 2 * N;
+  const uint32_t total = base[p.B];
+  const uint32_t shares = min(total, gridDim.x);
+  uint32_t w0 = 0, w1 = 0;  // no tiles: every role falls through to the end
+  if (blockIdx.x < shares) {
+    w0 = share_start(blockIdx.x, total, shares);
+    w1 = share_start(blockIdx.x + 1, total, shares);
+  }
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;  // ring slots used
+      bool ok = true;
+      for (uint32_t w = w0; ok && w < w1;) {
+        const TreeSpan s = tree_find(p, base, w);
+        const int nt = min(static_cast<int>(w1 - w), s.tiles - s.tile);
+        const int row = static_cast<int>((static_cast<int64_t>(s.b) * p.kvh + s.h) * p.P) +
+                        s.tile * kTTile;
+        for (int t = 0; ok && t < 2 * nt; ++t) {
+          const int st = it % NS;
+          if (!mbar_wait_bounded(empty + st, ((it / NS) & 1) ^ 1, abort_flag, p.err,
+                                 kErrWaitEmpty)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(full + st, S::kTile);
+          uint8_t* dst = smem + S::kOffRing + st * S::kTile;
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x)
+            tma_load_2d(dst + x * kTTile * 128, (t & 1) ? &tmV : &tmK, full + st, x * 64,
+                        row + (t >> 1) * kTTile);
+          ++it;
+        }
+        w += nt;
+      }
+      if (!ok) {  // let the copies in flight land before the CTA exits
+        volatile int never = 0;
+        for (int j = (it > NS ? it - NS : 0); j < it; ++j)
+          mbar_wait_bounded(full + j % NS, (j / NS) & 1, &never, p.err, kErrWaitOther);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr bool kBF = std::is_same<T, __nv_bfloat16>::value;
+      constexpr uint32_t idS = idesc_f16(128, N, kBF);
+      // A = V^T: M (dims) contiguous; B = P: N (rows) contiguous
+      constexpr uint32_t idO = idesc_f16(128, N, kBF, true) | (1u << 15);
+      // D = 64: the upper 64 lanes repeat the lower ones (chunk stride 0)
+      constexpr uint32_t kVChunk = D == 128 ? kTTile * 128 : 0;
+      const uint32_t aQ = smem_u32(smem), aP = smem_u32(smem + S::kOffP);
+      const uint32_t ring = smem_u32(smem + S::kOffRing);
+      int it = 0, seg = 0;  // tiles, segments so far
+      bool ok = true;
+      auto slot_wait = [&](int slot) {
+        return mbar_wait_bounded(full + slot % NS, (slot / NS) & 1, abort_flag, p.err, kErrWaitFull);
+      };
+      auto issue_s = [&](int j) -> bool {  // tile j of the CTA into S buffer j % 2
+        if (!slot_wait(2 * j)) return false;
+        if (j >= 2 && !mbar_wait_bounded(s_free + (j & 1), ((j >> 1) - 1) & 1, abort_flag, p.err,
+                                         kErrWaitOther))
+          return false;
+        tc_fence_after();
+        const uint32_t aK = ring + (2 * j % NS) * S::kTile;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          tc_mma_f16(tmem + (j & 1) * N,
+                     make_desc_kmajor_sw128(aK + (k >> 2) * kTTile * 128 + (k & 3) * 32),
+                     make_desc_kmajor_sw128(aQ + (k >> 2) * S::kQChunk + (k & 3) * 32), idS, k != 0);
+        tc_commit(s_full + (j & 1));
+        tc_commit(empty + 2 * j % NS);
+        return true;
+      };
+      auto issue_o = [&](int j, bool first) -> bool {
+        if (!mbar_wait_bounded(p_full, j & 1, abort_flag, p.err, kErrWaitFull)) return false;
+        if (!slot_wait(2 * j + 1)) return false;
+        tc_fence_after();
+        const uint32_t aV = ring + ((2 * j + 1) % NS) * S::kTile;
+#pragma unroll
+        for (int k = 0; k < kTTile / 16; ++k)
+          tc_mma_f16(tO, make_desc_mnmajor_sw128(aV + k * 2048, kVChunk),
+                     make_desc_mnmajor_sw128(aP + k * 2048, S::kPChunk), idO, !first || k != 0);
+        tc_commit(pv_done);
+        tc_commit(empty + (2 * j + 1) % NS);
+        return true;
+      };
+      for (uint32_t w = w0; ok && w < w1; ++seg) {
+        const TreeSpan s = tree_find(p, base, w);
+        const int nt = min(static_cast<int>(w1 - w), s.tiles - s.tile);
+        ok = mbar_wait_bounded(q_full, seg & 1, abort_flag, p.err, kErrWaitFull);
+        if (ok) ok = issue_s(it);
+        for (int t = 0; ok && t < nt; ++t) {
+          if (t + 1 < nt) ok = issue_s(it + t + 1);
+          if (ok) ok = issue_o(it + t, t == 0);
+        }
+        it += nt;
+        w += nt;
+      }
+      if (!ok) {  // what was issued completes before TMEM and shared memory go
+        volatile int never = 0;
+        tc_commit(drained);
+        mbar_wait_bounded(drained, 0, &never, p.err, kErrWaitOther);
+      }
+    }
+  } else if (warp >= 4) {
+    // ---- softmax: key `kt` of every tile, rows r0 .. r0 + RW
+    const int sw = warp - 4, q4 = warp & 3, kt = q4 * 32 + lane, tid = threadIdx.x - 128;
+    const int r0 = (sw >> 2) * RW;
+    const uint32_t lane_off = static_cast<uint32_t>(q4 * 32) << 16;
+    unsigned long long* mask =
+        reinterpret_cast<unsigned long long*>(smem + S::kOffMask) + sw * kTMaxTokens;
+    auto wait_warp = [&](uint64_t* bar, uint32_t parity) -> bool {
+      const bool r = mbar_wait_bounded(bar, parity, abort_flag, p.err, kErrWaitAccum);
+      return __all_sync(0xffffffffu, r);
+    };
+    int it = 0;
+    bool ok = true;
+    for (uint32_t w = w0; ok && w < w1;) {
+      const TreeSpan sp = tree_find(p, base, w);
+      const int nt = min(static_cast<int>(w1 - w), sp.tiles - sp.tile);
+      const int64_t head = static_cast<int64_t>(sp.b) * p.kvh + sp.h;
+      bool taken = false;
+      if ((sp.tile + nt) * kTTile > sp.len)
+        tree_masks(p, sp.b, sp.n, sp.rb * N + r0, RW, mask, lane);
+      // Q into its swizzled chunks (the last scores of the segment before have been
+      // read, so its MMAs are done); rows past the block are zeros
+      for (int u = tid; u < N * (D / 8); u += kSoft) {
+        const int r = u / (D / 8), x = u % (D / 8);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < sp.rows) {
+          const int rr = sp.rb * N + r, t = rr / p.G;
+          const T* qp = static_cast<const T*>(p.q) + sp.b * p.qb + t * p.qt +
+                        (static_cast<int64_t>(sp.h) * p.G + (rr - t * p.G)) * p.qh;
+          v = __ldg(reinterpret_cast<const uint4*>(qp) + x);
+        }
+        *reinterpret_cast<uint4*>(smem + (x >> 3) * S::kQChunk + r * 128 +
+                                  (((x & 7) ^ (r & 7)) << 4)) = v;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      float l[RW];
+#pragma unroll
+      for (int i = 0; i < RW; ++i) l[i] = 0.0f;
+
+      for (int t = 0; t < nt; ++t, ++it) {
+        const int at = (sp.tile + t) * kTTile + kt - sp.len;  // this key's place in the draft
+        const bool tail = (sp.tile + t + 1) * kTTile > sp.len, first = t == 0;
+        bool got = wait_warp(s_full + (it & 1), (it >> 1) & 1);
+        tc_fence_after();
+        // scores of 32 rows; a row sees a drafted key if its token's set holds it
+        auto scores = [&](int c, uint32_t (&s)[32]) {
+          tmem_ld_32x32b_x32(tmem + (it & 1) * N + lane_off + r0 + c * 32, s);
+          tmem_wait_ld_tie(s);
+          if (tail && at >= 0) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(at < sp.n && (mask[c * 32 + i] >> at & 1ull)))
+                s[i] = __float_as_uint(-INFINITY);
+          }
+        };
+        if (tail && got && sw < 4) {  // this thread's V row, once it has landed
+          const int slot = 2 * it + 1;
+          got = wait_warp(full + slot % NS, (slot / NS) & 1);
+          if (got && at >= 0) {
+            uint8_t* tv = smem + S::kOffRing + (slot % NS) * S::kTile;
+#pragma unroll 1
+            for (int u = 0; u < D / 8; ++u)
+              taken |= clean_unit<T>(tv + (u >> 3) * kTTile * 128 + kt * 128 +
+                                         (((u & 7) ^ (kt & 7)) << 4), at >= sp.n);
+          }
+        }
+        // ---- does a score pass its row's reference by more than the margin?
+        bool need = first || !got;
+        if (!need) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            uint32_t s[32];
+            scores(c, s);
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 nr = *reinterpret_cast<const float4*>(nref + r0 + c * 32 + i);
+              top = fmaxf(top, fmaxf(fmaf(__uint_as_float(s[i]), p.sl2, nr.x),
+                                     fmaf(__uint_as_float(s[i + 1]), p.sl2, nr.y)));
+              top = fmaxf(top, fmaxf(fmaf(__uint_as_float(s[i + 2]), p.sl2, nr.z),
+                                     fmaf(__uint_as_float(s[i + 3]), p.sl2, nr.w)));
+            }
+          }
+          need = top > kTRaise;
+        }
+        if (soft_any<kSoft>(need)) {
+          if (got) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              uint32_t s[32];
+              scores(c, s);
+              float v[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(s[i]);
+              smax[q4 * N + r0 + c * 32 + lane] = across_lanes<false>(v, lane);
+            }
+          }
+          if (lane == 0) wait_ok[sw] = got;
+          soft_sync<kSoft>();
+          bool all_ok = true;
+#pragma unroll
+          for (int k = 0; k < kSoft / 32; ++k) all_ok &= wait_ok[k] != 0;
+          if (!all_ok) {  // a wait ran out: the softmax warps leave together
+            ok = false;
+            break;
+          }
+          if (tid < N) {
+            const float top = fmaxf(fmaxf(smax[tid], smax[N + tid]),
+                                    fmaxf(smax[2 * N + tid], smax[3 * N + tid])) * p.sl2;
+            const float old = first ? -INFINITY : -nref[tid];
+            const float now = fmaxf(old, top);
+            // a row without a score above -inf keeps 0: its probabilities are 0 (or NaN)
+            nref[tid] = now == -INFINITY ? 0.0f : -now;
+            fact[tid] = first ? 0.0f : ex2_approx(old - now);
+          }
+          soft_sync<kSoft>();
+          // O is final up to the tile before; rescale it and the sums (where the wait
+          // runs out, the next vote ends the segment)
+          if (!first && wait_warp(pv_done, (it - 1) & 1)) {
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              uint32_t ov[32];
+              tmem_ld_32x32b_x32(tO + lane_off + r0 + c * 32, ov);
+              tmem_wait_ld_tie(ov);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float f = fact[r0 + c * 32 + i];
+                ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
+                l[c * 32 + i] *= f;
+              }
+              tmem_st_32x32b_x32(tO + lane_off + r0 + c * 32, ov);
+            }
+            tmem_wait_st();
+          }
+        }
+        // ---- probabilities, their sums, and P (16 bits, this key's row)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          uint32_t s[32], pk[16];
+          scores(c, s);
+          if (c == NC - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_free + (it & 1));  // S may be overwritten
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 nr = *reinterpret_cast<const float4*>(nref + r0 + c * 32 + i);
+            const float e0 = ex2_approx(fmaf(__uint_as_float(s[i]), p.sl2, nr.x));
+            const float e1 = ex2_approx(fmaf(__uint_as_float(s[i + 1]), p.sl2, nr.y));
+            const float e2 = ex2_approx(fmaf(__uint_as_float(s[i + 2]), p.sl2, nr.z));
+            const float e3 = ex2_approx(fmaf(__uint_as_float(s[i + 3]), p.sl2, nr.w));
+            l[c * 32 + i] += e0;
+            l[c * 32 + i + 1] += e1;
+            l[c * 32 + i + 2] += e2;
+            l[c * 32 + i + 3] += e3;
+            pk[i / 2] = pack16<std::is_same<T, __nv_bfloat16>::value>(e0, e1);
+            pk[i / 2 + 1] = pack16<std::is_same<T, __nv_bfloat16>::value>(e2, e3);
+          }
+          // P is free once the tile before has been contracted
+          if (c == 0 && !first) wait_warp(pv_done, (it - 1) & 1);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int u = (r0 + c * 32) / 8 + x;
+            *reinterpret_cast<uint4*>(smem + S::kOffP + (u >> 3) * S::kPChunk + kt * 128 +
+                                      (((u & 7) ^ (kt & 7)) << 4)) =
+                make_uint4(pk[4 * x], pk[4 * x + 1], pk[4 * x + 2], pk[4 * x + 3]);
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full);
+      }
+      if (!ok) break;
+      // ---- the segment's partial
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = l[c * 32 + i];
+        smax[q4 * N + r0 + c * 32 + lane] = across_lanes<true>(v, lane);
+      }
+      const bool any_taken = soft_any<kSoft>(taken);
+      ok = wait_warp(pv_done, (it - 1) & 1);
+      if (ok) {
+        tc_fence_after();
+        const int64_t item = head * p.nrb + sp.rb;
+        float* pp = p.part + (static_cast<int64_t>(blockIdx.x) + item) * N * part_stride<D>();
+        if (tid < sp.rows) {
+          float* row = pp + tid * part_stride<D>();
+          row[D] = -nref[tid];
+          row[D + 1] = (smax[tid] + smax[N + tid]) + (smax[2 * N + tid] + smax[3 * N + tid]);
+          row[D + 2] = any_taken ? 1.0f : 0.0f;
+        }
+        if (D == 128 || q4 < 2) {  // thread = output dim
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            uint32_t ov[32];
+            tmem_ld_32x32b_x32(tO + lane_off + r0 + c * 32, ov);
+            tmem_wait_ld_tie(ov);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (r0 + c * 32 + i < sp.rows)
+                pp[(r0 + c * 32 + i) * part_stride<D>() + kt] = __uint_as_float(ov[i]);
+          }
+        }
+        tc_fence_before();
+      }
+      // nref, smax and O are used again by the next segment only after this
+      if (soft_any<kSoft>(!ok)) ok = false;
+      w += nt;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kCols);
   }
 }
 
-template <class T, int D, bool Q8, int RB>
-__global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
+// ----------------------------------------------------------------- combine --
+constexpr int kCWarps = 8;  // query rows per CTA
+
+// One warp per query row: its block's partials are those of consecutive shares.
+template <class T, int D>
+__global__ void __launch_bounds__(32 * kCWarps) tree_combine_kernel(const TreeParams p) {
   constexpr int DL = D / 32;
-  constexpr int kRow = D * (Q8 ? 1 : 2), kUnits = kRow / 16;
-  extern __shared__ __align__(16) uint8_t draft[];  // K rows, V rows of the drafted tokens
   __shared__ uint32_t base[kTBatch + 2];
-  __shared__ float scales[2][kTMaxTokens];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int bh = blockIdx.x, b = bh / p.kvh, h = bh % p.kvh;
-  int len, n;
-  const bool valid = tree_seq(p, b, len, n);
-  if (!valid && h == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicExch(p.err, kErrBadCacheLen);
-  if (warp == 0) tree_scan<RB>(p, base, lane);
-  const int64_t row0 = static_cast<int64_t>(bh) * p.P + len;
-  uint8_t* sk = draft;
-  uint8_t* sv = draft + p.T * kRow;
-  for (int i = threadIdx.x; i < 2 * n * kUnits; i += blockDim.x) {
-    const int u = i < n * kUnits ? i : i - n * kUnits;
-    const uint8_t* src = static_cast<const uint8_t*>(i < n * kUnits ? p.kc : p.vc) + row0 * kRow;
-    reinterpret_cast<uint4*>(i < n * kUnits ? sk : sv)[u] =
-        __ldg(reinterpret_cast<const uint4*>(src) + u);
-  }
-  if constexpr (Q8) {
-    for (int i = threadIdx.x; i < 2 * n; i += blockDim.x)
-      scales[i >= n][i >= n ? i - n : i] = __ldg((i >= n ? p.vs : p.ks) + row0 + (i >= n ? i - n : i));
-  }
+  if (warp == 0) tree_scan(p, base, lane);
   __syncthreads();
   const uint32_t total = base[p.B];
   const uint32_t shares = min(total, static_cast<uint32_t>(p.grid));
-  const int tiles = tiles_of(len), nrb = row_blocks<RB>(p, n);
-  const int r1 = min(p.G * p.T, (static_cast<int>(blockIdx.y) + 1) * kCRows);
-  for (int r = blockIdx.y * kCRows + warp; r < r1; r += blockDim.x >> 5) {
-    const int t = r / p.G, gg = r - t * p.G;
-    const int head = h * p.G + gg;
-    T* og = static_cast<T*>(p.o) + b * p.ob + t * p.ot + head * p.oh + lane * DL;
-    float acc[DL], m = -INFINITY, l = 0.0f;
+  const int R = p.G * p.T;
+  const int row = blockIdx.x * kCWarps + warp;
+  if (row >= p.B * p.kvh * R) return;
+  const int bh = row / R, r = row - bh * R;
+  const int b = bh / p.kvh, h = bh - b * p.kvh;
+  const int t = r / p.G, head = h * p.G + (r - t * p.G);
+  int len, n;
+  const bool valid = tree_seq(p, b, len, n);
+  if (!valid && h == 0 && r == 0 && lane == 0) atomicExch(p.err, kErrBadCacheLen);
+  float acc[DL], m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < DL; ++i) acc[i] = 0.0f;
-    if (t < n) {
-      const T* qp = static_cast<const T*>(p.q) + b * p.qb + t * p.qt + head * p.qh + lane * DL;
-      float q[DL];
+  for (int i = 0; i < DL; ++i) acc[i] = 0.0f;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the partials are complete
+  if (t < n) {
+    const int rb = r / p.rb, tiles = tiles_of(len, n), nrb = row_blocks(p, n);
+    const uint32_t t0 = base[b] + (static_cast<uint32_t>(h) * nrb + rb) * tiles;
+    const uint32_t c0 = share_of(t0, total, shares), c1 = share_of(t0 + tiles - 1, total, shares);
+    const int64_t item = static_cast<int64_t>(bh) * p.nrb + rb;
+    const float* pr = p.part + ((c0 + item) * p.rb + (r - rb * p.rb)) * part_stride<D>();
+    bool taken = false;
+    for (uint32_t c = c0; c <= c1; ++c, pr += static_cast<int64_t>(p.rb) * part_stride<D>()) {
+      const float4 st = *reinterpret_cast<const float4*>(pr + D);  // max, sum, taken
+      float x[DL];
 #pragma unroll
-      for (int i = 0; i < DL; ++i) q[i] = to_f32(qp[i]);
-      // ancestors of token t (itself included) as a 64-bit mask
-      unsigned long long mask = 0ull;
-      if (p.parents == nullptr) {
-        mask = t == 63 ? ~0ull : (1ull << (t + 1)) - 1ull;
-      } else {
-        const int* par = p.parents + static_cast<int64_t>(b) * p.T;
-        const int p_lo = lane < n ? par[lane] : -1, p_hi = lane + 32 < n ? par[lane + 32] : -1;
-        for (int a = t; a >= 0;) {
-          mask |= 1ull << a;
-          const int lo = __shfl_sync(0xffffffffu, p_lo, a & 31);
-          const int hi = __shfl_sync(0xffffffffu, p_hi, a & 31);
-          int up = a < 32 ? lo : hi;
-          if (up >= a || up < -1) {  // not a tree: the token counts as a root
-            if (lane == 0) atomicExch(p.err, kErrBadParent);
-            up = -1;
-          }
-          a = up;
+      for (int i = 0; i < DL; ++i) x[i] = pr[lane * DL + i];
+      const float mn = fmaxf(m, st.x);
+      const float ref = mn == -INFINITY ? 0.0f : mn;
+      const float fa = exp2f(m - ref), fb = exp2f(st.x - ref);
+      l = l * fa + st.y * fb;
+#pragma unroll
+      for (int i = 0; i < DL; ++i) acc[i] = acc[i] * fa + x[i] * fb;
+      m = mn;
+      taken |= st.z != 0.0f;
+    }
+    if (taken) {
+      // infinities and NaN of the drafted values that this token sees
+      const T* v = static_cast<const T*>(p.vc) + (static_cast<int64_t>(bh) * p.P + len) * D + lane * DL;
+      for (int a = t, steps = 0; a >= 0 && steps < kTMaxTokens; ++steps) {
+#pragma unroll
+        for (int i = 0; i < DL; ++i) {
+          const float x = to_f32(v[static_cast<int64_t>(a) * D + i]);
+          if (!(fabsf(x) <= 3.402823466e38f)) acc[i] += x;
         }
-      }
-      // scores of the ancestors: lane a & 31 keeps that of token a
-      float s_lo = -INFINITY, s_hi = -INFINITY;
-      for (unsigned long long left = mask; left != 0ull;) {
-        int a[4];
-        float d[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          a[k] = left != 0ull ? __ffsll(left) - 1 : -1;
-          left &= left - 1ull;  // 0 stays 0
-          float x[DL];
-          const int at = a[k] < 0 ? t : a[k];
-          draft_part<T, Q8, DL>(sk + at * kRow, lane, Q8 ? scales[0][at] : 1.0f, x);
-          d[k] = 0.0f;
-#pragma unroll
-          for (int i = 0; i < DL; ++i) d[k] = fmaf(q[i], x[i], d[k]);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) d[k] += __shfl_xor_sync(0xffffffffu, d[k], o);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (a[k] >= 0 && (a[k] & 31) == lane) (a[k] < 32 ? s_lo : s_hi) = d[k] * p.sl2;
-      }
-      m = fmaxf(s_lo, s_hi);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float mu = m == -INFINITY ? 0.0f : m;
-      // a NaN score must stay one: lanes without an ancestor add 0
-      const bool has_lo = (mask >> lane) & 1ull, has_hi = (mask >> (lane + 32)) & 1ull;
-      const float e_lo = has_lo ? exp2f(s_lo - mu) : 0.0f, e_hi = has_hi ? exp2f(s_hi - mu) : 0.0f;
-      l = e_lo + e_hi;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      for (unsigned long long left = mask; left != 0ull; left &= left - 1ull) {
-        const int a = __ffsll(left) - 1;
-        const float lo = __shfl_sync(0xffffffffu, e_lo, a & 31);
-        const float hi = __shfl_sync(0xffffffffu, e_hi, a & 31);
-        const float e = a < 32 ? lo : hi;
-        float x[DL];
-        draft_part<T, Q8, DL>(sv + a * kRow, lane, Q8 ? scales[1][a] : 1.0f, x);
-#pragma unroll
-        for (int i = 0; i < DL; ++i) acc[i] = fmaf(e, x[i], acc[i]);
-      }
-      // the context's partials of this row's block
-      if (tiles > 0) {
-        const int rb = r / RB;
-        const uint32_t t0 = base[b] + (static_cast<uint32_t>(h) * nrb + rb) * tiles;
-        const uint32_t c0 = share_of(t0, total, shares);
-        const uint32_t c1 = share_of(t0 + tiles - 1, total, shares);
-        const int64_t item = static_cast<int64_t>(bh) * p.nrb + rb;
-        const float* pr = p.part + ((c0 + item) * RB + (r - rb * RB)) * part_stride<D>();
-        for (uint32_t cc = c0; cc <= c1; ++cc, pr += RB * part_stride<D>()) {
-          const float pm = pr[D], pl = pr[D + 1];
-          float x[DL];
-#pragma unroll
-          for (int i = 0; i < DL; ++i) x[i] = pr[lane * DL + i];
-          const float mn = fmaxf(m, pm);
-          const float ref = mn == -INFINITY ? 0.0f : mn;
-          const float fa = exp2f(m - ref), fb = exp2f(pm - ref);
-          l = l * fa + pl * fb;
-#pragma unroll
-          for (int i = 0; i < DL; ++i) acc[i] = acc[i] * fa + x[i] * fb;
-          m = mn;
-        }
+        const int up = p.parents ? p.parents[static_cast<int64_t>(b) * p.T + a] : a - 1;
+        a = up < a ? up : -1;
       }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a NaN sum stays one
-#pragma unroll
-    for (int i = 0; i < DL; ++i) og[i] = from_f32<T>(acc[i] * inv);
   }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a NaN sum stays one
+  T* og = static_cast<T*>(p.o) + b * p.ob + t * p.ot + head * p.oh + lane * DL;
+  T y[DL];
+#pragma unroll
+  for (int i = 0; i < DL; ++i) y[i] = from_f32<T>(acc[i] * inv);
+  if constexpr (DL == 4) *reinterpret_cast<uint2*>(og) = *reinterpret_cast<const uint2*>(y);
+  else *reinterpret_cast<uint32_t*>(og) = *reinterpret_cast<const uint32_t*>(y);
 }
 
 // ---------------------------------------------------------------- launchers --
-int row_tiles(int G, int T) { return G * T <= 16 ? 1 : 2; }  // 16-row tiles per block
+// Rows of a block.  Up to 16 rows go to mma.sync in one block, in which the other rows of a
+// 16-row tile are idle; int8 caches to blocks of 32.  More rows of a 16-bit cache go
+// to tcgen05 in the smallest block that holds them (at most 128).
+int block_rows(int rows, bool q8) {
+  if (rows <= 16) return 16;
+  if (rows <= 32 || q8) return 32;
+  return rows <= 64 ? 64 : 128;
+}
 
-size_t tree_slots(int B, int T, int G, int kvh, int grid, int& nrb) {
-  const int RB = 16 * row_tiles(G, T);
-  nrb = (G * T + RB - 1) / RB;
+size_t tree_slots(int B, int T, int G, int kvh, int grid, int rb, int& nrb) {
+  nrb = (G * T + rb - 1) / rb;
   return static_cast<size_t>(B) * kvh * nrb + grid;
 }
 
+template <class T, int D>
+void launch_combine(const TreeParams& p, cudaStream_t st) {
+  const int64_t rows = static_cast<int64_t>(p.B) * p.kvh * p.G * p.T;
+  // launched while the tiles are still contracted; it waits for them on the device
+  launch_dependent(tree_combine_kernel<T, D>,
+                   dim3(static_cast<unsigned>((rows + kCWarps - 1) / kCWarps)), 32 * kCWarps, 0, st,
+                   p);
+  check_launch("tree_combine_kernel", st);
+}
+
 template <class T, int D, bool Q8, int MT>
-void launch_tree(const TreeParams& p, cudaStream_t st) {
+void launch_mma(const TreeParams& p, cudaStream_t st) {
   using S = TreeSmem<D, Q8, MT>;
-  const CUtensorMapDataType dt = Q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                 : std::is_same<T, __nv_bfloat16>::value
-                                     ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUtensorMapDataType dt = Q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : tma_dtype_of<T>();
   const uint64_t rows = static_cast<uint64_t>(p.B) * p.kvh * p.P;
   const CUtensorMapSwizzle sw =
       S::kBox == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   CUtensorMap tk, tv;
   make_tma_2d(&tk, p.kc, dt, Q8 ? 1 : 2, rows, D, D, S::kBox / (Q8 ? 1 : 2), kTTile, sw);
   make_tma_2d(&tv, p.vc, dt, Q8 ? 1 : 2, rows, D, D, S::kBox / (Q8 ? 1 : 2), kTTile, sw);
-  auto kern = tree_context_kernel<T, D, Q8, MT>;
+  auto kern = tree_mma_kernel<T, D, Q8, MT>;
   LTM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
   kern<<<p.grid, 32 * (kTCons + 1), S::kBytes, st>>>(tk, tv, p);
-  check_launch("tree_context_kernel", st);
-  auto comb = tree_combine_kernel<T, D, Q8, 16 * MT>;
-  const int R = p.G * p.T;
-  const int warps = R < 8 ? R : 8;
-  const dim3 grid(static_cast<unsigned>(p.B) * p.kvh, (R + kCRows - 1) / kCRows);
-  comb<<<grid, 32 * warps, 2 * p.T * S::kRow, st>>>(p);
-  check_launch("tree_combine_kernel", st);
+  check_launch("tree_mma_kernel", st);
+  launch_combine<T, D>(p, st);
+}
+
+template <class T, int D, int N>
+void launch_tc(const TreeParams& p, cudaStream_t st) {
+  using S = TcSmem<D, N>;
+  const uint64_t rows = static_cast<uint64_t>(p.B) * p.kvh * p.P;
+  CUtensorMap tk, tv;
+  make_tma_2d(&tk, p.kc, tma_dtype_of<T>(), 2, rows, D, D, 64, kTTile);
+  make_tma_2d(&tv, p.vc, tma_dtype_of<T>(), 2, rows, D, D, 64, kTTile);
+  auto kern = tree_tc_kernel<T, D, N>;
+  LTM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
+  kern<<<p.grid, 128 + 128 * S::kGroups, S::kBytes, st>>>(tk, tv, p);
+  check_launch("tree_tc_kernel", st);
+  launch_combine<T, D>(p, st);
 }
 
 }  // namespace
@@ -893,9 +1387,13 @@ extern "C" ltm_status ltm_tree_attention_workspace(int B, int T, int num_heads, 
     check_tree(B, T, num_heads, kv_heads, head_dim, 1);
     const int G = num_heads / kv_heads;
     int nrb = 0;
-    // a context kernel never has more CTAs than this device-independent cap
-    const size_t slots = tree_slots(B < kTBatch ? B : kTBatch, T, G, kv_heads, 256, nrb);
-    *bytes = slots * 16 * row_tiles(G, T) * (head_dim + 4) * sizeof(float);
+    size_t most = 0;
+    for (int q8 = 0; q8 < 2; ++q8) {
+      const int rb = block_rows(G * T, q8 != 0);
+      const size_t n = tree_slots(B < kTBatch ? B : kTBatch, T, G, kv_heads, kTMaxGrid, rb, nrb) * rb;
+      if (n > most) most = n;
+    }
+    *bytes = most * (head_dim + 4) * sizeof(float);
   });
 }
 
@@ -922,8 +1420,8 @@ extern "C" ltm_status ltm_tree_attention(
       LTM_REQUIRE(q_strides[i] % 8 == 0 && o_strides[i] % 8 == 0,
                   "q and output strides must be multiples of 8 elements");
     const int G = num_heads / kv_heads;
-    const int mt = row_tiles(G, T);
     const bool q8 = k_scale != nullptr;
+    const int rb = block_rows(G * T, q8);
     TreeParams p{};
     p.qt = q_strides[1];
     p.qh = q_strides[2];
@@ -946,13 +1444,13 @@ extern "C" ltm_status ltm_tree_attention(
       LTM_REQUIRE(static_cast<int64_t>(p.B) * kv_heads * max_positions < (1ll << 31),
                   "cache rows exceed int32");
       const int64_t most = static_cast<int64_t>(p.B) * kv_heads *
-                           ((G * T + 16 * mt - 1) / (16 * mt)) *
-                           ((max_positions + kTTile - 1) / kTTile);
+                           ((G * T + rb - 1) / rb) * ((max_positions + kTTile - 1) / kTTile);
       LTM_REQUIRE(most < (1ll << 31), "too many tiles");
-      const int sms = device_sm_count() < 256 ? device_sm_count() : 256;
+      const int sms = device_sm_count() < kTMaxGrid ? device_sm_count() : kTMaxGrid;
       p.grid = static_cast<int>(most < sms ? most : sms);
-      const size_t slots = tree_slots(p.B, T, G, kv_heads, p.grid, p.nrb);
-      LTM_REQUIRE(workspace_bytes >= slots * 16 * mt * (head_dim + 4) * sizeof(float),
+      p.rb = rb;
+      const size_t slots = tree_slots(p.B, T, G, kv_heads, p.grid, rb, p.nrb);
+      LTM_REQUIRE(workspace_bytes >= slots * rb * (head_dim + 4) * sizeof(float),
                   "workspace too small");
       p.q = static_cast<const uint8_t*>(q) + 2 * b0 * p.qb;
       p.o = static_cast<uint8_t*>(o) + 2 * b0 * p.ob;
@@ -967,8 +1465,15 @@ extern "C" ltm_status ltm_tree_attention(
         using E = decltype(t_c);
         constexpr int D = decltype(d_c)::value;
         constexpr bool Q = decltype(q_c)::value;
-        if (mt == 1) launch_tree<E, D, Q, 1>(p, st);
-        else launch_tree<E, D, Q, 2>(p, st);
+        if (rb == 16) {
+          launch_mma<E, D, Q, 1>(p, st);
+        } else if constexpr (Q) {
+          launch_mma<E, D, Q, 2>(p, st);
+        } else {
+          if (rb == 32) launch_tc<E, D, 32>(p, st);
+          else if (rb == 64) launch_tc<E, D, 64>(p, st);
+          else launch_tc<E, D, 128>(p, st);
+        }
       };
       auto by_q = [&](auto t_c, auto d_c) {
         if (q8) go(t_c, d_c, std::true_type{});

@@ -214,6 +214,38 @@ def test_non_finite_values_stay_where_they_are_seen(ltm):
     assert torch.isnan(got[1]).all()
 
 
+@pytest.mark.parametrize("dt,cache,G,d", [("f16", "same", 4, 64), ("bf16", "same", 12, 128),
+                                         ("bf16", "same", 21, 64), ("bf16", "int8", 2, 128),
+                                         ("f16", "int8", 4, 64)])
+def test_non_finite_drafts_with_more_rows(ltm, dt, cache, G, d):
+    """The same with 12 to 126 rows per cached head, and with int8 rows whose scale is NaN
+    (what the append makes of a non-finite row)."""
+    import torch
+    B, T, kvh = 2, 6, 2
+    lens = [126, 300]  # the first draft crosses a tile
+    par = [[-1, 0, 0, 1, 2, -1]] * 2
+    q, k, v, ks, vs, vk, vv = make(B, T, kvh * G, kvh, d, 310, dt, cache, lens, 13)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    args = (torch.tensor(lens, **i32), torch.tensor(par, **i32), ks, vs)
+    clean = ltm.tree_attention(q, k, v, *args)
+    for b in range(B):
+        if cache == "int8":
+            vs[b, :, lens[b] + 1] = float("nan")
+            ks[b, :, lens[b] + 5] = float("nan")
+        else:
+            v[b, :, lens[b] + 1, ::3] = float("-inf")
+            v[b, :, lens[b] + 1, 1::3] = float("nan")
+            v[b, :, lens[b] + 1, 2::3] = float("inf")
+            k[b, :, lens[b] + 5] = float("inf")
+            k[b, :, lens[b] + 5, 0] = float("nan")
+    got = ltm.tree_attention(q, k, v, *args)
+    for t in (0, 2, 4):
+        assert torch.equal(got[:, t], clean[:, t])
+    for t in (1, 3):
+        assert not torch.isfinite(got[:, t]).any()
+    assert torch.isnan(got[:, 5]).all()
+
+
 def test_bad_lengths_and_parents(ltm):
     import torch
     B, T, h, d, dt = 4, 3, 2, 64, "bf16"
