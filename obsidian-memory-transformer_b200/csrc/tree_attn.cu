@@ -1033,18 +1033,26 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
       if ((sp.tile + nt) * kTTile > sp.len)
         tree_masks(p, sp.b, sp.n, sp.rb * N + r0, RW, mask, lane);
       // Q into its swizzled chunks (the last scores of the segment before have been
-      // read, so its MMAs are done); rows past the block are zeros
-      for (int u = tid; u < N * (D / 8); u += kSoft) {
-        const int r = u / (D / 8), x = u % (D / 8);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < sp.rows) {
+      // read, so its MMAs are done), all loads in flight together; rows past the
+      // block are zeros
+      {
+        constexpr int U = D / 8, NQ = N * U / kSoft;  // 16-byte units per row / thread
+        uint4 v[NQ];
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+          const int r = (tid + i * kSoft) / U, x = (tid + i * kSoft) % U;
           const int rr = sp.rb * N + r, t = rr / p.G;
           const T* qp = static_cast<const T*>(p.q) + sp.b * p.qb + t * p.qt +
                         (static_cast<int64_t>(sp.h) * p.G + (rr - t * p.G)) * p.qh;
-          v = __ldg(reinterpret_cast<const uint4*>(qp) + x);
+          v[i] = r < sp.rows ? __ldg(reinterpret_cast<const uint4*>(qp) + x)
+                             : make_uint4(0, 0, 0, 0);
         }
-        *reinterpret_cast<uint4*>(smem + (x >> 3) * S::kQChunk + r * 128 +
-                                  (((x & 7) ^ (r & 7)) << 4)) = v;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+          const int r = (tid + i * kSoft) / U, x = (tid + i * kSoft) % U;
+          *reinterpret_cast<uint4*>(smem + (x >> 3) * S::kQChunk + r * 128 +
+                                    (((x & 7) ^ (r & 7)) << 4)) = v[i];
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -1056,25 +1064,33 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
       for (int t = 0; t < nt; ++t, ++it) {
         const int at = (sp.tile + t) * kTTile + kt - sp.len;  // this key's place in the draft
         const bool tail = (sp.tile + t + 1) * kTTile > sp.len, first = t == 0;
+        // the rows that see this key, as bits: all of a context key, of a drafted one those
+        // whose token's set holds it
+        unsigned long long seen = ~0ull;
+        if (tail && at >= 0) {
+          seen = 0ull;
+          if (at < sp.n)
+#pragma unroll 8
+            for (int i = 0; i < RW; ++i) seen |= (mask[i] >> at & 1ull) << i;
+        }
         bool got = wait_warp(s_full + (it & 1), (it >> 1) & 1);
         tc_fence_after();
-        // scores of 32 rows; a row sees a drafted key if its token's set holds it
         auto scores = [&](int c, uint32_t (&s)[32]) {
           tmem_ld_32x32b_x32(tmem + (it & 1) * N + lane_off + r0 + c * 32, s);
           tmem_wait_ld_tie(s);
-          if (tail && at >= 0) {
+          if (tail) {
+            const uint32_t bits = static_cast<uint32_t>(seen >> (32 * c));
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (!(at < sp.n && (mask[c * 32 + i] >> at & 1ull)))
-                s[i] = __float_as_uint(-INFINITY);
+              if (!(bits >> i & 1u)) s[i] = __float_as_uint(-INFINITY);
           }
-        };
+        };  // scores of 32 rows
         if (tail && got && sw < 4) {  // this thread's V row, once it has landed
           const int slot = 2 * it + 1;
           got = wait_warp(full + slot % NS, (slot / NS) & 1);
           if (got && at >= 0) {
             uint8_t* tv = smem + S::kOffRing + (slot % NS) * S::kTile;
-#pragma unroll 1
+#pragma unroll 4
             for (int u = 0; u < D / 8; ++u)
               taken |= clean_unit<T>(tv + (u >> 3) * kTTile * 128 + kt * 128 +
                                          (((u & 7) ^ (kt & 7)) << 4), at >= sp.n);
