@@ -20,11 +20,14 @@
 // Two kernels contract the tiles, by the rows G * T that share a cached head:
 //
 // * tree_mma_kernel, up to 16 rows (and int8 caches): warp 0 streams K and V
-//   tiles by TMA into a ring of swizzled stages; eight consumer warps contract them
-//   on mma.sync m16n8k16 (the rows of a decode step fill a fraction of a 128-row
-//   tcgen05 tile): each warp scores 16 of the tile's keys, writes its
-//   probabilities to shared memory, and accumulates its D / 8 output dims over all
-//   128 keys.  int8 codes become f16 in registers (exact), with the row's scale
+//   tiles by TMA into a ring of swizzled slots; the consumer warps contract them on
+//   mma.sync m16n8k16 with the keys as M (a decode step's few rows are the 8 or 16
+//   columns; a 128-row tcgen05 tile would idle).  A warp takes 16 of a tile's keys
+//   through S^T = K Q^T, softmax and O^T += V^T P^T on its own; P^T is S^T's
+//   accumulator transposed in registers.  Nothing is exchanged until the segment's
+//   end, where the warps' (max, sum, output) are merged in shared memory.  Up to 8
+//   rows leave registers for 16 consumer warps, two sets that take turns at the tiles;
+//   more rows run 8.  int8 codes become f16 in registers (exact), with the row's scale
 //   applied to the fp32 score (K) and to the probability (V).
 // * tree_tc_kernel, more rows of a 16-bit cache: tcgen05, keys as the 128 lanes:
 //   S^T [128 keys x N rows] = K Q^T and O^T [D x N] += V^T P, N = 32, 64 or 128 rows.
@@ -32,8 +35,8 @@
 //   softmax work grows with the rows, and a thread owns a key: its mask test and
 //   the clean-up of rows past the end are its own.
 //
-// In both, the rows' reference maximum is shared and only raised when a score
-// exceeds it by more than 2^8.  A non-finite value of a drafted token must not
+// In both, a row's reference maximum is only raised when a score exceeds it by more
+// than 2^8.  A non-finite value of a drafted token must not
 // reach the tokens that do not see it (0 * inf): it is taken out of the tile, and
 // the combine kernel adds it to the rows that do.
 //
@@ -47,7 +50,6 @@ namespace ltm_b200 {
 namespace {
 
 constexpr int kTTile = 128;       // cache positions per tile
-constexpr int kTCons = 8;         // consumer warps
 constexpr int kTBatch = 512;      // sequences per launch
 constexpr int kTMaxGrid = 256;    // CTAs that share the tiles, whatever the device
 constexpr int kTMaxTokens = 64;   // drafted tokens (one 64-bit ancestor mask)
@@ -278,6 +280,13 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t biased, uint32_t sel) {
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x64806480u));
   return r;
 }
+// Power of two that brings the largest magnitude `am` of a query row to
+// [2^14, 2^15) (1 where it is 0 or not finite).
+__device__ __forceinline__ float query_scale(float am) {
+  int ex = static_cast<int>(__float_as_uint(am) >> 23);  // 2^(ex-127) <= am
+  if (ex == 0 || ex == 255) ex = 141;
+  return __uint_as_float(static_cast<uint32_t>(min(268 - ex, 254)) << 23);
+}
 template <bool BF>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   if constexpr (BF) {
@@ -288,43 +297,40 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return *reinterpret_cast<uint32_t*>(&h);
   }
 }
-// Barrier of the consumer warps; true where any thread's predicate holds.
-__device__ __forceinline__ bool cons_any(bool pred) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(static_cast<uint32_t>(pred)), "n"(kTCons * 32)
-      : "memory");
-  return r != 0;
-}
 __device__ __forceinline__ void launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
+template <int THREADS>
 __device__ __forceinline__ void cons_sync() {
-  asm volatile("barrier.cta.sync 1, %0;" ::"n"(kTCons * 32) : "memory");
+  asm volatile("barrier.cta.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
+// 8 x 8 16-bit transpose over the warp (a row of two values per lane).
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
-// ------------------------------------------------------------ shared memory --
-template <int D, bool Q8, int MT>
-struct TreeSmem {
-  static constexpr int kRow = D * (Q8 ? 1 : 2);                 // bytes per cached row
-  static constexpr int kBox = kRow > 128 ? 128 : kRow;          // bytes per row of a TMA box
+// ----------------------------------------------------------- mma.sync kernel --
+constexpr int kMRows = 16;  // most rows of a block
+
+template <int D, bool Q8, int NR>  // NR: 8-row columns of a block
+struct MmaSmem {
+  static constexpr int kWarps = NR == 1 ? 16 : 8;          // consumers
+  static constexpr int kRows = 8 * NR;
+  static constexpr int kRow = D * (Q8 ? 1 : 2);            // bytes per cached row
+  static constexpr int kBox = kRow > 128 ? 128 : kRow;     // bytes per row of a TMA box
   static constexpr int kBoxes = kRow / kBox;
-  static constexpr int kTile = kTTile * kRow;                   // K or V tile
-  static constexpr int kStage = 2 * kTile;
-  static constexpr int kStages = 196608 / kStage > 8 ? 8 : 196608 / kStage;
-  static constexpr int RB = 16 * MT;
-  static constexpr int kOffP = kStages * kStage;                // probabilities [RB][128] 16-bit
-  static constexpr int kOffMax = kOffP + RB * kTTile * 2;       // [8][RB] x 2 row maxima, sums
-  static constexpr int kOffBase = kOffMax + 2 * kTCons * RB * 4;
-  static constexpr int kOffMask = kOffBase + (kTBatch + 2) * 4;  // [8][64] ancestor sets
-  static constexpr int kOffBar = kOffMask + kTCons * kTMaxTokens * 8;
-  static constexpr int kOffFlag = kOffBar + 2 * kStages * 8;
-  static constexpr int kBytes = kOffFlag + 64 + 1024;
+  static constexpr int kTile = kTTile * kRow;              // K or V tile
+  static constexpr int kSlots = 131072 / kTile > 8 ? 8 : 131072 / kTile;
+  static constexpr int kMergeRow = D + 4;                  // output, max, sum
+  static constexpr int kOffMerge = kSlots * kTile;         // [warps][rows]
+  static constexpr int kOffMask = kOffMerge + kWarps * kRows * kMergeRow * 4;  // [warps][rows]
+  static constexpr int kOffBase = kOffMask + kWarps * kRows * 8;
+  static constexpr int kOffBar = kOffBase + (kTBatch + 2) * 4;
+  static constexpr int kOffFlag = kOffBar + 2 * kSlots * 8;
+  static constexpr int kBytes = kOffFlag + 96 + 1024;
+  static_assert(kBytes <= 232448, "shared memory of one CTA");
 };
 
 // Shared-memory offset of 16-byte unit c of row r of a tile (the TMA swizzle).
@@ -336,34 +342,33 @@ __device__ __forceinline__ uint32_t tile_unit(int r, int c) {
     return static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
-template <class T, int D, bool Q8, int MT>
-__global__ void __launch_bounds__(32 * (kTCons + 1), 1)
+template <class T, int D, bool Q8, int NR>
+__global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
     tree_mma_kernel(const __grid_constant__ CUtensorMap tmK,
-                        const __grid_constant__ CUtensorMap tmV, const TreeParams p) {
-  using S = TreeSmem<D, Q8, MT>;
-  constexpr int NS = S::kStages, KS = D / 16, RB = S::RB;
-  constexpr int NO = D / 64;  // 8-dim output blocks per warp
+                    const __grid_constant__ CUtensorMap tmV, const TreeParams p) {
+  using S = MmaSmem<D, Q8, NR>;
+  constexpr int NS = S::kSlots, KS = D / 16, NU = D / 16, NW = S::kWarps, NG = NW / 8;
+  constexpr int ROWS = S::kRows;
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value && !Q8;  // type of the products
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  float* smax = reinterpret_cast<float*>(smem + S::kOffMax);  // [kTCons][RB]
-  float* sevm = smax + kTCons * RB;                           // [kTCons][RB]
+  float* merge = reinterpret_cast<float*>(smem + S::kOffMerge);
   uint32_t* base = reinterpret_cast<uint32_t*>(smem + S::kOffBase);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kOffBar);
   uint64_t* empty = full + NS;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kOffFlag);
-  int* wait_ok = reinterpret_cast<int*>(smem + S::kOffFlag) + 1;  // [kTCons]
-  int* taken = wait_ok + kTCons;                                  // by segment parity
+  int* wait_ok = reinterpret_cast<int*>(smem + S::kOffFlag) + 1;  // [NW]
+  int* taken = wait_ok + NW;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 32) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, kTCons);
+      mbar_init(empty + i, 8);
     }
     *abort_flag = 0;
-    taken[0] = taken[1] = 0;
+    *taken = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -372,14 +377,13 @@ __global__ void __launch_bounds__(32 * (kTCons + 1), 1)
   __syncthreads();
   launch_dependents();
   const uint32_t total = base[p.B];
-  if (total == 0) return;
   const uint32_t shares = min(total, gridDim.x);
   if (blockIdx.x >= shares) return;
   const uint32_t w0 = share_start(blockIdx.x, total, shares);
   const uint32_t w1 = share_start(blockIdx.x + 1, total, shares);
 
   if (warp == 0) {
-    // ---- producer
+    // ---- producer: K(0), V(0), K(1), ... into the ring
     if (lane == 0) {
       int it = 0;
       bool ok = true;
@@ -388,21 +392,20 @@ __global__ void __launch_bounds__(32 * (kTCons + 1), 1)
         const int nt = min(static_cast<int>(w1 - w), s.tiles - s.tile);
         const int row = static_cast<int>((static_cast<int64_t>(s.b) * p.kvh + s.h) * p.P) +
                         s.tile * kTTile;
-        for (int t = 0; t < nt; ++t, ++it) {
+        for (int t = 0; t < 2 * nt; ++t) {
           const int st = it % NS;
           if (!mbar_wait_bounded(empty + st, ((it / NS) & 1) ^ 1, abort_flag, p.err,
                                  kErrWaitEmpty)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(full + st, S::kStage);
-          uint8_t* dst = smem + st * S::kStage;
+          mbar_arrive_expect_tx(full + st, S::kTile);
+          uint8_t* dst = smem + st * S::kTile;
 #pragma unroll
-          for (int x = 0; x < S::kBoxes; ++x) {
-            tma_load_2d(dst + x * kTTile * 128, &tmK, full + st, x * 64, row + t * kTTile);
-            tma_load_2d(dst + S::kTile + x * kTTile * 128, &tmV, full + st, x * 64,
-                        row + t * kTTile);
-          }
+          for (int x = 0; x < S::kBoxes; ++x)
+            tma_load_2d(dst + x * kTTile * 128, (t & 1) ? &tmV : &tmK, full + st, x * 64,
+                        row + (t >> 1) * kTTile);
+          ++it;
         }
         w += nt;
       }
@@ -415,382 +418,338 @@ __global__ void __launch_bounds__(32 * (kTCons + 1), 1)
     return;
   }
 
-  // ---- consumers: this warp's keys of a tile are cw * 16 .. + 15
-  const int cw = warp - 1, g = lane >> 2, c = lane & 3;
-  const uint32_t sP = smem_u32(smem + S::kOffP);
-  unsigned long long* mask =
-      reinterpret_cast<unsigned long long*>(smem + S::kOffMask) + cw * kTMaxTokens;
-  int it = 0, seg = 0;
-  for (uint32_t w = w0; w < w1; seg ^= 1) {
+  // ---- consumers: keys wk .. wk + 15 of every NG-th tile
+  const int cw = warp - 1, g = lane >> 2, c = lane & 3, i8 = lane >> 3, r8 = lane & 7;
+  const int wk = (cw & 7) * 16, ct = threadIdx.x - 32;
+  unsigned long long* mask = reinterpret_cast<unsigned long long*>(smem + S::kOffMask) + cw * ROWS;
+  int it = 0;  // the CTA's tiles so far
+  for (uint32_t w = w0; w < w1;) {
     const TreeSpan sp = tree_find(p, base, w);
     const int nt = min(static_cast<int>(w1 - w), sp.tiles - sp.tile);
     const int64_t head = static_cast<int64_t>(sp.b) * p.kvh + sp.h;
     const int keys = sp.len + sp.n;
-    if ((sp.tile + nt) * kTTile > sp.len)
-      tree_masks(p, sp.b, sp.n, sp.rb * RB, RB, mask, lane);
-    // Q as A fragments.  int8 codes: lane c of a quad holds dims c * D/4 ..
-    // (the codes' own order, any order of the dims gives the same products) in
-    // f16, each row scaled by a power of two so that its largest value is
-    // below 2^15 (bf16 values reach beyond f16; the scale is undone in fp32).
-    uint32_t aq[MT][KS][4];
-    float qinv[MT][2];
+    const int t_first = (cw / 8 - it % NG + NG) % NG;  // this warp's first tile of the segment
+    // the scales of this warp's 16 keys (K in lanes 0-15, V in lanes 16-31), loaded
+    // kAhead of its tiles before their use: a tile's time is less than a load takes
+    constexpr int kAhead = 3;
+    float sc_next[kAhead];
+    auto load_scale = [&](int t) -> float {
+      const int key = (sp.tile + t) * kTTile + wk + (lane & 15);
+      return key < keys ? __ldg((lane < 16 ? p.ks : p.vs) + head * p.P + key) : 0.0f;
+    };
+    if constexpr (Q8)
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int i = 0; i < kAhead; ++i) sc_next[i] = load_scale(t_first + i * NG);
+    // Q as B fragments (row g of each 8-row column).  int8 codes: lane c of a quad
+    // holds dims c * D/4 .. (the codes' own order, any order of the dims gives the
+    // same products) in f16, each row scaled by a power of two so that its largest value
+    // is below 2^15 (bf16 values reach beyond f16; the scale is undone in fp32).
+    uint32_t bq[NR][KS][2];
+    float qinv[NR][2];  // of rows 2c, 2c + 1
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int r = mt * 16 + hf * 8 + g;
-        const int rr = sp.rb * RB + r;
-        const int t = rr / p.G, gg = rr - t * p.G;
-        const T* qp = static_cast<const T*>(p.q) + sp.b * p.qb + t * p.qt +
-                      (static_cast<int64_t>(sp.h) * p.G + gg) * p.qh;
-        const bool live = r < sp.rows;
-        if constexpr (!Q8) {
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            aq[mt][s][hf] = live ? *reinterpret_cast<const uint32_t*>(qp + s * 16 + 2 * c) : 0u;
-            aq[mt][s][hf + 2] =
-                live ? *reinterpret_cast<const uint32_t*>(qp + s * 16 + 8 + 2 * c) : 0u;
-          }
-          qinv[mt][hf] = p.sl2;
-        } else {
-          uint2 raw[KS];
-          float am = 0.0f;
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            raw[s] = live ? *reinterpret_cast<const uint2*>(qp + c * (D / 4) + 4 * s)
-                          : make_uint2(0u, 0u);
-            const T* e = reinterpret_cast<const T*>(&raw[s]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) am = fmaxf(am, fabsf(to_f32(e[i])));
-          }
-          am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
-          am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
-          int ex = static_cast<int>(__float_as_uint(am) >> 23);  // 2^(ex-127) <= am
-          if (ex == 0 || ex == 255) ex = 141;                     // 0 or infinite: as it is
-          const float qs = __uint_as_float(static_cast<uint32_t>(min(268 - ex, 254)) << 23);
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            const T* e = reinterpret_cast<const T*>(&raw[s]);
-            aq[mt][s][hf] = pack16<false>(to_f32(e[0]) * qs, to_f32(e[1]) * qs);
-            aq[mt][s][hf + 2] = pack16<false>(to_f32(e[2]) * qs, to_f32(e[3]) * qs);
-          }
-          qinv[mt][hf] = p.sl2 / qs;
-        }
-      }
-    float o[MT][NO][4], l[MT][2], mref[MT][2], eref[MT][2], frow[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-      for (int n = 0; n < NO; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[mt][n][i] = 0.0f;
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        l[mt][hf] = 0.0f;
-        mref[mt][hf] = eref[mt][hf] = -INFINITY;
-        frow[mt][hf] = 0.0f;
-      }
-    }
-    // the scales of this warp's 16 keys: K in lanes 0-15, V in lanes 16-31
-    const float* scp = nullptr;
-    float sc_next = 0.0f;
-    if constexpr (Q8) {
-      scp = (lane < 16 ? p.ks : p.vs) + head * p.P + cw * 16 + (lane & 15);
-      const int key = sp.tile * kTTile + cw * 16 + (lane & 15);
-      sc_next = key < keys ? __ldg(scp + sp.tile * kTTile) : 0.0f;
-    }
-
-    for (int t = 0; t < nt; ++t, ++it) {
-      const int st = it % NS;
-      const int key0 = (sp.tile + t) * kTTile;
-      const float sc = sc_next;
-      if constexpr (Q8) {
-        if (t + 1 < nt)
-          sc_next = key0 + kTTile + cw * 16 + (lane & 15) < keys ? __ldg(scp + key0 + kTTile)
-                                                                 : 0.0f;
-      }
-      const bool got = __all_sync(
-          0xffffffffu,
-          mbar_wait_bounded(full + st, (it / NS) & 1, abort_flag, p.err, kErrWaitFull));
-      uint8_t* tk = smem + st * S::kStage;
-      uint8_t* tv = tk + S::kTile;
-      const uint32_t ak = smem_u32(tk), av = smem_u32(tv);
-      const bool tail = key0 + kTTile > sp.len;
-
-      // ---- scores of this warp's 16 keys
-      float acc[MT][2][4];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[mt][n][i] = 0.0f;
+    for (int nr = 0; nr < NR; ++nr) {
+      const int r = nr * 8 + g, rr = sp.rb * p.rb + r;
+      const int t = rr / p.G, gg = rr - t * p.G;
+      const T* qp = static_cast<const T*>(p.q) + sp.b * p.qb + t * p.qt +
+                    (static_cast<int64_t>(sp.h) * p.G + gg) * p.qh;
+      const bool live = r < sp.rows;
       if constexpr (!Q8) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          uint32_t kb[4];
-          const int i = lane >> 3;
-          ldsm4(ak + tile_unit<S>(cw * 16 + (i >> 1) * 8 + (lane & 7), 2 * s + (i & 1)), kb);
+          bq[nr][s][0] = live ? *reinterpret_cast<const uint32_t*>(qp + s * 16 + 2 * c) : 0u;
+          bq[nr][s][1] = live ? *reinterpret_cast<const uint32_t*>(qp + s * 16 + 8 + 2 * c) : 0u;
+        }
+        qinv[nr][0] = qinv[nr][1] = p.sl2;
+      } else {
+        uint4 raw[KS / 2];
+        float am = 0.0f;
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            mma16816<BF>(acc[mt][0], aq[mt][s], kb[0], kb[1]);
-            mma16816<BF>(acc[mt][1], aq[mt][s], kb[2], kb[3]);
-          }
+        for (int s = 0; s < KS / 2; ++s) {
+          raw[s] = live ? *reinterpret_cast<const uint4*>(qp + c * (D / 4) + 8 * s)
+                        : make_uint4(0u, 0u, 0u, 0u);
+          const T* e = reinterpret_cast<const T*>(&raw[s]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) am = fmaxf(am, fabsf(to_f32(e[i])));
+        }
+        am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
+        am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
+        const float qs = query_scale(am), inv = p.sl2 / qs;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const T* e = reinterpret_cast<const T*>(&raw[s / 2]) + (s & 1) * 4;
+          bq[nr][s][0] = pack16<false>(to_f32(e[0]) * qs, to_f32(e[1]) * qs);
+          bq[nr][s][1] = pack16<false>(to_f32(e[2]) * qs, to_f32(e[3]) * qs);
+        }
+        qinv[nr][0] = __shfl_sync(0xffffffffu, inv, 8 * c);
+        qinv[nr][1] = __shfl_sync(0xffffffffu, inv, 8 * c + 4);
+      }
+    }
+    if ((sp.tile + nt) * kTTile > sp.len)
+      tree_masks(p, sp.b, sp.n, sp.rb * p.rb, ROWS, mask, lane);
+    // o[nr][u]: dims of 16-byte-pair u (rows of the A tile) x rows 2c, 2c + 1
+    float o[NR][NU][4], l[NR][2], mref[NR][2], eref[NR][2], frow[NR][2];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nr][u][i] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        l[nr][j] = frow[nr][j] = 0.0f;
+        mref[nr][j] = eref[nr][j] = -INFINITY;
+      }
+    }
+
+    bool ok = true;
+    for (int t = t_first; t < nt; t += NG) {
+      const int sk = 2 * (it + t), sv = sk + 1;
+      const int key0 = (sp.tile + t) * kTTile + wk;
+      float ks[2] = {1.0f, 1.0f}, vsc[2], lvs[2];
+      if constexpr (Q8) {
+        const float sc = sc_next[0];
+#pragma unroll
+        for (int i = 0; i + 1 < kAhead; ++i) sc_next[i] = sc_next[i + 1];
+        sc_next[kAhead - 1] = load_scale(t + kAhead * NG);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // keys g, g + 8
+          ks[h] = __shfl_sync(0xffffffffu, sc, g + 8 * h);
+          vsc[h] = __shfl_sync(0xffffffffu, sc, 16 + g + 8 * h);
+          asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lvs[h]) : "f"(vsc[h]));
+        }
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(full + sk % NS, (sk / NS) & 1, abort_flag,
+                                                     p.err, kErrWaitFull));
+      if (!ok) break;
+      const uint32_t ak = smem_u32(smem + (sk % NS) * S::kTile);
+      const bool tail = key0 + 16 > sp.len;
+
+      // ---- S^T: keys g, g + 8 x rows 2c, 2c + 1
+      float acc[NR][4];
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[nr][i] = 0.0f;
+      if constexpr (!Q8) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          uint32_t ka[4];
+          ldsm4(ak + tile_unit<S>(wk + (i8 & 1) * 8 + r8, 2 * s + (i8 >> 1)), ka);
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr) mma16816<BF>(acc[nr], ka, bq[nr][s][0], bq[nr][s][1]);
         }
       } else {
-        constexpr int NU = D / 64;  // 16-byte units per lane and key
+        constexpr int NL = D / 64;  // 16-byte units per lane and key
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int u = 0; u < NU; ++u) {
-            const uint4 raw = lds128(ak + tile_unit<S>(cw * 16 + n * 8 + g, NU * c + u));
-            const uint32_t wd[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t x = wd[i] ^ 0x80808080u;
-              const uint32_t b0 = codes_f16(x, 0x4140), b1 = codes_f16(x, 0x4342);
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt)
-                mma16816<false>(acc[mt][n], aq[mt][4 * u + i], b0, b1);
-            }
-          }
-      }
-      // ---- log2 scores; does any pass the reference by more than the margin?
-      float ksc[2][2], vsc[2][2], lvs[2][2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if constexpr (Q8) {
-            ksc[n][i] = __shfl_sync(0xffffffffu, sc, n * 8 + 2 * c + i);
-            vsc[n][i] = __shfl_sync(0xffffffffu, sc, 16 + n * 8 + 2 * c + i);
-            lvs[n][i] = __log2f(vsc[n][i]);
-          } else {
-            ksc[n][i] = vsc[n][i] = 1.0f;
-            lvs[n][i] = 0.0f;
-          }
-        }
-      bool need = !got;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int u = 0; u < NL; ++u) {
+          const uint4 lo = lds128(ak + tile_unit<S>(wk + g, NL * c + u));
+          const uint4 hi = lds128(ak + tile_unit<S>(wk + 8 + g, NL * c + u));
+          const uint32_t a[4] = {lo.x, lo.y, lo.z, lo.w}, b[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float s = acc[mt][n][i] * qinv[mt][i >> 1];
-            if constexpr (Q8) s *= ksc[n][i & 1];
-            if (tail) {
-              const int at = key0 + cw * 16 + n * 8 + 2 * c + (i & 1) - sp.len;  // in the draft
-              if (at >= 0 && !(at < sp.n && (mask[mt * 16 + (i >> 1) * 8 + g] >> at & 1ull)))
-                s = -INFINITY;
-            }
-            acc[mt][n][i] = s;
-            need |= s > mref[mt][i >> 1] + kTRaise;
-            if constexpr (Q8) need |= s + lvs[n][i & 1] > eref[mt][i >> 1] + kTRaise;
-          }
-      if constexpr (!Q8) {
-        if (tail && got) {  // rows past the end may hold anything, and drafted ones infinities
-          for (int u = lane; u < 16 * (S::kRow / 16); u += 32) {
-            const int r = cw * 16 + u / (S::kRow / 16);
-            if (key0 + r >= sp.len &&
-                clean_unit<T>(tv + tile_unit<S>(r, u % (S::kRow / 16)), key0 + r >= keys))
-              taken[seg] = 1;
+            const uint32_t x = a[i] ^ 0x80808080u, y = b[i] ^ 0x80808080u;
+            const uint32_t ka[4] = {codes_f16(x, 0x4140), codes_f16(y, 0x4140),
+                                    codes_f16(x, 0x4342), codes_f16(y, 0x4342)};
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr)
+              mma16816<false>(acc[nr], ka, bq[nr][4 * u + i][0], bq[nr][4 * u + i][1]);
           }
         }
       }
-      if (cons_any(need)) {
-        // raise the references to the tile's maxima (and rescale what is summed)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + sk % NS);
+      // ---- log2 scores; does any pass its row's reference by more than the margin?
+      bool need = false;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+      for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            float a = -INFINITY, e = -INFINITY;
+        for (int j = 0; j < 2; ++j) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+          for (int h = 0; h < 2; ++h) {
+            float s = acc[nr][2 * h + j] * qinv[nr][j];
+            if constexpr (Q8) s *= ks[h];
+            if (tail) {
+              const int at = key0 + g + 8 * h - sp.len;  // place in the draft
+              if (at >= 0 && !(at < sp.n && (mask[nr * 8 + 2 * c + j] >> at & 1ull)))
+                s = -INFINITY;
+            }
+            acc[nr][2 * h + j] = s;
+          }
+          need |= fmaxf(acc[nr][j], acc[nr][2 + j]) > mref[nr][j] + kTRaise;
+          if constexpr (Q8)
+            need |= fmaxf(acc[nr][j] + lvs[0], acc[nr][2 + j] + lvs[1]) > eref[nr][j] + kTRaise;
+        }
+      if (__any_sync(0xffffffffu, need)) {
+        // raise the references to the maxima (and rescale what is summed)
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                a = fmaxf(a, acc[mt][n][2 * hf + i]);
-                if constexpr (Q8) e = fmaxf(e, acc[mt][n][2 * hf + i] + lvs[n][i]);
-              }
+        for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-            for (int x = 1; x < 4; x <<= 1) {
+          for (int j = 0; j < 2; ++j) {
+            float a = fmaxf(mref[nr][j], fmaxf(acc[nr][j], acc[nr][2 + j]));
+            float e = eref[nr][j];
+            if constexpr (Q8)
+              e = fmaxf(e, fmaxf(acc[nr][j] + lvs[0], acc[nr][2 + j] + lvs[1]));
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
               a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, x));
               if constexpr (Q8) e = fmaxf(e, __shfl_xor_sync(0xffffffffu, e, x));
             }
-            if (c == 0) {
-              smax[cw * RB + mt * 16 + hf * 8 + g] = a;
-              if constexpr (Q8) sevm[cw * RB + mt * 16 + hf * 8 + g] = e;
-            }
-          }
-        if (lane == 0) wait_ok[cw] = got;
-        cons_sync();
-        bool all_ok = true;
-#pragma unroll
-        for (int k = 0; k < kTCons; ++k) all_ok &= wait_ok[k] != 0;
-        if (!all_ok) return;  // a wait ran out: every consumer leaves here
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const int r = mt * 16 + hf * 8 + g;
-            float a = mref[mt][hf], e = eref[mt][hf];
-#pragma unroll
-            for (int k = 0; k < kTCons; ++k) {
-              a = fmaxf(a, smax[k * RB + r]);
-              if constexpr (Q8) e = fmaxf(e, sevm[k * RB + r]);
-            }
-            const float fl = mref[mt][hf] == -INFINITY ? 0.0f : ex2_approx(mref[mt][hf] - a);
+            const float fl = mref[nr][j] == -INFINITY ? 0.0f : ex2_approx(mref[nr][j] - a);
             float fo = fl;
             if constexpr (Q8)
-              fo = eref[mt][hf] == -INFINITY ? 0.0f : ex2_approx(eref[mt][hf] - e);
-            l[mt][hf] *= fl;
+              fo = eref[nr][j] == -INFINITY ? 0.0f : ex2_approx(eref[nr][j] - e);
+            l[nr][j] *= fl;
 #pragma unroll
-            for (int n = 0; n < NO; ++n) {
-              o[mt][n][2 * hf] *= fo;
-              o[mt][n][2 * hf + 1] *= fo;
+            for (int u = 0; u < NU; ++u) {
+              o[nr][u][j] *= fo;
+              o[nr][u][2 + j] *= fo;
             }
-            mref[mt][hf] = a;
-            eref[mt][hf] = e;
-            if constexpr (Q8) frow[mt][hf] = e == -INFINITY ? 0.0f : ex2_approx(a - e);
+            mref[nr][j] = a;
+            eref[nr][j] = e;
+            if constexpr (Q8) frow[nr][j] = e == -INFINITY ? 0.0f : ex2_approx(a - e);
           }
       }
-      // ---- probabilities into shared memory
+      // ---- probabilities, transposed to the B fragment of the value product
+      uint32_t bp[NR][2];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int r = mt * 16 + hf * 8 + g;
-          const float mu = mref[mt][hf] == -INFINITY ? 0.0f : mref[mt][hf];
+        for (int h = 0; h < 2; ++h) {
+          float x[2];
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            float x[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              x[i] = ex2_approx(acc[mt][n][2 * hf + i] - mu);
-              l[mt][hf] += x[i];
-              if constexpr (Q8) {
-                // p * v's scale, against its own reference: at most 2^8.  The
-                // factor only overflows where p is 0.
-                float f = vsc[n][i] * frow[mt][hf];
-                f = f > 3.0e38f ? 3.0e38f : f;
-                // a key that the row does not see may have the scale NaN
-                x[i] = acc[mt][n][2 * hf + i] == -INFINITY ? 0.0f : x[i] * f;
-              }
+          for (int j = 0; j < 2; ++j) {
+            const float s = acc[nr][2 * h + j];
+            x[j] = ex2_approx(s - (mref[nr][j] == -INFINITY ? 0.0f : mref[nr][j]));
+            l[nr][j] += x[j];
+            if constexpr (Q8) {
+              // p * v's scale, against its own reference: at most 2^8.  The factor only
+              // overflows where p is 0.  A scale NaN becomes an infinity here, and a NaN by
+              // its row's zero codes; a row that does not see the key takes nothing of it.
+              x[j] *= fminf(vsc[h] * frow[nr][j], 3.0e38f);
+              if (tail && s == -INFINITY) x[j] = 0.0f;
             }
-            const uint32_t at = sP + r * 256 + (((2 * cw + n) ^ (r & 7)) << 4) + 4 * c;
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(pack16<BF>(x[0], x[1]))
-                         : "memory");
+          }
+          bp[nr][h] = transpose8x8(pack16<BF>(x[0], x[1]));
+        }
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(full + sv % NS, (sv / NS) & 1, abort_flag,
+                                                     p.err, kErrWaitFull));
+      if (!ok) break;
+      uint8_t* tv = smem + (sv % NS) * S::kTile;
+      const uint32_t av = smem_u32(tv);
+      if constexpr (!Q8) {
+        if (tail) {  // rows past the end may hold anything, and drafted ones infinities
+          for (int u = lane; u < 16 * (S::kRow / 16); u += 32) {
+            const int r = u / (S::kRow / 16);
+            if (key0 + r >= sp.len &&
+                clean_unit<T>(tv + tile_unit<S>(wk + r, u % (S::kRow / 16)), key0 + r >= keys))
+              *taken = 1;
+          }
+          __syncwarp();
+        }
+      }
+      // ---- O^T += V^T P^T, 16 dims at a time
+      if constexpr (!Q8) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          uint32_t va[4];
+          ldsm4_t(av + tile_unit<S>(wk + (i8 >> 1) * 8 + r8, 2 * u + (i8 & 1)), va);
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr) mma16816<BF>(o[nr][u], va, bp[nr][0], bp[nr][1]);
+        }
+      } else {
+        // a 16-byte unit holds 16 dims; the transposed 16-bit element is a pair of
+        // neighbouring dims: the even ones become rows 0-7 of the A tile, the odd ones 8-15
+#pragma unroll
+        for (int u = 0; u < NU; u += 2) {
+          uint32_t vb[4];
+          ldsm4_t(av + tile_unit<S>(wk + (i8 & 1) * 8 + r8, u + (i8 >> 1)), vb);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t y0 = vb[2 * x] ^ 0x80808080u, y1 = vb[2 * x + 1] ^ 0x80808080u;
+            const uint32_t va[4] = {codes_f16(y0, 0x4240), codes_f16(y0, 0x4341),
+                                    codes_f16(y1, 0x4240), codes_f16(y1, 0x4341)};
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr)
+              mma16816<false>(o[nr][u + x], va, bp[nr][0], bp[nr][1]);
           }
         }
-      cons_sync();
-      // ---- output dims of this warp over the tile's 128 keys
-      const int i8 = lane >> 3, r8 = lane & 7;
-#pragma unroll
-      for (int s2 = 0; s2 < kTTile / 32; ++s2) {
-        uint32_t vb[2][NO][2];  // [16-key step][output block][k half]
-        if constexpr (!Q8 && D == 128) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t r[4];
-            ldsm4_t(av + tile_unit<S>(32 * s2 + 16 * h + (i8 & 1) * 8 + r8, 2 * cw + (i8 >> 1)), r);
-            vb[h][0][0] = r[0];
-            vb[h][0][1] = r[1];
-            vb[h][NO - 1][0] = r[2];
-            vb[h][NO - 1][1] = r[3];
-          }
-        } else {
-          // int8: 16-byte units hold 16 dims; the transposed 16-bit element is
-          // a pair of neighbouring dims, split into an even and an odd block
-          uint32_t r[4];
-          const int unit = Q8 ? (D == 128 ? cw : cw >> 1) : cw;
-          ldsm4_t(av + tile_unit<S>(32 * s2 + i8 * 8 + r8, unit), r);
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int kh = 0; kh < 2; ++kh) {
-              if constexpr (!Q8) {
-                vb[h][0][kh] = r[2 * h + kh];
-              } else {
-                const uint32_t x = r[2 * h + kh] ^ 0x80808080u;
-                if constexpr (D == 128) {
-                  vb[h][0][kh] = codes_f16(x, 0x4240);
-                  vb[h][NO - 1][kh] = codes_f16(x, 0x4341);
-                } else {
-                  vb[h][0][kh] = codes_f16(x, (cw & 1) ? 0x4341 : 0x4240);
-                }
-              }
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            uint32_t ap[4];
-            const int r = mt * 16 + (i8 & 1) * 8 + r8;
-            const int unit = 4 * s2 + 2 * h + (i8 >> 1);
-            ldsm4(sP + r * 256 + ((unit ^ (r & 7)) << 4), ap);
-#pragma unroll
-            for (int n = 0; n < NO; ++n) mma16816<BF>(o[mt][n], ap, vb[h][n][0], vb[h][n][1]);
-          }
       }
       if constexpr (!Q8) {
-        if (tail) fence_proxy_async_smem();  // the zeros above, before the next TMA write
+        if (tail) fence_proxy_async_smem();  // the clean-up above, before the next TMA write
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(empty + st);
+      if (lane == 0) mbar_arrive(empty + sv % NS);
     }
+    it += nt;
 
-    // ---- the segment's partial: row sums over the warps, output to the true reference
+    // ---- the segment's partial: the warps' (max, sum, output) merged
+    float* mine = merge + cw * ROWS * S::kMergeRow;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        float a = l[mt][hf];
-        a += __shfl_xor_sync(0xffffffffu, a, 1);
-        a += __shfl_xor_sync(0xffffffffu, a, 2);
-        if (c == 0) smax[cw * RB + mt * 16 + hf * 8 + g] = a;
-      }
-    cons_sync();
-    const int64_t item = head * p.nrb + sp.rb;
-    float* pp = p.part + (static_cast<int64_t>(blockIdx.x) + item) * RB * part_stride<D>();
+      for (int j = 0; j < 2; ++j) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int r = mt * 16 + hf * 8 + g;
+        for (int x = 4; x < 32; x <<= 1)
+          l[nr][j] += __shfl_xor_sync(0xffffffffu, l[nr][j], x);
+        const int r = nr * 8 + 2 * c + j;
         if (r < sp.rows) {
-          float* row = pp + r * part_stride<D>();
-          float f = 1.0f;
-          if constexpr (Q8)
-            f = eref[mt][hf] == -INFINITY ? 0.0f : ex2_approx(eref[mt][hf] - mref[mt][hf]);
-          const float* a = o[mt][0];
-          const float* b = o[mt][NO - 1];
-          if constexpr (Q8 && D == 128) {
-            *reinterpret_cast<float4*>(row + cw * 16 + 4 * c) =
-                make_float4(a[2 * hf] * f, b[2 * hf] * f, a[2 * hf + 1] * f, b[2 * hf + 1] * f);
-          } else if constexpr (Q8) {
-            row[(cw >> 1) * 16 + 4 * c + (cw & 1)] = a[2 * hf] * f;
-            row[(cw >> 1) * 16 + 4 * c + 2 + (cw & 1)] = a[2 * hf + 1] * f;
+          float* row = mine + r * S::kMergeRow;
+          if constexpr (Q8) {
+            // back to the scores' own reference
+            const float f = eref[nr][j] == -INFINITY ? 0.0f : ex2_approx(eref[nr][j] - mref[nr][j]);
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+              *reinterpret_cast<float2*>(row + u * 16 + 2 * g) =
+                  make_float2(o[nr][u][j] * f, o[nr][u][2 + j] * f);
           } else {
 #pragma unroll
-            for (int n = 0; n < NO; ++n)
-              *reinterpret_cast<float2*>(row + cw * (D / 8) + n * 8 + 2 * c) =
-                  make_float2(o[mt][n][2 * hf], o[mt][n][2 * hf + 1]);
+            for (int u = 0; u < NU; ++u) {
+              row[u * 16 + g] = o[nr][u][j];
+              row[u * 16 + 8 + g] = o[nr][u][2 + j];
+            }
           }
-          if (cw == 0 && c == 0) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kTCons; ++k) sum += smax[k * RB + r];
-            row[D] = mref[mt][hf];
-            row[D + 1] = sum;
-            row[D + 2] = Q8 ? 0.0f : static_cast<float>(taken[seg]);
+          if (g == 0) {
+            row[D] = mref[nr][j];
+            row[D + 1] = l[nr][j];
           }
         }
       }
-    if (cw == 0) {
-      __syncwarp();
-      if (lane == 0) taken[seg] = 0;  // next used two segments on
+    if (lane == 0) wait_ok[cw] = ok;
+    cons_sync<NW * 32>();
+    bool all_ok = true;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) all_ok &= wait_ok[k] != 0;
+    if (!all_ok) return;  // a wait ran out: every consumer leaves here
+    const int64_t item = head * p.nrb + sp.rb;
+    float* pp = p.part + (static_cast<int64_t>(blockIdx.x) + item) * p.rb * part_stride<D>();
+    for (int i = ct; i < sp.rows * (D / 4); i += NW * 32) {
+      const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+      const float* in = merge + r * S::kMergeRow;
+      float m = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) m = fmaxf(m, in[k * ROWS * S::kMergeRow + D]);
+      const float ref = m == -INFINITY ? 0.0f : m;
+      float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {
+        const float* x = in + k * ROWS * S::kMergeRow;
+        const float f = ex2_approx(x[D] - ref);
+        const float4 y = *reinterpret_cast<const float4*>(x + d);
+        a.x = fmaf(y.x, f, a.x);
+        a.y = fmaf(y.y, f, a.y);
+        a.z = fmaf(y.z, f, a.z);
+        a.w = fmaf(y.w, f, a.w);
+        sum = fmaf(x[D + 1], f, sum);
+      }
+      float* row = pp + r * part_stride<D>();
+      *reinterpret_cast<float4*>(row + d) = a;
+      if (d == 0)
+        *reinterpret_cast<float4*>(row + D) =
+            make_float4(m, sum, Q8 ? 0.0f : static_cast<float>(*taken), 0.0f);
     }
+    cons_sync<NW * 32>();  // the merge rows and the flag are free
+    if (ct == 0) *taken = 0;
     w += nt;
   }
 }
@@ -1325,12 +1284,12 @@ __global__ void __launch_bounds__(32 * kCWarps) tree_combine_kernel(const TreePa
 }
 
 // ---------------------------------------------------------------- launchers --
-// Rows of a block.  Up to 16 rows go to mma.sync in one block, in which the other rows of a
-// 16-row tile are idle; int8 caches to blocks of 32.  More rows of a 16-bit cache go
+// Rows of a block.  Up to 16 rows go to mma.sync in one block, int8 caches in blocks of 16.  More rows of a 16-bit cache go
 // to tcgen05 in the smallest block that holds them (at most 128).
 int block_rows(int rows, bool q8) {
-  if (rows <= 16) return 16;
-  if (rows <= 32 || q8) return 32;
+  if (rows <= 8) return 8;
+  if (rows <= kMRows || q8) return kMRows;
+  if (rows <= 32) return 32;
   return rows <= 64 ? 64 : 128;
 }
 
@@ -1349,9 +1308,9 @@ void launch_combine(const TreeParams& p, cudaStream_t st) {
   check_launch("tree_combine_kernel", st);
 }
 
-template <class T, int D, bool Q8, int MT>
+template <class T, int D, bool Q8, int NR>
 void launch_mma(const TreeParams& p, cudaStream_t st) {
-  using S = TreeSmem<D, Q8, MT>;
+  using S = MmaSmem<D, Q8, NR>;
   const CUtensorMapDataType dt = Q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : tma_dtype_of<T>();
   const uint64_t rows = static_cast<uint64_t>(p.B) * p.kvh * p.P;
   const CUtensorMapSwizzle sw =
@@ -1359,9 +1318,9 @@ void launch_mma(const TreeParams& p, cudaStream_t st) {
   CUtensorMap tk, tv;
   make_tma_2d(&tk, p.kc, dt, Q8 ? 1 : 2, rows, D, D, S::kBox / (Q8 ? 1 : 2), kTTile, sw);
   make_tma_2d(&tv, p.vc, dt, Q8 ? 1 : 2, rows, D, D, S::kBox / (Q8 ? 1 : 2), kTTile, sw);
-  auto kern = tree_mma_kernel<T, D, Q8, MT>;
+  auto kern = tree_mma_kernel<T, D, Q8, NR>;
   LTM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
-  kern<<<p.grid, 32 * (kTCons + 1), S::kBytes, st>>>(tk, tv, p);
+  kern<<<p.grid, 32 * (S::kWarps + 1), S::kBytes, st>>>(tk, tv, p);
   check_launch("tree_mma_kernel", st);
   launch_combine<T, D>(p, st);
 }
@@ -1481,11 +1440,11 @@ extern "C" ltm_status ltm_tree_attention(
         using E = decltype(t_c);
         constexpr int D = decltype(d_c)::value;
         constexpr bool Q = decltype(q_c)::value;
-        if (rb == 16) {
+        if (rb == 8) {
           launch_mma<E, D, Q, 1>(p, st);
-        } else if constexpr (Q) {
+        } else if (rb == kMRows) {
           launch_mma<E, D, Q, 2>(p, st);
-        } else {
+        } else if constexpr (!Q) {
           if (rb == 32) launch_tc<E, D, 32>(p, st);
           else if (rb == 64) launch_tc<E, D, 64>(p, st);
           else launch_tc<E, D, 128>(p, st);
