@@ -22,13 +22,14 @@
 // * tree_mma_kernel, up to 16 rows (and int8 caches): warp 0 streams K and V
 //   tiles by TMA into a ring of swizzled slots; the consumer warps contract them on
 //   mma.sync m16n8k16 with the keys as M (a decode step's few rows are the 8 or 16
-//   columns; a 128-row tcgen05 tile would idle).  A warp takes 16 of a tile's keys
+//   columns; a 128-row tcgen05 tile would idle).  A warp takes 16 keys at a time
 //   through S^T = K Q^T, softmax and O^T += V^T P^T on its own; P^T is S^T's
 //   accumulator transposed in registers.  Nothing is exchanged until the segment's
 //   end, where the warps' (max, sum, output) are merged in shared memory.  Up to 8
-//   rows leave registers for 16 consumer warps, two sets that take turns at the tiles;
-//   more rows run 8.  int8 codes become f16 in registers (exact), with the row's scale
-//   applied to the fp32 score (K) and to the probability (V).
+//   rows leave registers for 15 consumer warps (16 warps with the producer: 128
+//   registers a thread), more rows for 11 (168); the warps take 16-key slices in turn.
+//   int8 codes become f16 in registers (exact), with the row's scale applied to the
+//   fp32 score (K) and to the probability (V).
 // * tree_tc_kernel, more rows of a 16-bit cache: tcgen05, keys as the 128 lanes:
 //   S^T [128 keys x N rows] = K Q^T and O^T [D x N] += V^T P, N = 32, 64 or 128 rows.
 //   K and V tiles are used as they lie (K-major and M-major operands), the
@@ -316,7 +317,7 @@ constexpr int kMRows = 16;  // most rows of a block
 
 template <int D, bool Q8, int NR>  // NR: 8-row columns of a block
 struct MmaSmem {
-  static constexpr int kWarps = NR == 1 ? 16 : 8;          // consumers
+  static constexpr int kWarps = NR == 1 ? 15 : 11;         // consumers
   static constexpr int kRows = 8 * NR;
   static constexpr int kRow = D * (Q8 ? 1 : 2);            // bytes per cached row
   static constexpr int kBox = kRow > 128 ? 128 : kRow;     // bytes per row of a TMA box
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
     tree_mma_kernel(const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const TreeParams p) {
   using S = MmaSmem<D, Q8, NR>;
-  constexpr int NS = S::kSlots, KS = D / 16, NU = D / 16, NW = S::kWarps, NG = NW / 8;
+  constexpr int NS = S::kSlots, KS = D / 16, NU = D / 16, NW = S::kWarps;
   constexpr int ROWS = S::kRows;
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value && !Q8;  // type of the products
   extern __shared__ uint8_t smem_raw[];
@@ -418,9 +419,9 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
     return;
   }
 
-  // ---- consumers: keys wk .. wk + 15 of every NG-th tile
+  // ---- consumers: every NW-th slice of 16 keys
   const int cw = warp - 1, g = lane >> 2, c = lane & 3, i8 = lane >> 3, r8 = lane & 7;
-  const int wk = (cw & 7) * 16, ct = threadIdx.x - 32;
+  const int ct = threadIdx.x - 32;
   unsigned long long* mask = reinterpret_cast<unsigned long long*>(smem + S::kOffMask) + cw * ROWS;
   int it = 0;  // the CTA's tiles so far
   for (uint32_t w = w0; w < w1;) {
@@ -428,18 +429,18 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
     const int nt = min(static_cast<int>(w1 - w), sp.tiles - sp.tile);
     const int64_t head = static_cast<int64_t>(sp.b) * p.kvh + sp.h;
     const int keys = sp.len + sp.n;
-    const int t_first = (cw / 8 - it % NG + NG) % NG;  // this warp's first tile of the segment
+    const int x_first = (cw + NW - it * 8 % NW) % NW;  // this warp's first slice of the segment
     // the scales of this warp's 16 keys (K in lanes 0-15, V in lanes 16-31), loaded
-    // kAhead of its tiles before their use: a tile's time is less than a load takes
-    constexpr int kAhead = 3;
+    // kAhead of its slices before their use: a slice's time is less than a load takes
+    constexpr int kAhead = 2;
     float sc_next[kAhead];
-    auto load_scale = [&](int t) -> float {
-      const int key = (sp.tile + t) * kTTile + wk + (lane & 15);
+    auto load_scale = [&](int x) -> float {
+      const int key = sp.tile * kTTile + x * 16 + (lane & 15);
       return key < keys ? __ldg((lane < 16 ? p.ks : p.vs) + head * p.P + key) : 0.0f;
     };
     if constexpr (Q8)
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) sc_next[i] = load_scale(t_first + i * NG);
+      for (int i = 0; i < kAhead; ++i) sc_next[i] = load_scale(x_first + i * NW);
     // Q as B fragments (row g of each 8-row column).  int8 codes: lane c of a quad
     // holds dims c * D/4 .. (the codes' own order, any order of the dims gives the
     // same products) in f16, each row scaled by a power of two so that its largest value
@@ -502,15 +503,15 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
     }
 
     bool ok = true;
-    for (int t = t_first; t < nt; t += NG) {
-      const int sk = 2 * (it + t), sv = sk + 1;
-      const int key0 = (sp.tile + t) * kTTile + wk;
+    for (int x = x_first; x < nt * 8; x += NW) {
+      const int sk = 2 * (it + (x >> 3)), sv = sk + 1, wk = (x & 7) * 16;
+      const int key0 = sp.tile * kTTile + x * 16;
       float ks[2] = {1.0f, 1.0f}, vsc[2], lvs[2];
       if constexpr (Q8) {
         const float sc = sc_next[0];
 #pragma unroll
         for (int i = 0; i + 1 < kAhead; ++i) sc_next[i] = sc_next[i + 1];
-        sc_next[kAhead - 1] = load_scale(t + kAhead * NG);
+        sc_next[kAhead - 1] = load_scale(x + kAhead * NW);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // keys g, g + 8
           ks[h] = __shfl_sync(0xffffffffu, sc, g + 8 * h);
@@ -615,21 +616,21 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
       for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float x[2];
+          float pr[2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float s = acc[nr][2 * h + j];
-            x[j] = ex2_approx(s - (mref[nr][j] == -INFINITY ? 0.0f : mref[nr][j]));
-            l[nr][j] += x[j];
+            pr[j] = ex2_approx(s - (mref[nr][j] == -INFINITY ? 0.0f : mref[nr][j]));
+            l[nr][j] += pr[j];
             if constexpr (Q8) {
               // p * v's scale, against its own reference: at most 2^8.  The factor only
               // overflows where p is 0.  A scale NaN becomes an infinity here, and a NaN by
               // its row's zero codes; a row that does not see the key takes nothing of it.
-              x[j] *= fminf(vsc[h] * frow[nr][j], 3.0e38f);
-              if (tail && s == -INFINITY) x[j] = 0.0f;
+              pr[j] *= fminf(vsc[h] * frow[nr][j], 3.0e38f);
+              if (tail && s == -INFINITY) pr[j] = 0.0f;
             }
           }
-          bp[nr][h] = transpose8x8(pack16<BF>(x[0], x[1]));
+          bp[nr][h] = transpose8x8(pack16<BF>(pr[0], pr[1]));
         }
       ok = __all_sync(0xffffffffu, mbar_wait_bounded(full + sv % NS, (sv / NS) & 1, abort_flag,
                                                      p.err, kErrWaitFull));
