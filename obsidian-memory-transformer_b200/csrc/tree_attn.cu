@@ -9,7 +9,7 @@
 // heads share a cached head.
 //
 // The keys of a (sequence, head) -- context, then draft -- are cut into tiles of
-// 128 positions.  The tiles of the whole batch, whatever the lengths, form one
+// 128 to 240 positions.  The tiles of the whole batch, whatever the lengths, form one
 // list that the persistent CTAs (one per SM) share out evenly; a CTA that ends or
 // starts inside a head leaves a partial (max, sum, output) there, and
 // tree_combine_kernel merges them, one warp per query row.  Every cached byte is
@@ -25,11 +25,13 @@
 //   columns; a 128-row tcgen05 tile would idle).  A warp takes 16 keys at a time
 //   through S^T = K Q^T, softmax and O^T += V^T P^T on its own; P^T is S^T's
 //   accumulator transposed in registers.  Nothing is exchanged until the segment's
-//   end, where the warps' (max, sum, output) are merged in shared memory.  Up to 8
-//   rows leave registers for 15 consumer warps (16 warps with the producer: 128
-//   registers a thread), more rows for 11 (168); the warps take 16-key slices in turn.
-//   int8 codes become f16 in registers (exact), with the row's scale applied to the
-//   fp32 score (K) and to the probability (V).
+//   end, where the warps' (max, sum, output) are merged in shared memory.  int8 codes
+//   become f16 in registers (exact), with the row's scale applied to the fp32 score (K)
+//   and to the probability (V); those conversions bound the kernel, so int8 caches run
+//   15 consumer warps up to 8 rows (16 warps with the producer: 128 registers a
+//   thread) and 11 beyond (168), 16-bit ones 8.  A tile is 16 keys for every warp:
+//   each warp waits for every load in turn (a warp that skipped tiles could take a
+//   barrier's phase for the one before).
 // * tree_tc_kernel, more rows of a 16-bit cache: tcgen05, keys as the 128 lanes:
 //   S^T [128 keys x N rows] = K Q^T and O^T [D x N] += V^T P, N = 32, 64 or 128 rows.
 //   K and V tiles are used as they lie (K-major and M-major operands), the
@@ -50,7 +52,7 @@
 namespace ltm_b200 {
 namespace {
 
-constexpr int kTTile = 128;       // cache positions per tile
+constexpr int kTcTile = 128;      // cache positions per tile of the tcgen05 kernel
 constexpr int kTBatch = 512;      // sequences per launch
 constexpr int kTMaxGrid = 256;    // CTAs that share the tiles, whatever the device
 constexpr int kTMaxTokens = 64;   // drafted tokens (one 64-bit ancestor mask)
@@ -69,6 +71,7 @@ struct TreeParams {
   const int* ntok;
   const int* parents;
   int B, T, G, kvh, nrb, rb;  // nrb: row blocks per cached head, of rb rows
+  int tile;                   // positions per tile
   int64_t P;
   float sl2;
   float* part;
@@ -88,8 +91,8 @@ __device__ __forceinline__ bool tree_seq(const TreeParams& p, int b, int& len, i
   return ok;
 }
 
-__device__ __forceinline__ int tiles_of(int len, int n) {
-  return n > 0 ? (len + n - 1) / kTTile + 1 : 0;
+__device__ __forceinline__ int tiles_of(const TreeParams& p, int len, int n) {
+  return n > 0 ? (len + n - 1) / p.tile + 1 : 0;
 }
 __device__ __forceinline__ int row_blocks(const TreeParams& p, int n) {
   return (p.G * n + p.rb - 1) / p.rb;
@@ -104,7 +107,7 @@ __device__ __forceinline__ void tree_scan(const TreeParams& p, uint32_t* base, i
     if (b < p.B) {
       int len, n;
       tree_seq(p, b, len, n);
-      w = static_cast<uint32_t>(p.kvh) * row_blocks(p, n) * tiles_of(len, n);
+      w = static_cast<uint32_t>(p.kvh) * row_blocks(p, n) * tiles_of(p, len, n);
     }
     uint32_t s = w;
 #pragma unroll
@@ -141,7 +144,7 @@ __device__ __forceinline__ TreeSpan tree_find(const TreeParams& p, const uint32_
   TreeSpan s;
   s.b = lo;
   tree_seq(p, lo, s.len, s.n);
-  s.tiles = tiles_of(s.len, s.n);
+  s.tiles = tiles_of(p, s.len, s.n);
   const int nrb = row_blocks(p, s.n);
   const uint32_t at = w - base[lo];
   const uint32_t item = at / s.tiles;
@@ -317,20 +320,24 @@ constexpr int kMRows = 16;  // most rows of a block
 
 template <int D, bool Q8, int NR>  // NR: 8-row columns of a block
 struct MmaSmem {
-  static constexpr int kWarps = NR == 1 ? 15 : 11;         // consumers
+  static constexpr int kWarps = !Q8 ? 8 : NR == 1 ? 15 : 11;  // consumers
+  static constexpr int kKeys = 16 * kWarps;                // positions per tile
   static constexpr int kRows = 8 * NR;
   static constexpr int kRow = D * (Q8 ? 1 : 2);            // bytes per cached row
   static constexpr int kBox = kRow > 128 ? 128 : kRow;     // bytes per row of a TMA box
   static constexpr int kBoxes = kRow / kBox;
-  static constexpr int kTile = kTTile * kRow;              // K or V tile
-  static constexpr int kSlots = 131072 / kTile > 8 ? 8 : 131072 / kTile;
+  static constexpr int kTile = kKeys * kRow;               // K or V tile
   static constexpr int kMergeRow = D + 4;                  // output, max, sum
+  static constexpr int kMerge = kWarps * kRows * kMergeRow * 4;
+  static constexpr int kFit = (214 * 1024 - kMerge) / kTile;
+  static constexpr int kSlots = kFit > 8 ? 8 : kFit;
+  static_assert(kTile % 1024 == 0 && kSlots >= 4, "swizzle atoms; K and V of two tiles");
   static constexpr int kOffMerge = kSlots * kTile;         // [warps][rows]
-  static constexpr int kOffMask = kOffMerge + kWarps * kRows * kMergeRow * 4;  // [warps][rows]
+  static constexpr int kOffMask = kOffMerge + kMerge;  // [warps][rows]
   static constexpr int kOffBase = kOffMask + kWarps * kRows * 8;
   static constexpr int kOffBar = kOffBase + (kTBatch + 2) * 4;
   static constexpr int kOffFlag = kOffBar + 2 * kSlots * 8;
-  static constexpr int kBytes = kOffFlag + 96 + 1024;
+  static constexpr int kBytes = kOffFlag + 128 + 1024;
   static_assert(kBytes <= 232448, "shared memory of one CTA");
 };
 
@@ -338,7 +345,7 @@ struct MmaSmem {
 template <class S>
 __device__ __forceinline__ uint32_t tile_unit(int r, int c) {
   if constexpr (S::kBox == 128)
-    return static_cast<uint32_t>((c >> 3) * (kTTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+    return static_cast<uint32_t>((c >> 3) * (S::kKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
   else  // 64-byte rows, 64-byte swizzle
     return static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
@@ -360,16 +367,16 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
   uint64_t* empty = full + NS;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kOffFlag);
   int* wait_ok = reinterpret_cast<int*>(smem + S::kOffFlag) + 1;  // [NW]
-  int* taken = wait_ok + NW;
+  int* taken = wait_ok + NW;  // [2], by segment parity
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 32) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, 8);
+      mbar_init(empty + i, NW);
     }
     *abort_flag = 0;
-    *taken = 0;
+    taken[0] = taken[1] = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -392,7 +399,7 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
         const TreeSpan s = tree_find(p, base, w);
         const int nt = min(static_cast<int>(w1 - w), s.tiles - s.tile);
         const int row = static_cast<int>((static_cast<int64_t>(s.b) * p.kvh + s.h) * p.P) +
-                        s.tile * kTTile;
+                        s.tile * S::kKeys;
         for (int t = 0; t < 2 * nt; ++t) {
           const int st = it % NS;
           if (!mbar_wait_bounded(empty + st, ((it / NS) & 1) ^ 1, abort_flag, p.err,
@@ -404,8 +411,8 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
           uint8_t* dst = smem + st * S::kTile;
 #pragma unroll
           for (int x = 0; x < S::kBoxes; ++x)
-            tma_load_2d(dst + x * kTTile * 128, (t & 1) ? &tmV : &tmK, full + st, x * 64,
-                        row + (t >> 1) * kTTile);
+            tma_load_2d(dst + x * S::kKeys * 128, (t & 1) ? &tmV : &tmK, full + st, x * 64,
+                        row + (t >> 1) * S::kKeys);
           ++it;
         }
         w += nt;
@@ -419,28 +426,27 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
     return;
   }
 
-  // ---- consumers: every NW-th slice of 16 keys
+  // ---- consumers: keys wk .. wk + 15 of every tile
   const int cw = warp - 1, g = lane >> 2, c = lane & 3, i8 = lane >> 3, r8 = lane & 7;
-  const int ct = threadIdx.x - 32;
+  const int wk = cw * 16, ct = threadIdx.x - 32;
   unsigned long long* mask = reinterpret_cast<unsigned long long*>(smem + S::kOffMask) + cw * ROWS;
-  int it = 0;  // the CTA's tiles so far
-  for (uint32_t w = w0; w < w1;) {
+  int it = 0, seg = 0;  // the CTA's tiles so far; parity of its segments
+  for (uint32_t w = w0; w < w1; seg ^= 1) {
     const TreeSpan sp = tree_find(p, base, w);
     const int nt = min(static_cast<int>(w1 - w), sp.tiles - sp.tile);
     const int64_t head = static_cast<int64_t>(sp.b) * p.kvh + sp.h;
     const int keys = sp.len + sp.n;
-    const int x_first = (cw + NW - it * 8 % NW) % NW;  // this warp's first slice of the segment
     // the scales of this warp's 16 keys (K in lanes 0-15, V in lanes 16-31), loaded
-    // kAhead of its slices before their use: a slice's time is less than a load takes
+    // kAhead tiles before their use: a tile's time is less than a load takes
     constexpr int kAhead = 2;
     float sc_next[kAhead];
-    auto load_scale = [&](int x) -> float {
-      const int key = sp.tile * kTTile + x * 16 + (lane & 15);
+    auto load_scale = [&](int t) -> float {
+      const int key = (sp.tile + t) * S::kKeys + wk + (lane & 15);
       return key < keys ? __ldg((lane < 16 ? p.ks : p.vs) + head * p.P + key) : 0.0f;
     };
     if constexpr (Q8)
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) sc_next[i] = load_scale(x_first + i * NW);
+      for (int i = 0; i < kAhead; ++i) sc_next[i] = load_scale(i);
     // Q as B fragments (row g of each 8-row column).  int8 codes: lane c of a quad
     // holds dims c * D/4 .. (the codes' own order, any order of the dims gives the
     // same products) in f16, each row scaled by a power of two so that its largest value
@@ -485,7 +491,7 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
         qinv[nr][1] = __shfl_sync(0xffffffffu, inv, 8 * c + 4);
       }
     }
-    if ((sp.tile + nt) * kTTile > sp.len)
+    if ((sp.tile + nt) * S::kKeys > sp.len)
       tree_masks(p, sp.b, sp.n, sp.rb * p.rb, ROWS, mask, lane);
     // o[nr][u]: dims of 16-byte-pair u (rows of the A tile) x rows 2c, 2c + 1
     float o[NR][NU][4], l[NR][2], mref[NR][2], eref[NR][2], frow[NR][2];
@@ -503,15 +509,15 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
     }
 
     bool ok = true;
-    for (int x = x_first; x < nt * 8; x += NW) {
-      const int sk = 2 * (it + (x >> 3)), sv = sk + 1, wk = (x & 7) * 16;
-      const int key0 = sp.tile * kTTile + x * 16;
+    for (int t = 0; t < nt; ++t) {
+      const int sk = 2 * (it + t), sv = sk + 1;
+      const int key0 = (sp.tile + t) * S::kKeys + wk;
       float ks[2] = {1.0f, 1.0f}, vsc[2], lvs[2];
       if constexpr (Q8) {
         const float sc = sc_next[0];
 #pragma unroll
         for (int i = 0; i + 1 < kAhead; ++i) sc_next[i] = sc_next[i + 1];
-        sc_next[kAhead - 1] = load_scale(x + kAhead * NW);
+        sc_next[kAhead - 1] = load_scale(t + kAhead);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // keys g, g + 8
           ks[h] = __shfl_sync(0xffffffffu, sc, g + 8 * h);
@@ -643,7 +649,7 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
             const int r = u / (S::kRow / 16);
             if (key0 + r >= sp.len &&
                 clean_unit<T>(tv + tile_unit<S>(wk + r, u % (S::kRow / 16)), key0 + r >= keys))
-              *taken = 1;
+              taken[seg] = 1;
           }
           __syncwarp();
         }
@@ -747,10 +753,10 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
       *reinterpret_cast<float4*>(row + d) = a;
       if (d == 0)
         *reinterpret_cast<float4*>(row + D) =
-            make_float4(m, sum, Q8 ? 0.0f : static_cast<float>(*taken), 0.0f);
+            make_float4(m, sum, Q8 ? 0.0f : static_cast<float>(taken[seg]), 0.0f);
     }
-    cons_sync<NW * 32>();  // the merge rows and the flag are free
-    if (ct == 0) *taken = 0;
+    cons_sync<NW * 32>();  // the merge rows are free
+    if (ct == 0) taken[seg] = 0;  // set again two segments on, past another barrier
     w += nt;
   }
 }
@@ -760,10 +766,10 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
 // of 128-position K and V tiles, all in 128-byte-swizzled chunks of 64 columns.
 template <int D, int N>
 struct TcSmem {
-  static constexpr int kTile = kTTile * D * 2;        // K or V tile
+  static constexpr int kTile = kTcTile * D * 2;        // K or V tile
   static constexpr int kQChunk = N * 128;             // N rows x 64 dims
   static constexpr int kQ = (D / 64) * kQChunk;
-  static constexpr int kPChunk = kTTile * 128;        // 128 keys x 64 rows
+  static constexpr int kPChunk = kTcTile * 128;        // 128 keys x 64 rows
   static constexpr int kP = ((N + 63) / 64) * kPChunk;
   static constexpr int kOffP = kQ;
   static constexpr int kOffRing = kOffP + kP;
@@ -886,7 +892,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
         const TreeSpan s = tree_find(p, base, w);
         const int nt = min(static_cast<int>(w1 - w), s.tiles - s.tile);
         const int row = static_cast<int>((static_cast<int64_t>(s.b) * p.kvh + s.h) * p.P) +
-                        s.tile * kTTile;
+                        s.tile * kTcTile;
         for (int t = 0; ok && t < 2 * nt; ++t) {
           const int st = it % NS;
           if (!mbar_wait_bounded(empty + st, ((it / NS) & 1) ^ 1, abort_flag, p.err,
@@ -898,8 +904,8 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
           uint8_t* dst = smem + S::kOffRing + st * S::kTile;
 #pragma unroll
           for (int x = 0; x < D / 64; ++x)
-            tma_load_2d(dst + x * kTTile * 128, (t & 1) ? &tmV : &tmK, full + st, x * 64,
-                        row + (t >> 1) * kTTile);
+            tma_load_2d(dst + x * kTcTile * 128, (t & 1) ? &tmV : &tmK, full + st, x * 64,
+                        row + (t >> 1) * kTcTile);
           ++it;
         }
         w += nt;
@@ -917,7 +923,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
       // A = V^T: M (dims) contiguous; B = P: N (rows) contiguous
       constexpr uint32_t idO = idesc_f16(128, N, kBF, true) | (1u << 15);
       // D = 64: the upper 64 lanes repeat the lower ones (chunk stride 0)
-      constexpr uint32_t kVChunk = D == 128 ? kTTile * 128 : 0;
+      constexpr uint32_t kVChunk = D == 128 ? kTcTile * 128 : 0;
       const uint32_t aQ = smem_u32(smem), aP = smem_u32(smem + S::kOffP);
       const uint32_t ring = smem_u32(smem + S::kOffRing);
       int it = 0, seg = 0;  // tiles, segments so far
@@ -935,7 +941,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           tc_mma_f16(tmem + (j & 1) * N,
-                     make_desc_kmajor_sw128(aK + (k >> 2) * kTTile * 128 + (k & 3) * 32),
+                     make_desc_kmajor_sw128(aK + (k >> 2) * kTcTile * 128 + (k & 3) * 32),
                      make_desc_kmajor_sw128(aQ + (k >> 2) * S::kQChunk + (k & 3) * 32), idS, k != 0);
         tc_commit(s_full + (j & 1));
         tc_commit(empty + 2 * j % NS);
@@ -947,7 +953,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
         tc_fence_after();
         const uint32_t aV = ring + ((2 * j + 1) % NS) * S::kTile;
 #pragma unroll
-        for (int k = 0; k < kTTile / 16; ++k)
+        for (int k = 0; k < kTcTile / 16; ++k)
           tc_mma_f16(tO, make_desc_mnmajor_sw128(aV + k * 2048, kVChunk),
                      make_desc_mnmajor_sw128(aP + k * 2048, S::kPChunk), idO, !first || k != 0);
         tc_commit(pv_done);
@@ -990,7 +996,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
       const int nt = min(static_cast<int>(w1 - w), sp.tiles - sp.tile);
       const int64_t head = static_cast<int64_t>(sp.b) * p.kvh + sp.h;
       bool taken = false;
-      if ((sp.tile + nt) * kTTile > sp.len)
+      if ((sp.tile + nt) * kTcTile > sp.len)
         tree_masks(p, sp.b, sp.n, sp.rb * N + r0, RW, mask, lane);
       // Q into its swizzled chunks (the last scores of the segment before have been
       // read, so its MMAs are done), all loads in flight together; rows past the
@@ -1022,8 +1028,8 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
       for (int i = 0; i < RW; ++i) l[i] = 0.0f;
 
       for (int t = 0; t < nt; ++t, ++it) {
-        const int at = (sp.tile + t) * kTTile + kt - sp.len;  // this key's place in the draft
-        const bool tail = (sp.tile + t + 1) * kTTile > sp.len, first = t == 0;
+        const int at = (sp.tile + t) * kTcTile + kt - sp.len;  // this key's place in the draft
+        const bool tail = (sp.tile + t + 1) * kTcTile > sp.len, first = t == 0;
         // the rows that see this key, as bits: all of a context key, of a drafted one those
         // whose token's set holds it
         unsigned long long seen = ~0ull;
@@ -1052,7 +1058,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
             uint8_t* tv = smem + S::kOffRing + (slot % NS) * S::kTile;
 #pragma unroll 4
             for (int u = 0; u < D / 8; ++u)
-              taken |= clean_unit<T>(tv + (u >> 3) * kTTile * 128 + kt * 128 +
+              taken |= clean_unit<T>(tv + (u >> 3) * kTcTile * 128 + kt * 128 +
                                          (((u & 7) ^ (kt & 7)) << 4), at >= sp.n);
           }
         }
@@ -1241,7 +1247,7 @@ __global__ void __launch_bounds__(32 * kCWarps) tree_combine_kernel(const TreePa
   for (int i = 0; i < DL; ++i) acc[i] = 0.0f;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the partials are complete
   if (t < n) {
-    const int rb = r / p.rb, tiles = tiles_of(len, n), nrb = row_blocks(p, n);
+    const int rb = r / p.rb, tiles = tiles_of(p, len, n), nrb = row_blocks(p, n);
     const uint32_t t0 = base[b] + (static_cast<uint32_t>(h) * nrb + rb) * tiles;
     const uint32_t c0 = share_of(t0, total, shares), c1 = share_of(t0 + tiles - 1, total, shares);
     const int64_t item = static_cast<int64_t>(bh) * p.nrb + rb;
@@ -1299,6 +1305,15 @@ size_t tree_slots(int B, int T, int G, int kvh, int grid, int rb, int& nrb) {
   return static_cast<size_t>(B) * kvh * nrb + grid;
 }
 
+// Tile length, and the CTAs that share the tiles (at most kTMaxGrid).
+void set_tiles(TreeParams& p, int tile) {
+  const int64_t most = static_cast<int64_t>(p.B) * p.kvh * p.nrb * ((p.P + tile - 1) / tile);
+  LTM_REQUIRE(most < (1ll << 31), "too many tiles");
+  const int sms = device_sm_count() < kTMaxGrid ? device_sm_count() : kTMaxGrid;
+  p.tile = tile;
+  p.grid = static_cast<int>(most < sms ? most : sms);
+}
+
 template <class T, int D>
 void launch_combine(const TreeParams& p, cudaStream_t st) {
   const int64_t rows = static_cast<int64_t>(p.B) * p.kvh * p.G * p.T;
@@ -1310,15 +1325,16 @@ void launch_combine(const TreeParams& p, cudaStream_t st) {
 }
 
 template <class T, int D, bool Q8, int NR>
-void launch_mma(const TreeParams& p, cudaStream_t st) {
+void launch_mma(TreeParams p, cudaStream_t st) {
   using S = MmaSmem<D, Q8, NR>;
+  set_tiles(p, S::kKeys);
   const CUtensorMapDataType dt = Q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : tma_dtype_of<T>();
   const uint64_t rows = static_cast<uint64_t>(p.B) * p.kvh * p.P;
   const CUtensorMapSwizzle sw =
       S::kBox == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   CUtensorMap tk, tv;
-  make_tma_2d(&tk, p.kc, dt, Q8 ? 1 : 2, rows, D, D, S::kBox / (Q8 ? 1 : 2), kTTile, sw);
-  make_tma_2d(&tv, p.vc, dt, Q8 ? 1 : 2, rows, D, D, S::kBox / (Q8 ? 1 : 2), kTTile, sw);
+  make_tma_2d(&tk, p.kc, dt, Q8 ? 1 : 2, rows, D, D, S::kBox / (Q8 ? 1 : 2), S::kKeys, sw);
+  make_tma_2d(&tv, p.vc, dt, Q8 ? 1 : 2, rows, D, D, S::kBox / (Q8 ? 1 : 2), S::kKeys, sw);
   auto kern = tree_mma_kernel<T, D, Q8, NR>;
   LTM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
   kern<<<p.grid, 32 * (S::kWarps + 1), S::kBytes, st>>>(tk, tv, p);
@@ -1327,12 +1343,13 @@ void launch_mma(const TreeParams& p, cudaStream_t st) {
 }
 
 template <class T, int D, int N>
-void launch_tc(const TreeParams& p, cudaStream_t st) {
+void launch_tc(TreeParams p, cudaStream_t st) {
   using S = TcSmem<D, N>;
+  set_tiles(p, kTcTile);
   const uint64_t rows = static_cast<uint64_t>(p.B) * p.kvh * p.P;
   CUtensorMap tk, tv;
-  make_tma_2d(&tk, p.kc, tma_dtype_of<T>(), 2, rows, D, D, 64, kTTile);
-  make_tma_2d(&tv, p.vc, tma_dtype_of<T>(), 2, rows, D, D, 64, kTTile);
+  make_tma_2d(&tk, p.kc, tma_dtype_of<T>(), 2, rows, D, D, 64, kTcTile);
+  make_tma_2d(&tv, p.vc, tma_dtype_of<T>(), 2, rows, D, D, 64, kTcTile);
   auto kern = tree_tc_kernel<T, D, N>;
   LTM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
   kern<<<p.grid, 128 + 128 * S::kGroups, S::kBytes, st>>>(tk, tv, p);
@@ -1419,13 +1436,8 @@ extern "C" ltm_status ltm_tree_attention(
       const int64_t heads0 = static_cast<int64_t>(b0) * kv_heads;
       LTM_REQUIRE(static_cast<int64_t>(p.B) * kv_heads * max_positions < (1ll << 31),
                   "cache rows exceed int32");
-      const int64_t most = static_cast<int64_t>(p.B) * kv_heads *
-                           ((G * T + rb - 1) / rb) * ((max_positions + kTTile - 1) / kTTile);
-      LTM_REQUIRE(most < (1ll << 31), "too many tiles");
-      const int sms = device_sm_count() < kTMaxGrid ? device_sm_count() : kTMaxGrid;
-      p.grid = static_cast<int>(most < sms ? most : sms);
       p.rb = rb;
-      const size_t slots = tree_slots(p.B, T, G, kv_heads, p.grid, rb, p.nrb);
+      const size_t slots = tree_slots(p.B, T, G, kv_heads, kTMaxGrid, rb, p.nrb);
       LTM_REQUIRE(workspace_bytes >= slots * rb * (head_dim + 4) * sizeof(float),
                   "workspace too small");
       p.q = static_cast<const uint8_t*>(q) + 2 * b0 * p.qb;
