@@ -251,6 +251,13 @@ int persistent_grid(K kernel, int block, size_t smem, int64_t want) {
   return static_cast<int>(want < cap ? (want < 1 ? 1 : want) : cap);
 }
 
+// Raises a kernel's dynamic shared-memory limit, once per kernel and device.
+void allow_smem_of(const void* kernel, int bytes);
+template <class K>
+void allow_smem(K kernel, int bytes) {
+  allow_smem_of(reinterpret_cast<const void*>(kernel), bytes);
+}
+
 // Launches a kernel that starts by waiting (griddepcontrol.wait) for the kernel
 // before it on the stream: its CTAs may be scheduled once every CTA of that
 // kernel has executed griddepcontrol.launch_dependents or ended.

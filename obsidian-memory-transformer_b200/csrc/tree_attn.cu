@@ -1336,7 +1336,7 @@ void launch_mma(TreeParams p, cudaStream_t st) {
   make_tma_2d(&tk, p.kc, dt, Q8 ? 1 : 2, rows, D, D, S::kBox / (Q8 ? 1 : 2), S::kKeys, sw);
   make_tma_2d(&tv, p.vc, dt, Q8 ? 1 : 2, rows, D, D, S::kBox / (Q8 ? 1 : 2), S::kKeys, sw);
   auto kern = tree_mma_kernel<T, D, Q8, NR>;
-  LTM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
+  allow_smem(kern, S::kBytes);
   kern<<<p.grid, 32 * (S::kWarps + 1), S::kBytes, st>>>(tk, tv, p);
   check_launch("tree_mma_kernel", st);
   launch_combine<T, D>(p, st);
@@ -1351,7 +1351,7 @@ void launch_tc(TreeParams p, cudaStream_t st) {
   make_tma_2d(&tk, p.kc, tma_dtype_of<T>(), 2, rows, D, D, 64, kTcTile);
   make_tma_2d(&tv, p.vc, tma_dtype_of<T>(), 2, rows, D, D, 64, kTcTile);
   auto kern = tree_tc_kernel<T, D, N>;
-  LTM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
+  allow_smem(kern, S::kBytes);
   kern<<<p.grid, 128 + 128 * S::kGroups, S::kBytes, st>>>(tk, tv, p);
   check_launch("tree_tc_kernel", st);
   launch_combine<T, D>(p, st);

@@ -493,27 +493,33 @@ class _Call:
     __slots__ = ("device", "other", "stream", "_back")
 
     def __init__(self, t, stream):
-        torch = _torch()
+        C_ = _torch()._C
         self.device = t.device
-        index = self.device.index
-        self.other = self._back = None
-        if torch.cuda.current_device() != index:
-            self._back = torch.cuda.current_device()
-            torch.cuda.set_device(index)
-        raw = torch._C._cuda_getCurrentRawStream(index)
-        if stream is not None and stream.cuda_stream != raw:
+        index = t.get_device()
+        back = C_._cuda_getDevice()
+        self._back = None
+        if back != index:
+            self._back = back
+            C_._cuda_setDevice(index)
+        self.stream = C_._cuda_getCurrentRawStream(index)
+        self.other = None
+        if stream is not None and stream.cuda_stream != self.stream:
             self.other = stream
-            raw = stream.cuda_stream
-        self.stream = raw
+            self.stream = stream.cuda_stream
 
     def done(self, status: int) -> None:
         if self._back is not None:
-            _torch().cuda.set_device(self._back)
+            _torch()._C._cuda_setDevice(self._back)
         if status != OK:
             _check(status)
 
     def empty(self, shape, dtype):
-        t = _torch().empty(shape, dtype=dtype, device=self.device)
+        """Uninitialized contiguous memory."""
+        strides, n = [], 1
+        for d in reversed(shape):
+            strides.append(n)
+            n *= d
+        t = _torch().empty_strided(shape, strides[::-1], dtype=dtype, device=self.device)
         if self.other is not None:
             t.record_stream(self.other)
         return t
@@ -525,36 +531,41 @@ def _bad(msg: str):
 
 def _check_device(first, *tensors):
     """Tensors (None allowed) on `first`'s CUDA device."""
-    if not first.is_cuda:
+    index = first.get_device()
+    if index < 0:
         raise ValueError("ltm_b200 operates on CUDA tensors only")
-    device = first.device
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             _bad("all tensors must be on one device")
 
 
 def _check_index(t, shape):
-    """A contiguous int32 tensor of `shape` (or None)."""
-    if t is not None and (t.dtype != _torch().int32 or t.shape != shape or not t.is_contiguous()):
+    """A contiguous int32 tensor of `shape`."""
+    if t.dtype is not _torch().int32 or t.shape != shape or not t.is_contiguous():
         _bad(f"lengths and indices must be contiguous int32 {list(shape)}")
 
 
 def _check_cache(cache, scale, what: str):
-    if cache.dim() != 4 or not cache.is_contiguous():
-        _bad(f"{what} must be contiguous [B, kv_heads, max_positions, head_dim]")
+    """A cache with its scales (None: not int8); returns its shape."""
     torch = _torch()
-    if (scale is not None) != (cache.dtype == torch.int8):
-        _bad(f"{what}: int8 caches need scales, others take none")
-    if scale is not None and (scale.dtype != torch.float32 or scale.shape != cache.shape[:3]
-                              or not scale.is_contiguous()):
-        _bad(f"{what}: scales must be contiguous fp32 [B, kv_heads, max_positions]")
+    shape = cache.shape
+    if len(shape) != 4 or not cache.is_contiguous():
+        _bad(f"{what} must be contiguous [B, kv_heads, max_positions, head_dim]")
+    if scale is None:
+        if cache.dtype is torch.int8:
+            _bad(f"{what}: int8 caches need scales")
+    elif (cache.dtype is not torch.int8 or scale.dtype is not torch.float32
+          or scale.shape != shape[:3] or not scale.is_contiguous()):
+        _bad(f"{what}: an int8 cache takes contiguous fp32 scales [B, kv_heads, max_positions], "
+             "other caches none")
+    return shape
 
 
 def _check_pair(k_cache, v_cache, k_scale, v_scale):
-    _check_cache(k_cache, k_scale, "k_cache")
-    _check_cache(v_cache, v_scale, "v_cache")
-    if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+    shape = _check_cache(k_cache, k_scale, "k_cache")
+    if _check_cache(v_cache, v_scale, "v_cache") != shape or k_cache.dtype is not v_cache.dtype:
         _bad("k_cache and v_cache must have one shape and type")
+    return shape
 
 
 @functools.lru_cache(maxsize=256)
@@ -592,22 +603,24 @@ def kv_cache_append(k, v, k_cache, v_cache, cache_lens, k_scale=None, v_scale=No
     or bf16), or of k's type (f16 / bf16).  cache_lens, num_tokens (how many of the
     T tokens a sequence has): int32 [B].  The lengths are not advanced."""
     _check_device(k, v, k_cache, v_cache, cache_lens, k_scale, v_scale, num_tokens)
-    _check_pair(k_cache, v_cache, k_scale, v_scale)
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+    cB, ch, P, cd = _check_pair(k_cache, v_cache, k_scale, v_scale)
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape or k.dtype is not v.dtype:
         _bad("k and v must both be [B, T, kv_heads, head_dim]")
-    B, T, h, d = k.shape
-    if k_cache.shape[0] != B or k_cache.shape[1] != h or k_cache.shape[3] != d:
+    B, T, h, d = shape
+    if cB != B or ch != h or cd != d:
         _bad("the caches do not fit k and v")
-    if k_scale is None and k_cache.dtype != k.dtype:
+    if k_scale is None and k_cache.dtype is not k.dtype:
         _bad("the caches must be int8 or have k's type")
     _check_index(cache_lens, (B,))
-    _check_index(num_tokens, (B,))
+    if num_tokens is not None:
+        _check_index(num_tokens, (B,))
     sk, sv, dt = _strides3(k, "k"), _strides3(v, "v"), dtype_code(k.dtype)
     c = _Call(k, stream)
     c.done(lib().ltm_kv_cache_append(
         k.data_ptr(), sk, v.data_ptr(), sv, dt, k_cache.data_ptr(), v_cache.data_ptr(),
-        _dp(k_scale), _dp(v_scale), k_cache.shape[2], cache_lens.data_ptr(), _dp(num_tokens), B, T,
-        h, d, c.stream))
+        _dp(k_scale), _dp(v_scale), P, cache_lens.data_ptr(), _dp(num_tokens), B, T, h, d,
+        c.stream))
 
 
 def kv_cache_read(cache, scale, length: int, first=None, cache_lens=None, dtype=None, out=None,
@@ -618,18 +631,20 @@ def kv_cache_read(cache, scale, length: int, first=None, cache_lens=None, dtype=
     (scale None) their values.  Positions outside [0, cache_lens[b]) (int32 [B];
     max_positions when None) give zeros."""
     _check_device(cache, scale, first, cache_lens, out)
-    _check_cache(cache, scale, "cache")
+    B, h, P, d = _check_cache(cache, scale, "cache")
     if length < 0:
         _bad("length must not be negative")
     if dtype is None:
         dtype = cache.dtype if scale is None else _torch().float32
-    if scale is None and dtype != cache.dtype:
+    if scale is None and dtype is not cache.dtype:
         _bad("a 16-bit cache is read in its own type")
-    B, h, P, d = cache.shape
-    _check_index(first, (B,))
-    _check_index(cache_lens, (B,))
+    if first is not None:
+        _check_index(first, (B,))
+    if cache_lens is not None:
+        _check_index(cache_lens, (B,))
     shape, dt = (B, h, length, d), dtype_code(dtype)
-    if out is not None and (out.shape != shape or out.dtype != dtype or not out.is_contiguous()):
+    if out is not None and (out.shape != shape or out.dtype is not dtype
+                            or not out.is_contiguous()):
         _bad(f"out must be contiguous {list(shape)} of the read type")
     c = _Call(cache, stream)
     if out is None:
@@ -651,26 +666,27 @@ def tree_attention(q, k_cache, v_cache, cache_lens, parents=None, k_scale=None, 
     None for a chain.  num_tokens: int32 [B], how many of the T tokens a sequence
     has (the others get zeros).  Returns [B, T, heads, head_dim]."""
     _check_device(q, k_cache, v_cache, cache_lens, parents, k_scale, v_scale, num_tokens, out)
-    _check_pair(k_cache, v_cache, k_scale, v_scale)
-    if q.dim() != 4 or k_cache.shape[0] != q.shape[0] or k_cache.shape[3] != q.shape[3]:
+    cB, kvh, P, cd = _check_pair(k_cache, v_cache, k_scale, v_scale)
+    shape, qt = q.shape, q.dtype
+    if len(shape) != 4 or cB != shape[0] or cd != shape[3]:
         _bad("q must be [B, T, heads, head_dim] for the caches' B and head_dim")
-    if k_scale is None and k_cache.dtype != q.dtype:
+    if k_scale is None and k_cache.dtype is not qt:
         _bad("the caches must be int8 or have q's type")
-    shape = q.shape
     B, T, heads, d = shape
-    kvh, P = k_cache.shape[1], k_cache.shape[2]
     _check_index(cache_lens, (B,))
-    _check_index(num_tokens, (B,))
-    _check_index(parents, (B, T))
-    if out is not None and (out.shape != shape or out.dtype != q.dtype):
+    if num_tokens is not None:
+        _check_index(num_tokens, (B,))
+    if parents is not None:
+        _check_index(parents, (B, T))
+    if out is not None and (out.shape != shape or out.dtype is not qt):
         _bad("out must have q's shape and type")
-    sq, dt = _strides3(q, "q"), dtype_code(q.dtype)
+    sq, dt = _strides3(q, "q"), dtype_code(qt)
     so = (_int64s(T * heads * d, heads * d, d) if out is None else _strides3(out, "out"))
     nbytes = _workspace_bytes("ltm_tree_attention_workspace", B, T, heads, kvh, d)
     c = _Call(q, stream)
     if out is None:
-        out = c.empty(shape, q.dtype)
-    ws = c.empty(nbytes, _torch().uint8)
+        out = c.empty(shape, qt)
+    ws = c.empty((nbytes,), _torch().uint8)
     c.done(lib().ltm_tree_attention(
         q.data_ptr(), sq, k_cache.data_ptr(), v_cache.data_ptr(), _dp(k_scale), _dp(v_scale), P,
         cache_lens.data_ptr(), _dp(num_tokens), _dp(parents), out.data_ptr(), so, B, T, heads, kvh,
@@ -688,23 +704,24 @@ def beam_select(logits, scores, num_out: int | None = None, done=None, end_token
     and a fourth output [B, K] bool says which continuations are finished."""
     torch = _torch()
     _check_device(logits, scores, done)
-    if logits.dim() != 3 or logits.stride(2) != 1:
+    shape, strides = logits.shape, logits.stride()
+    if len(shape) != 3 or strides[2] != 1:
         _bad("logits must be [B, W, V] with unit stride in V")
-    B, W, V = logits.shape
-    if scores.dtype != torch.float32 or scores.shape != (B, W) or not scores.is_contiguous():
+    B, W, V = shape
+    if scores.dtype is not torch.float32 or scores.shape != (B, W) or not scores.is_contiguous():
         _bad("scores must be contiguous fp32 [B, W]")
-    if done is not None and (done.dtype != torch.bool or done.shape != (B, W)
+    if done is not None and (done.dtype is not torch.bool or done.shape != (B, W)
                              or not done.is_contiguous()):
         _bad("done must be contiguous bool [B, W]")
     K = W if num_out is None else num_out
-    sb, sw, _ = logits.stride()
+    sb, sw, _ = strides
     dt = dtype_code(logits.dtype)
     nbytes = _workspace_bytes("ltm_beam_select_workspace", B, W, V, K)
     c = _Call(logits, stream)
     best = c.empty((B, K), torch.float32)
-    beams, tokens = c.empty((2, B, K), torch.int32).unbind(0)
+    beams, tokens = c.empty((B, K), torch.int32), c.empty((B, K), torch.int32)
     fin = c.empty((B, K), torch.bool) if done is not None else None
-    ws = c.empty(nbytes, torch.uint8)
+    ws = c.empty((nbytes,), torch.uint8)
     c.done(lib().ltm_beam_select(
         logits.data_ptr(), dt, sb, sw, scores.data_ptr(), _dp(done), end_token, B, W, V, K,
         best.data_ptr(), beams.data_ptr(), tokens.data_ptr(), _dp(fin), ws.data_ptr(), nbytes,
@@ -721,23 +738,28 @@ def kv_cache_reorder(caches, beams, cache_lens=None, first=None, stream=None) ->
     cache_lens, first: int32 [B] (max_positions and 0 when None)."""
     caches = list(caches)
     _check_device(beams, cache_lens, first, *caches)
-    if beams.dim() != 2:
+    shape = beams.shape
+    if len(shape) != 2:
         _bad("beams must be int32 [B, W]")
-    B, W = beams.shape
-    _check_index(beams, (B, W))
-    _check_index(cache_lens, (B,))
-    _check_index(first, (B,))
+    _check_index(beams, shape)
+    B, W = shape
+    if cache_lens is not None:
+        _check_index(cache_lens, (B,))
+    if first is not None:
+        _check_index(first, (B,))
     n = len(caches)
     if n == 0:
         return
-    lead = caches[0].shape[:3]
+    lead, ptrs, rows = caches[0].shape[:3], [], []
     for t in caches:
-        if t.dim() not in (3, 4) or t.shape[:3] != lead or not t.is_contiguous():
+        s = t.shape
+        if s[:3] != lead or not 3 <= len(s) <= 4 or not t.is_contiguous():
             _bad("caches must be contiguous [B * W, kv_heads, max_positions(, head_dim)]")
-    if lead[0] != B * W:
+        ptrs.append(t.data_ptr())
+        rows.append(t.element_size() * (s[3] if len(s) == 4 else 1))
+    if len(lead) != 3 or lead[0] != B * W:
         _bad("caches must have B * W sequences")
-    ptrs = (C.c_void_p * n)(*[t.data_ptr() for t in caches])
-    rows = _int64s(*[t.element_size() * (t.shape[3] if t.dim() == 4 else 1) for t in caches])
+    ptrs, rows = (C.c_void_p * n)(*ptrs), _int64s(*rows)
     c = _Call(beams, stream)
     c.done(lib().ltm_kv_cache_reorder(ptrs, rows, n, beams.data_ptr(), _dp(first),
                                       _dp(cache_lens), B, W, lead[1], lead[2], c.stream))
