@@ -29,8 +29,8 @@ namespace ltm_b200 {
 namespace {
 
 constexpr int kBThreads = 256;
-constexpr int kPer = 32;                     // logits per thread
-constexpr int kChunk = kBThreads * kPer;     // logits per CTA
+constexpr int kPer = 32, kPerMany = 64;      // logits per thread
+constexpr int kManyK = 16;                   // most continuations with kPerMany
 constexpr int kMaxCand = 1024;               // candidates ranked in shared memory
 constexpr int kMaxK = 64;
 constexpr int kMaxW = 32;
@@ -56,20 +56,70 @@ __device__ __forceinline__ uint64_t list_key(float x, int token) {
   return (static_cast<uint64_t>(ordered(x)) << 32) | ~static_cast<uint32_t>(token);
 }
 
+// Larger of two 16-byte vectors' elements (a NaN gives way), element by element.
+template <class T>
+__device__ __forceinline__ uint4 vec_max(const uint4& a, const uint4& b) {
+  uint4 r;
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+  uint32_t z[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, float>::value) {
+      z[i] = __float_as_uint(fmaxf(__uint_as_float(x[i]), __uint_as_float(y[i])));
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&x[i]),
+                                *reinterpret_cast<const __half2*>(&y[i]));
+      z[i] = *reinterpret_cast<const uint32_t*>(&m);
+    } else {
+      const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x[i]),
+                                       *reinterpret_cast<const __nv_bfloat162*>(&y[i]));
+      z[i] = *reinterpret_cast<const uint32_t*>(&m);
+    }
+  }
+  r.x = z[0];
+  r.y = z[1];
+  r.z = z[2];
+  r.w = z[3];
+  return r;
+}
+
+template <class T>
+__device__ __forceinline__ uint4 vec_none() {  // -inf everywhere
+  constexpr uint32_t k = std::is_same<T, float>::value    ? 0xff800000u
+                         : std::is_same<T, __half>::value ? 0xfc00fc00u
+                                                          : 0xff80ff80u;
+  return make_uint4(k, k, k, k);
+}
+
+// The vector of logits x .. of a row, where only those in [c0, c1) are there (-inf
+// elsewhere).  Not inlined: at most two threads of a chunk need it.
+template <class T>
+__device__ __noinline__ uint4 cut_vector(const T* r, int x, int c0, int c1) {
+  constexpr int N = 16 / sizeof(T);
+  T e[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    e[j] = x + j >= c0 && x + j < c1 ? r[x + j] : from_f32<T>(-INFINITY);
+  return *reinterpret_cast<const uint4*>(e);
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
 struct BeamPartial {
   float m, sum;  // maximum logit of the chunk and sum of exp(logit - m)
 };
 
 // Workspace: [rows, nchunk] BeamPartial, then [rows, nchunk, K] sorted keys
 // (ordered logit << 32 | ~token; 0 = none).
-template <class T>
-__global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 5 : 3)
+template <class T, int PER>
+__global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 && PER == kPer ? 4 : 3)
     beam_chunk_kernel(const T* __restrict__ logits, int64_t ldb, int64_t ldw,
                       const float* __restrict__ scores, const uint8_t* __restrict__ done, int end,
                       int W, int V, int K, int nchunk, int groups, BeamPartial* __restrict__ stats,
                       uint64_t* __restrict__ lists) {
   constexpr int N = 16 / sizeof(T);  // logits per vector
-  constexpr int NV = kPer / N;       // vectors per thread
+  constexpr int NV = PER / N;        // vectors per thread
+  constexpr int kChunk = kBThreads * PER;
   __shared__ float s_group[kBThreads];
   __shared__ float s_sum[kBThreads / 32];
   __shared__ uint64_t s_cand[kMaxCand];
@@ -120,15 +170,12 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 5 : 3)
     return;
   }
   if (tid == 0) s_count = s_slots = 0;
-  const T none = from_f32<T>(-INFINITY);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int x = t0 + i * kBThreads * N;
     if (!(x >= c0 && x + N <= c1)) {
-      T e[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j) e[j] = (x + j >= c0 && x + j < c1) ? r[x + j] : none;
-      raw[i] = *reinterpret_cast<const uint4*>(e);
+      raw[i] = vec_none<T>();
+      if (x < c1 && x + N > c0) raw[i] = cut_vector<T>(r, x, c0, c1);
     }
   }
   // a misaligned row's last `shift` logits lie past the vectors: one per thread
@@ -141,9 +188,11 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 5 : 3)
   float m, tau, tm;
   while (true) {
     tm = extra;
+    uint4 vm = raw[0];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const T* e = reinterpret_cast<const T*>(&raw[i]);
+    for (int i = 1; i < NV; ++i) vm = vec_max<T>(vm, raw[i]);
+    {
+      const T* e = reinterpret_cast<const T*>(&vm);
 #pragma unroll
       for (int j = 0; j < N; ++j) tm = fmaxf(tm, to_f32(e[j]));
     }
@@ -162,12 +211,12 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 5 : 3)
     m = unordered(__reduce_max_sync(0xffffffffu, ordered(fmaxf(g0, g1))));
     tau = unordered(__reduce_min_sync(0xffffffffu, ordered(fminf(g0, g1))));
     const float ref = m == -INFINITY ? 0.0f : m;
-    float sum = __expf(extra - ref);
+    float sum = ex2_approx((extra - ref) * kLog2e);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const T* e = reinterpret_cast<const T*>(&raw[i]);
 #pragma unroll
-      for (int j = 0; j < N; ++j) sum += __expf(to_f32(e[j]) - ref);
+      for (int j = 0; j < N; ++j) sum += ex2_approx((to_f32(e[j]) - ref) * kLog2e);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -202,11 +251,13 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 5 : 3)
     stats[item] = BeamPartial{m, t};
   }
   __syncthreads();
-  const int nval = s_slots * kPer;
-  for (int i = tid; i < nval; i += kBThreads) {
-    const float y = to_f32(reinterpret_cast<const T*>(s_slot)[i]);
-    const int e = i % kPer;
-    offer(y, s_owner[i / kPer] + (e / N) * kBThreads * N + e % N);
+  const int nvec = s_slots * NV;
+  for (int i = tid; i < nvec; i += kBThreads) {
+    const uint4 v = s_slot[i];
+    const T* e = reinterpret_cast<const T*>(&v);
+    const int x = s_owner[i / NV] + (i % NV) * kBThreads * N;
+#pragma unroll
+    for (int j = 0; j < N; ++j) offer(to_f32(e[j]), x + j);
   }
   __syncthreads();
   const int n = s_count;
@@ -221,17 +272,23 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 5 : 3)
     for (int i = n + tid; i < K; i += kBThreads) list[i] = 0ull;
     return;
   }
-  // too many: the K best one after the other (each below the last one taken)
+  // too many: the K best one after the other (each below the last one taken), from
+  // shared memory
+  uint4* mine = s_slot + tid * NV;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) mine[i] = raw[i];
   uint64_t last = ~0ull;
+#pragma unroll 1
   for (int kk = 0; kk < K; ++kk) {
     uint64_t best = 0ull;
     auto look = [&](float y, int x) {
       const uint64_t full = list_key(y, x);
       if (x >= c0 && x < c1 && full < last && full > best) best = full;
     };
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < NV; ++i) {
-      const T* e = reinterpret_cast<const T*>(&raw[i]);
+      const uint4 v = mine[i];
+      const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
       for (int j = 0; j < N; ++j) look(to_f32(e[j]), t0 + i * kBThreads * N + j);
     }
@@ -443,7 +500,15 @@ __global__ void __launch_bounds__(kBThreads)
   }
 }
 
-int chunks_of(int V) { return (V + kChunk - 1) / kChunk; }
+int chunks_of(int V, int per) { return (V + kBThreads * per - 1) / (kBThreads * per); }
+
+// Logits per thread: 32, or 64 of 16 bits where the chunks of 8192 would be more than
+// the device holds at a time: half as many chunks share each one's fixed part (the
+// filter and its barriers).
+int logits_per_thread(int64_t rows, int V, int K, ltm_dtype dt) {
+  const bool many = rows * chunks_of(V, kPer) > 4 * device_sm_count();
+  return many && dt != LTM_DTYPE_F32 && K <= kManyK && V > kBThreads * kPer ? kPerMany : kPer;
+}
 
 }  // namespace
 }  // namespace ltm_b200
@@ -454,7 +519,7 @@ extern "C" ltm_status ltm_beam_select_workspace(int B, int W, int V, int K, size
   return guarded([&] {
     LTM_REQUIRE(bytes != nullptr, "NULL pointer");
     LTM_REQUIRE(B >= 0 && W >= 1 && V >= 1 && K >= 1, "bad size");
-    const int64_t items = static_cast<int64_t>(B) * W * chunks_of(V);
+    const int64_t items = static_cast<int64_t>(B) * W * chunks_of(V, kPer);
     *bytes = static_cast<size_t>(items) * (sizeof(BeamPartial) + static_cast<size_t>(K) * 8);
   });
 }
@@ -482,11 +547,12 @@ extern "C" ltm_status ltm_beam_select(const void* logits, ltm_dtype dtype, int64
     LTM_REQUIRE(reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype) == 0,
                 "logits are not aligned to their type");
     LTM_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 7) == 0, "workspace must be 8-byte aligned");
-    const int nchunk = chunks_of(V);
-    const int64_t items = static_cast<int64_t>(B) * W * nchunk;
-    LTM_REQUIRE(items < (1ll << 31), "too many beams");
-    LTM_REQUIRE(workspace_bytes >= items * (sizeof(BeamPartial) + static_cast<size_t>(K) * 8),
+    const int64_t rows = static_cast<int64_t>(B) * W, most = rows * chunks_of(V, kPer);
+    LTM_REQUIRE(most < (1ll << 31), "too many beams");
+    LTM_REQUIRE(workspace_bytes >= most * (sizeof(BeamPartial) + static_cast<size_t>(K) * 8),
                 "workspace too small");
+    const int per = logits_per_thread(rows, V, K, dtype), nchunk = chunks_of(V, per);
+    const int64_t items = rows * nchunk;
     BeamPartial* stats = static_cast<BeamPartial*>(workspace);
     uint64_t* lists = reinterpret_cast<uint64_t*>(stats + items);
     int groups = 8;
@@ -494,9 +560,16 @@ extern "C" ltm_status ltm_beam_select(const void* logits, ltm_dtype dtype, int64
     const cudaStream_t st = as_stream(stream);
     dispatch_dtype(dtype, [&](auto tag) {
       using T = decltype(tag);
-      beam_chunk_kernel<T><<<static_cast<unsigned>(items), kBThreads, 0, st>>>(
-          static_cast<const T*>(logits), batch_stride, beam_stride, scores, done, end_token, W, V,
-          K, nchunk, groups, stats, lists);
+      auto go = [&](auto per_c) {
+        beam_chunk_kernel<T, decltype(per_c)::value><<<static_cast<unsigned>(items), kBThreads, 0,
+                                                       st>>>(
+            static_cast<const T*>(logits), batch_stride, beam_stride, scores, done, end_token, W,
+            V, K, nchunk, groups, stats, lists);
+      };
+      if constexpr (sizeof(T) == 2) {
+        if (per == kPerMany) return go(std::integral_constant<int, kPerMany>{});
+      }
+      go(std::integral_constant<int, kPer>{});
     });
     check_launch("beam_chunk_kernel", st);
     // launched while the chunks still run; it waits for their completion on the device
