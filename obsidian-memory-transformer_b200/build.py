@@ -1,7 +1,9 @@
 """Build recipe of libltm_b200.so: every csrc/*.cu compiled for sm_100a with
 nvcc and linked into ltm_b200/libltm_b200.so (in-tree, so it travels with the
-repository snapshot).  Incremental: an object is rebuilt when its source or
-any header under csrc/ or include/ is newer.
+repository snapshot), and of ltm_b200/_torch_ops.so, the tensor-level callers of
+its per-token operators (binding/torch_ops.cpp, g++ against PyTorch's headers).
+Incremental: an object is rebuilt when its source or any header under csrc/ or
+include/ is newer.
 
     python obsidian-memory-transformer_b200/build.py [--force] [-j N]
 """
@@ -20,6 +22,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "ltm_b200" / "libltm_b200.so"
+OPS_SRC = PKG / "binding" / "torch_ops.cpp"
+OPS = PKG / "ltm_b200" / "_torch_ops.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -50,6 +54,30 @@ def _compile(src: Path, obj: Path, verbose: bool) -> tuple[Path, str]:
     return obj, r.stdout + r.stderr
 
 
+def build_torch_ops(force: bool = False) -> Path:
+    """The CPython module of tensor-level callers; links to libltm_b200.so beside it."""
+    newest = max(p.stat().st_mtime for p in (OPS_SRC, ROOT / "include" / "ltm_b200.h"))
+    if not force and OPS.exists() and OPS.stat().st_mtime >= newest:
+        return OPS
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    torch_lib = Path(torch.__file__).resolve().parent / "lib"
+    inc = cpp_extension.include_paths() + [sysconfig.get_paths()["include"],
+                                           "/usr/local/cuda/include"]
+    tmp = OPS.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *[f"-isystem{i}" for i in inc], str(OPS_SRC), "-o", str(tmp), f"-L{LIB.parent}",
+           "-l:libltm_b200.so", f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {OPS_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, OPS)
+    return OPS
+
+
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.cu"))
@@ -75,6 +103,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
+    build_torch_ops(force)
     if verbose:
         for name, log in logs:
             print(f"== {name}\n{log}")

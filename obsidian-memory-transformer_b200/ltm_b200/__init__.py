@@ -12,7 +12,6 @@ from __future__ import annotations
 
 import ctypes as C
 import dataclasses
-import functools
 from pathlib import Path
 
 import numpy as np
@@ -274,26 +273,14 @@ class KernelTimer:
 
 
 # ---------------------------------------------------------------- torch glue --
-_torch_module = None
-
-
 def _torch():
-    global _torch_module
-    if _torch_module is None:
-        import torch  # noqa: WPS433
-        _torch_module = torch
-    return _torch_module
-
-
-_dtype_codes: dict = {}
+    import torch  # noqa: WPS433
+    return torch
 
 
 def dtype_code(t) -> int:
-    if not _dtype_codes:
-        torch = _torch()
-        _dtype_codes.update({torch.float32: DTYPE_F32, torch.float16: DTYPE_F16,
-                             torch.bfloat16: DTYPE_BF16})
-    return _dtype_codes[t]
+    torch = _torch()
+    return {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}[t]
 
 
 def torch_dtype(code: int):
@@ -485,111 +472,24 @@ def memory_store_noalloc(memory, keys, queries, state, num_heads: int, update_ra
 
 
 # ------------------------------------------------- KV cache, beam search --
-class _Call:
-    """Device and stream of one call: its tensors' device is made the current
-    one (done() puts the old one back), and memory made for the call is safe on a
-    stream that is not the current one."""
-
-    __slots__ = ("device", "other", "stream", "_back")
-
-    def __init__(self, t, stream):
-        C_ = _torch()._C
-        self.device = t.device
-        index = t.get_device()
-        back = C_._cuda_getDevice()
-        self._back = None
-        if back != index:
-            self._back = back
-            C_._cuda_setDevice(index)
-        self.stream = C_._cuda_getCurrentRawStream(index)
-        self.other = None
-        if stream is not None and stream.cuda_stream != self.stream:
-            self.other = stream
-            self.stream = stream.cuda_stream
-
-    def done(self, status: int) -> None:
-        if self._back is not None:
-            _torch()._C._cuda_setDevice(self._back)
-        if status != OK:
-            _check(status)
-
-    def empty(self, shape, dtype):
-        """Uninitialized contiguous memory."""
-        strides, n = [], 1
-        for d in reversed(shape):
-            strides.append(n)
-            n *= d
-        t = _torch().empty_strided(shape, strides[::-1], dtype=dtype, device=self.device)
-        if self.other is not None:
-            t.record_stream(self.other)
-        return t
+# These are called per token and layer: their checks, output memory and stream
+# are in a compiled caller of the C ABI (binding/torch_ops.cpp).
+_ops_module = None
 
 
-def _bad(msg: str):
-    raise LtmError(ERR_INVALID_ARG, msg)
-
-
-def _check_device(first, *tensors):
-    """Tensors (None allowed) on `first`'s CUDA device."""
-    index = first.get_device()
-    if index < 0:
-        raise ValueError("ltm_b200 operates on CUDA tensors only")
-    for t in tensors:
-        if t is not None and t.get_device() != index:
-            _bad("all tensors must be on one device")
-
-
-def _check_index(t, shape):
-    """A contiguous int32 tensor of `shape`."""
-    if t.dtype is not _torch().int32 or t.shape != shape or not t.is_contiguous():
-        _bad(f"lengths and indices must be contiguous int32 {list(shape)}")
-
-
-def _check_cache(cache, scale, what: str):
-    """A cache with its scales (None: not int8); returns its shape."""
-    torch = _torch()
-    shape = cache.shape
-    if len(shape) != 4 or not cache.is_contiguous():
-        _bad(f"{what} must be contiguous [B, kv_heads, max_positions, head_dim]")
-    if scale is None:
-        if cache.dtype is torch.int8:
-            _bad(f"{what}: int8 caches need scales")
-    elif (cache.dtype is not torch.int8 or scale.dtype is not torch.float32
-          or scale.shape != shape[:3] or not scale.is_contiguous()):
-        _bad(f"{what}: an int8 cache takes contiguous fp32 scales [B, kv_heads, max_positions], "
-             "other caches none")
-    return shape
-
-
-def _check_pair(k_cache, v_cache, k_scale, v_scale):
-    shape = _check_cache(k_cache, k_scale, "k_cache")
-    if _check_cache(v_cache, v_scale, "v_cache") != shape or k_cache.dtype is not v_cache.dtype:
-        _bad("k_cache and v_cache must have one shape and type")
-    return shape
-
-
-@functools.lru_cache(maxsize=256)
-def _int64s(*v):
-    return (C.c_int64 * len(v))(*v)
-
-
-def _strides3(t, what: str):
-    """Batch, token and head strides of a [B, T, heads, head_dim] view."""
-    s = t.stride()
-    if s[3] != 1:
-        _bad(f"{what} must have unit stride in head_dim")
-    return _int64s(s[0], s[1], s[2])
-
-
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(name: str, *sizes) -> int:
-    n = C.c_size_t()
-    _check(getattr(lib(), name)(*sizes, C.byref(n)))
-    return n.value
-
-
-def _dp(t):
-    return None if t is None else t.data_ptr()
+def _ops():
+    global _ops_module
+    if _ops_module is None:
+        lib()
+        _torch()
+        try:
+            from . import _torch_ops as ops
+        except ImportError as e:
+            raise RuntimeError(f"{_HERE}/_torch_ops.so cannot be loaded ({e}): build it with "
+                               "`python obsidian-memory-transformer_b200/build.py`") from e
+        ops.set_error(LtmError)
+        _ops_module = ops
+    return _ops_module
 
 
 def kv_cache_append(k, v, k_cache, v_cache, cache_lens, k_scale=None, v_scale=None,
@@ -602,25 +502,8 @@ def kv_cache_append(k, v, k_cache, v_cache, cache_lens, k_scale=None, v_scale=No
     head_dim]: int8 with fp32 scales [B, kv_heads, max_positions] (k, v f32, f16
     or bf16), or of k's type (f16 / bf16).  cache_lens, num_tokens (how many of the
     T tokens a sequence has): int32 [B].  The lengths are not advanced."""
-    _check_device(k, v, k_cache, v_cache, cache_lens, k_scale, v_scale, num_tokens)
-    cB, ch, P, cd = _check_pair(k_cache, v_cache, k_scale, v_scale)
-    shape = k.shape
-    if len(shape) != 4 or shape != v.shape or k.dtype is not v.dtype:
-        _bad("k and v must both be [B, T, kv_heads, head_dim]")
-    B, T, h, d = shape
-    if cB != B or ch != h or cd != d:
-        _bad("the caches do not fit k and v")
-    if k_scale is None and k_cache.dtype is not k.dtype:
-        _bad("the caches must be int8 or have k's type")
-    _check_index(cache_lens, (B,))
-    if num_tokens is not None:
-        _check_index(num_tokens, (B,))
-    sk, sv, dt = _strides3(k, "k"), _strides3(v, "v"), dtype_code(k.dtype)
-    c = _Call(k, stream)
-    c.done(lib().ltm_kv_cache_append(
-        k.data_ptr(), sk, v.data_ptr(), sv, dt, k_cache.data_ptr(), v_cache.data_ptr(),
-        _dp(k_scale), _dp(v_scale), P, cache_lens.data_ptr(), _dp(num_tokens), B, T, h, d,
-        c.stream))
+    _ops().kv_cache_append(k, v, k_cache, v_cache, cache_lens, k_scale, v_scale, num_tokens,
+                                 stream)
 
 
 def kv_cache_read(cache, scale, length: int, first=None, cache_lens=None, dtype=None, out=None,
@@ -630,28 +513,7 @@ def kv_cache_read(cache, scale, length: int, first=None, cache_lens=None, dtype=
     caches give code * scale in `dtype` (f32, f16 or bf16; f32 when None), other caches
     (scale None) their values.  Positions outside [0, cache_lens[b]) (int32 [B];
     max_positions when None) give zeros."""
-    _check_device(cache, scale, first, cache_lens, out)
-    B, h, P, d = _check_cache(cache, scale, "cache")
-    if length < 0:
-        _bad("length must not be negative")
-    if dtype is None:
-        dtype = cache.dtype if scale is None else _torch().float32
-    if scale is None and dtype is not cache.dtype:
-        _bad("a 16-bit cache is read in its own type")
-    if first is not None:
-        _check_index(first, (B,))
-    if cache_lens is not None:
-        _check_index(cache_lens, (B,))
-    shape, dt = (B, h, length, d), dtype_code(dtype)
-    if out is not None and (out.shape != shape or out.dtype is not dtype
-                            or not out.is_contiguous()):
-        _bad(f"out must be contiguous {list(shape)} of the read type")
-    c = _Call(cache, stream)
-    if out is None:
-        out = c.empty(shape, dtype)
-    c.done(lib().ltm_kv_cache_read(cache.data_ptr(), _dp(scale), dt, P, _dp(first),
-                                   _dp(cache_lens), B, h, d, length, out.data_ptr(), c.stream))
-    return out
+    return _ops().kv_cache_read(cache, scale, length, first, cache_lens, dtype, out, stream)
 
 
 def tree_attention(q, k_cache, v_cache, cache_lens, parents=None, k_scale=None, v_scale=None,
@@ -665,33 +527,8 @@ def tree_attention(q, k_cache, v_cache, cache_lens, parents=None, k_scale=None, 
     have been appended (kv_cache_append).  parents: int32 [B, T], -1 for a root;
     None for a chain.  num_tokens: int32 [B], how many of the T tokens a sequence
     has (the others get zeros).  Returns [B, T, heads, head_dim]."""
-    _check_device(q, k_cache, v_cache, cache_lens, parents, k_scale, v_scale, num_tokens, out)
-    cB, kvh, P, cd = _check_pair(k_cache, v_cache, k_scale, v_scale)
-    shape, qt = q.shape, q.dtype
-    if len(shape) != 4 or cB != shape[0] or cd != shape[3]:
-        _bad("q must be [B, T, heads, head_dim] for the caches' B and head_dim")
-    if k_scale is None and k_cache.dtype is not qt:
-        _bad("the caches must be int8 or have q's type")
-    B, T, heads, d = shape
-    _check_index(cache_lens, (B,))
-    if num_tokens is not None:
-        _check_index(num_tokens, (B,))
-    if parents is not None:
-        _check_index(parents, (B, T))
-    if out is not None and (out.shape != shape or out.dtype is not qt):
-        _bad("out must have q's shape and type")
-    sq, dt = _strides3(q, "q"), dtype_code(qt)
-    so = (_int64s(T * heads * d, heads * d, d) if out is None else _strides3(out, "out"))
-    nbytes = _workspace_bytes("ltm_tree_attention_workspace", B, T, heads, kvh, d)
-    c = _Call(q, stream)
-    if out is None:
-        out = c.empty(shape, qt)
-    ws = c.empty((nbytes,), _torch().uint8)
-    c.done(lib().ltm_tree_attention(
-        q.data_ptr(), sq, k_cache.data_ptr(), v_cache.data_ptr(), _dp(k_scale), _dp(v_scale), P,
-        cache_lens.data_ptr(), _dp(num_tokens), _dp(parents), out.data_ptr(), so, B, T, heads, kvh,
-        d, dt, ws.data_ptr(), nbytes, c.stream))
-    return out
+    return _ops().tree_attention(q, k_cache, v_cache, cache_lens, parents, k_scale, v_scale,
+                                       num_tokens, out, stream)
 
 
 def beam_select(logits, scores, num_out: int | None = None, done=None, end_token: int = -1,
@@ -702,31 +539,7 @@ def beam_select(logits, scores, num_out: int | None = None, done=None, end_token
     int32) of the K = num_out (W when None) best continuations, best first.  With
     `done` (bool [B, W]) finished beams continue as themselves with `end_token`
     and a fourth output [B, K] bool says which continuations are finished."""
-    torch = _torch()
-    _check_device(logits, scores, done)
-    shape, strides = logits.shape, logits.stride()
-    if len(shape) != 3 or strides[2] != 1:
-        _bad("logits must be [B, W, V] with unit stride in V")
-    B, W, V = shape
-    if scores.dtype is not torch.float32 or scores.shape != (B, W) or not scores.is_contiguous():
-        _bad("scores must be contiguous fp32 [B, W]")
-    if done is not None and (done.dtype is not torch.bool or done.shape != (B, W)
-                             or not done.is_contiguous()):
-        _bad("done must be contiguous bool [B, W]")
-    K = W if num_out is None else num_out
-    sb, sw, _ = strides
-    dt = dtype_code(logits.dtype)
-    nbytes = _workspace_bytes("ltm_beam_select_workspace", B, W, V, K)
-    c = _Call(logits, stream)
-    best = c.empty((B, K), torch.float32)
-    beams, tokens = c.empty((B, K), torch.int32), c.empty((B, K), torch.int32)
-    fin = c.empty((B, K), torch.bool) if done is not None else None
-    ws = c.empty((nbytes,), torch.uint8)
-    c.done(lib().ltm_beam_select(
-        logits.data_ptr(), dt, sb, sw, scores.data_ptr(), _dp(done), end_token, B, W, V, K,
-        best.data_ptr(), beams.data_ptr(), tokens.data_ptr(), _dp(fin), ws.data_ptr(), nbytes,
-        c.stream))
-    return (best, beams, tokens) if fin is None else (best, beams, tokens, fin)
+    return _ops().beam_select(logits, scores, num_out, done, end_token, stream)
 
 
 def kv_cache_reorder(caches, beams, cache_lens=None, first=None, stream=None) -> None:
@@ -736,33 +549,7 @@ def kv_cache_reorder(caches, beams, cache_lens=None, first=None, stream=None) ->
     max_positions, head_dim] tensors (K and V of all layers) and [B * W, kv_heads,
     max_positions] tensors (int8 caches' scales), each once; beams int32 [B, W];
     cache_lens, first: int32 [B] (max_positions and 0 when None)."""
-    caches = list(caches)
-    _check_device(beams, cache_lens, first, *caches)
-    shape = beams.shape
-    if len(shape) != 2:
-        _bad("beams must be int32 [B, W]")
-    _check_index(beams, shape)
-    B, W = shape
-    if cache_lens is not None:
-        _check_index(cache_lens, (B,))
-    if first is not None:
-        _check_index(first, (B,))
-    n = len(caches)
-    if n == 0:
-        return
-    lead, ptrs, rows = caches[0].shape[:3], [], []
-    for t in caches:
-        s = t.shape
-        if s[:3] != lead or not 3 <= len(s) <= 4 or not t.is_contiguous():
-            _bad("caches must be contiguous [B * W, kv_heads, max_positions(, head_dim)]")
-        ptrs.append(t.data_ptr())
-        rows.append(t.element_size() * (s[3] if len(s) == 4 else 1))
-    if len(lead) != 3 or lead[0] != B * W:
-        _bad("caches must have B * W sequences")
-    ptrs, rows = (C.c_void_p * n)(*ptrs), _int64s(*rows)
-    c = _Call(beams, stream)
-    c.done(lib().ltm_kv_cache_reorder(ptrs, rows, n, beams.data_ptr(), _dp(first),
-                                      _dp(cache_lens), B, W, lead[1], lead[2], c.stream))
+    _ops().kv_cache_reorder(caches, beams, cache_lens, first, stream)
 
 
 # --------------------------------------------------------------------- block --
