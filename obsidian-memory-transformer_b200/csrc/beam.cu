@@ -15,7 +15,8 @@
 // n * H_n for n groups, 22 for 8 beams), so only those are compacted and ranked.
 // Where too many pass (long runs of equal or masked logits) the K best are
 // taken one by one instead.  beam_merge_kernel (one CTA per request) evaluates the
-// totals of the chunks' sorted lists in 64 bits, because nearly equal totals of
+// totals of the chunks' sorted lists in 64 bits (the fp32 logarithm of the row's sum
+// aside), because nearly equal totals of
 // different beams decide the order, and filters and ranks them the same way;
 // within a row the order is that of the logits.
 //
@@ -327,6 +328,7 @@ __device__ __forceinline__ bool before(const Total& a, const Total& b) {
 
 constexpr int kMergeCand = 512;   // continuations ranked in shared memory
 constexpr int kMergeKeys = 8192;  // entries whose keys fit in shared memory
+constexpr int kMergeAll = 128;    // entries that are ranked without a bound
 constexpr int kMergeSlack = 24;   // continuations past K that are ranked rather than sorted out
 
 // One CTA per request.  Its W * nchunk lists are sorted, so the best
@@ -375,7 +377,7 @@ __global__ void __launch_bounds__(kBThreads)
     if (lane == 0) {
       const float s = sc == sc ? sc : -INFINITY;
       s_max[w] = m;
-      s_base[w] = static_cast<double>(s) - log(static_cast<double>(sum));
+      s_base[w] = static_cast<double>(s) - static_cast<double>(logf(sum));
       s_score[w] = s;
       s_done[w] = done != nullptr && done[row] != 0;
     }
@@ -400,6 +402,22 @@ __global__ void __launch_bounds__(kBThreads)
     out_tokens[o] = tok;
     if (out_done) out_done[o] = s_done[w] || tok == end;
   };
+  auto rank_all = [&](int n) {
+#pragma unroll 1
+    for (int i = tid; i < n; i += kBThreads) {
+      const Total x = s_cand[i];
+      int rank = 0;
+#pragma unroll 2
+      for (int j = 0; j < n; ++j) rank += before(s_cand[j], x);
+      if (rank < K) put(rank, x);
+    }
+  };
+  if (entries <= kMergeAll) {  // few enough to rank as they are
+    if (tid < entries) s_cand[tid] = entry(tid / K, tid);
+    __syncthreads();
+    rank_all(entries);
+    return;
+  }
   // ---- the bound: `low` is reached by at least K continuations
   const bool staged = entries <= kMergeKeys;
   auto key_of = [&](int i) -> uint32_t {
@@ -465,14 +483,7 @@ __global__ void __launch_bounds__(kBThreads)
     for (int i = tid; i < entries; i += kBThreads)
       if (key_of(i) >= low) s_cand[atomicAdd(&s_count[0], 1)] = entry(i / K, i);
     __syncthreads();
-#pragma unroll 1
-    for (int i = tid; i < n; i += kBThreads) {
-      const Total x = s_cand[i];
-      int rank = 0;
-#pragma unroll 2
-      for (int j = 0; j < n; ++j) rank += before(s_cand[j], x);
-      if (rank < K) put(rank, x);
-    }
+    rank_all(n);
     return;
   }
   Total last{~0ull, 0u, 0u};

@@ -777,14 +777,15 @@ struct TcSmem {
   static constexpr int kSlots = kLeft / kTile > 8 ? 8 : kLeft / kTile;
   static constexpr int kOffMax = kOffRing + kSlots * kTile;  // [4][N] maxima / sums
   static constexpr int kOffRef = kOffMax + 4 * N * 4;        // [N] -reference, [N] factor
-  static constexpr int kOffMask = kOffRef + 2 * N * 4;       // [8][64] ancestor sets
-  static constexpr int kOffBase = kOffMask + 8 * kTMaxTokens * 8;
+  static constexpr int kOffMask = kOffRef + 2 * N * 4;       // [softmax warps][rows] ancestor sets
+  static constexpr int kOffBase = kOffMask + 4 * N * 8;
   static constexpr int kOffBar = (kOffBase + (kTBatch + 2) * 4 + 7) / 8 * 8;
   static constexpr int kBars = 2 * kSlots + 8;
   static constexpr int kOffFlag = kOffBar + kBars * 8;
   static constexpr int kBytes = kOffFlag + 48 + 1024;
-  // softmax: groups of four warps, each with up to 64 of the block's rows
-  static constexpr int kRows = N < 64 ? N : 64, kGroups = N / kRows;
+  // softmax: groups of four warps, each with 32 rows, or with 64 of 128 (four groups would
+  // leave 96 registers a thread: 2.1 -> 3.0 us a tile)
+  static constexpr int kRows = N <= 64 ? 32 : 64, kGroups = N / kRows;
   static_assert(kBytes <= 232448, "shared memory of one CTA");
 };
 
@@ -824,9 +825,9 @@ __device__ __forceinline__ void soft_sync() {
 
 // warp 0: TMA producer (K(0), V(0), K(1), ... into the ring); warp 1: TMEM and
 // the MMAs, in the order S(0), S(1), O(0), S(2), O(1), ... within a head's
-// segment; warps 4-7 (and 8-11 for the upper 64 of 128 rows): softmax, thread =
-// key = TMEM lane.  TMEM: S^T twice, O^T.  The softmax reads a row block of S twice,
-// 32 rows at a time (for the vote, then for the exponentials), instead of holding it.
+// segment; warps 4-7 (and 8-11 for the upper half of 64 or 128 rows): softmax,
+// thread = key = TMEM lane.  TMEM: S^T twice, O^T.  The softmax reads its rows of S
+// twice, 32 at a time (for the vote, then for the exponentials), instead of holding them.
 template <class T, int D, int N>
 __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -984,7 +985,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
     const int r0 = (sw >> 2) * RW;
     const uint32_t lane_off = static_cast<uint32_t>(q4 * 32) << 16;
     unsigned long long* mask =
-        reinterpret_cast<unsigned long long*>(smem + S::kOffMask) + sw * kTMaxTokens;
+        reinterpret_cast<unsigned long long*>(smem + S::kOffMask) + sw * RW;
     auto wait_warp = [&](uint64_t* bar, uint32_t parity) -> bool {
       const bool r = mbar_wait_bounded(bar, parity, abort_flag, p.err, kErrWaitAccum);
       return __all_sync(0xffffffffu, r);
