@@ -1072,6 +1072,72 @@ class TitanModel:
             trace.append(hid.clone())
         return out, trace
 
+    def generate_beam(self, prompt, new_tokens: int, num_beams: int, end_token: int | None = None,
+                      max_positions: int | None = None, use_graph: bool = True):
+        """Beam search of `new_tokens` tokens after the prompts (CUDA int32
+        [B,S]): one prefill a prompt, then per token one decode step of all B *
+        num_beams beams, beam_select and kv_cache_reorder (only the generated
+        positions move: the beams of a prompt share its keys and values), on the
+        device (the step captured once in a CUDA graph and replayed when
+        use_graph).  Beams that reach end_token are finished: they keep their
+        score and repeat end_token.  Returns (tokens [B, num_beams, new_tokens],
+        scores fp32 [B, num_beams]), best first; a score is the sum of the tokens'
+        log-probabilities."""
+        torch = _torch()
+        B, S = prompt.shape
+        W, P, dev = num_beams, max_positions or S + new_tokens, prompt.device
+        if new_tokens < 1 or W < 1 or P < S + new_tokens - 1:
+            raise LtmError(ERR_INVALID_ARG, "beam search needs a token, a beam and room in the cache")
+        one = self.make_cache(B, S)
+        _, logits = self.prefill(prompt, one)
+        cache = self.make_cache(B * W, P)
+        for src, dst in zip(one._k + one._v, cache._k + cache._v):
+            dst.unflatten(0, (B, W))[:, :, :, :S] = src[:, None]
+        del one
+        end = -1 if end_token is None else end_token
+        none = None if end_token is None else torch.zeros((B, 1), dtype=torch.bool, device=dev)
+        first = beam_select(logits[:, None], torch.zeros((B, 1), device=dev), W, none, end)
+        scores, beams, tok = first[0], first[1], first[2].reshape(-1)
+        done = first[3] if end_token is not None else None
+        start = torch.full((B,), S, dtype=torch.int32, device=dev)
+        lens = torch.full((B * W,), S, dtype=torch.int32, device=dev)
+        ends = start + 1  # positions in the caches after a step, per prompt
+        tokens = torch.empty((new_tokens, B, W), dtype=torch.int32, device=dev)
+        parents = torch.empty((new_tokens, B, W), dtype=torch.int32, device=dev)
+        tokens[0], parents[0] = tok.view(B, W), beams
+        step_logits = torch.empty((B * W, self.vocab), dtype=logits.dtype, device=dev)
+
+        def step():
+            self.decode_step(tok, lens, cache, logits=step_logits)
+            r = beam_select(step_logits.view(B, W, -1), scores, W, done, end)
+            kv_cache_reorder(cache._k + cache._v, r[1], ends, first=start)
+            scores.copy_(r[0])
+            beams.copy_(r[1])
+            tok.copy_(r[2].view(-1))
+            if done is not None:
+                done.copy_(r[3])
+            lens.add_(1)
+            ends.add_(1)
+
+        graph = None
+        for i in range(1, new_tokens):
+            if use_graph and graph is None and i >= 2:
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, capture_error_mode="relaxed"):
+                    step()
+            if graph is not None:
+                graph.replay()
+            else:
+                step()
+            tokens[i], parents[i] = tok.view(B, W), beams
+        # each final beam's tokens, back along its parents
+        out = torch.empty((B, W, new_tokens), dtype=torch.int32, device=dev)
+        at = torch.arange(W, device=dev).expand(B, W)
+        for i in range(new_tokens - 1, -1, -1):
+            out[:, :, i] = tokens[i].gather(1, at)
+            at = parents[i].gather(1, at).long()
+        return out, scores
+
     def close(self) -> None:
         if getattr(self, "_h", None):
             lib().ltm_model_destroy(self._h)
