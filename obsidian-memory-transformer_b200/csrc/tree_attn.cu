@@ -57,6 +57,7 @@ constexpr int kTBatch = 512;      // sequences per launch
 constexpr int kTMaxGrid = 256;    // CTAs that share the tiles, whatever the device
 constexpr int kTMaxTokens = 64;   // drafted tokens (one 64-bit ancestor mask)
 constexpr float kTRaise = 8.0f;   // log2 of the largest probability before the reference is raised
+constexpr float kTMost = 256.0f;  // 2^kTRaise
 
 struct TreeParams {
   const void* q;
@@ -762,7 +763,8 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
 }
 
 // ------------------------------------------------------------ tcgen05 kernel --
-// Shared memory: Q [N rows x D] (K-major), P [128 keys x N] (N contiguous), a ring
+// Shared memory: Q [N rows x D] (K-major), P [128 keys x N] (N contiguous; twice up to 64
+// rows, so that P(j + 1) is written while P(j) is contracted), a ring
 // of 128-position K and V tiles, all in 128-byte-swizzled chunks of 64 columns.
 template <int D, int N>
 struct TcSmem {
@@ -770,7 +772,9 @@ struct TcSmem {
   static constexpr int kQChunk = N * 128;             // N rows x 64 dims
   static constexpr int kQ = (D / 64) * kQChunk;
   static constexpr int kPChunk = kTcTile * 128;        // 128 keys x 64 rows
-  static constexpr int kP = ((N + 63) / 64) * kPChunk;
+  static constexpr int kPOne = ((N + 63) / 64) * kPChunk;
+  static constexpr int kPs = N <= 64 ? 2 : 1;         // P buffers
+  static constexpr int kP = kPs * kPOne;
   static constexpr int kOffP = kQ;
   static constexpr int kOffRing = kOffP + kP;
   static constexpr int kLeft = 222 * 1024 - kOffRing;
@@ -780,7 +784,7 @@ struct TcSmem {
   static constexpr int kOffMask = kOffRef + 2 * N * 4;       // [softmax warps][rows] ancestor sets
   static constexpr int kOffBase = kOffMask + 4 * N * 8;
   static constexpr int kOffBar = (kOffBase + (kTBatch + 2) * 4 + 7) / 8 * 8;
-  static constexpr int kBars = 2 * kSlots + 8;
+  static constexpr int kBars = 2 * kSlots + 10;
   static constexpr int kOffFlag = kOffBar + kBars * 8;
   static constexpr int kBytes = kOffFlag + 48 + 1024;
   // softmax: groups of four warps, each with 32 rows, or with 64 of 128 (four groups would
@@ -834,7 +838,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
                    const TreeParams p) {
   using S = TcSmem<D, N>;
   constexpr int NS = S::kSlots;
-  constexpr int RW = S::kRows, NC = RW / 32, kSoft = 128 * S::kGroups;
+  constexpr int RW = S::kRows, NC = RW / 32, kSoft = 128 * S::kGroups, PB = S::kPs;
   constexpr uint32_t kCols = N <= 32 ? 128 : N <= 64 ? 256 : 512;  // 3 N columns
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -848,9 +852,9 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
   uint64_t* q_full = empty + NS;  // an arrival per softmax warp: q_full, s_free, p_full
   uint64_t* s_full = q_full + 1;  // [2]
   uint64_t* s_free = s_full + 2;  // [2]
-  uint64_t* p_full = s_free + 2;
-  uint64_t* pv_done = p_full + 1;
-  uint64_t* drained = pv_done + 1;
+  uint64_t* p_full = s_free + 2;  // [2], as is pv_done: by P buffer
+  uint64_t* pv_done = p_full + 2;
+  uint64_t* drained = pv_done + 2;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kOffFlag);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + S::kOffFlag) + 1;
   int* wait_ok = reinterpret_cast<int*>(tslot) + 1;  // [softmax warps]
@@ -859,7 +863,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
   if (threadIdx.x == 32) {
     for (int i = 0; i < S::kBars; ++i) {
       const bool per_warp = full + i == q_full || full + i == s_free || full + i == s_free + 1 ||
-                            full + i == p_full;
+                            full + i == p_full || full + i == p_full + 1;
       mbar_init(full + i, per_warp ? kSoft / 32 : 1);
     }
     *abort_flag = 0;
@@ -949,15 +953,17 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
         return true;
       };
       auto issue_o = [&](int j, bool first) -> bool {
-        if (!mbar_wait_bounded(p_full, j & 1, abort_flag, p.err, kErrWaitFull)) return false;
+        const int pb = j % PB;
+        if (!mbar_wait_bounded(p_full + pb, (j / PB) & 1, abort_flag, p.err, kErrWaitFull))
+          return false;
         if (!slot_wait(2 * j + 1)) return false;
         tc_fence_after();
         const uint32_t aV = ring + ((2 * j + 1) % NS) * S::kTile;
 #pragma unroll
         for (int k = 0; k < kTcTile / 16; ++k)
           tc_mma_f16(tO, make_desc_mnmajor_sw128(aV + k * 2048, kVChunk),
-                     make_desc_mnmajor_sw128(aP + k * 2048, S::kPChunk), idO, !first || k != 0);
-        tc_commit(pv_done);
+                     make_desc_mnmajor_sw128(aP + pb * S::kPOne + k * 2048, S::kPChunk), idO, !first || k != 0);
+        tc_commit(pv_done + pb);
         tc_commit(empty + (2 * j + 1) % NS);
         return true;
       };
@@ -989,6 +995,9 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
     auto wait_warp = [&](uint64_t* bar, uint32_t parity) -> bool {
       const bool r = mbar_wait_bounded(bar, parity, abort_flag, p.err, kErrWaitAccum);
       return __all_sync(0xffffffffu, r);
+    };
+    auto wait_pv = [&](int j) -> bool {  // tile j's value product is in O
+      return wait_warp(pv_done + j % PB, (j / PB) & 1);
     };
     int it = 0;
     bool ok = true;
@@ -1063,24 +1072,45 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
                                          (((u & 7) ^ (kt & 7)) << 4), at >= sp.n);
           }
         }
-        // ---- does a score pass its row's reference by more than the margin?
+        // ---- does a score pass its row's reference by more than the margin?  With 32 rows
+        // the exponentials are taken at once and looked at afterwards
+        auto expo = [&](uint32_t (&x)[32], int c) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 nr = *reinterpret_cast<const float4*>(nref + r0 + c * 32 + i);
+            const float n4[4] = {nr.x, nr.y, nr.z, nr.w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              x[i + y] = __float_as_uint(
+                  ex2_approx(fmaf(__uint_as_float(x[i + y]), p.sl2, n4[y])));
+          }
+        };
+        uint32_t e[32];  // NC == 1: the tile's exponentials
         bool need = first || !got;
         if (!need) {
           float top = -INFINITY;
+          if constexpr (NC == 1) {
+            scores(0, e);
+            expo(e, 0);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            uint32_t s[32];
-            scores(c, s);
+            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(e[i]));
+            need = top > kTMost;
+          } else {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 nr = *reinterpret_cast<const float4*>(nref + r0 + c * 32 + i);
-              top = fmaxf(top, fmaxf(fmaf(__uint_as_float(s[i]), p.sl2, nr.x),
-                                     fmaf(__uint_as_float(s[i + 1]), p.sl2, nr.y)));
-              top = fmaxf(top, fmaxf(fmaf(__uint_as_float(s[i + 2]), p.sl2, nr.z),
-                                     fmaf(__uint_as_float(s[i + 3]), p.sl2, nr.w)));
+            for (int c = 0; c < NC; ++c) {
+              uint32_t s[32];
+              scores(c, s);
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const float4 nr = *reinterpret_cast<const float4*>(nref + r0 + c * 32 + i);
+                top = fmaxf(top, fmaxf(fmaf(__uint_as_float(s[i]), p.sl2, nr.x),
+                                       fmaf(__uint_as_float(s[i + 1]), p.sl2, nr.y)));
+                top = fmaxf(top, fmaxf(fmaf(__uint_as_float(s[i + 2]), p.sl2, nr.z),
+                                       fmaf(__uint_as_float(s[i + 3]), p.sl2, nr.w)));
+              }
             }
+            need = top > kTRaise;
           }
-          need = top > kTRaise;
         }
         if (soft_any<kSoft>(need)) {
           if (got) {
@@ -1115,7 +1145,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
           soft_sync<kSoft>();
           // O is final up to the tile before; rescale it and the sums (where the wait
           // runs out, the next vote ends the segment)
-          if (!first && wait_warp(pv_done, (it - 1) & 1)) {
+          if (!first && wait_pv(it - 1)) {
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
@@ -1132,45 +1162,43 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
             }
             tmem_wait_st();
           }
+          if constexpr (NC == 1) {
+            scores(0, e);
+            expo(e, 0);
+          }
         }
         // ---- probabilities, their sums, and P (16 bits, this key's row)
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          uint32_t s[32], pk[16];
-          scores(c, s);
+          uint32_t pk[16];
+          if constexpr (NC > 1) scores(c, e);
           if (c == NC - 1) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(s_free + (it & 1));  // S may be overwritten
           }
+          if constexpr (NC > 1) expo(e, c);
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 nr = *reinterpret_cast<const float4*>(nref + r0 + c * 32 + i);
-            const float e0 = ex2_approx(fmaf(__uint_as_float(s[i]), p.sl2, nr.x));
-            const float e1 = ex2_approx(fmaf(__uint_as_float(s[i + 1]), p.sl2, nr.y));
-            const float e2 = ex2_approx(fmaf(__uint_as_float(s[i + 2]), p.sl2, nr.z));
-            const float e3 = ex2_approx(fmaf(__uint_as_float(s[i + 3]), p.sl2, nr.w));
-            l[c * 32 + i] += e0;
-            l[c * 32 + i + 1] += e1;
-            l[c * 32 + i + 2] += e2;
-            l[c * 32 + i + 3] += e3;
-            pk[i / 2] = pack16<std::is_same<T, __nv_bfloat16>::value>(e0, e1);
-            pk[i / 2 + 1] = pack16<std::is_same<T, __nv_bfloat16>::value>(e2, e3);
+          for (int i = 0; i < 32; i += 2) {
+            const float a = __uint_as_float(e[i]), b = __uint_as_float(e[i + 1]);
+            l[c * 32 + i] += a;
+            l[c * 32 + i + 1] += b;
+            pk[i / 2] = pack16<std::is_same<T, __nv_bfloat16>::value>(a, b);
           }
-          // P is free once the tile before has been contracted
-          if (c == 0 && !first) wait_warp(pv_done, (it - 1) & 1);
+          // this P buffer is free once the tile that was in it has been contracted
+          if (c == 0 && it >= PB) wait_pv(it - PB);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int u = (r0 + c * 32) / 8 + x;
-            *reinterpret_cast<uint4*>(smem + S::kOffP + (u >> 3) * S::kPChunk + kt * 128 +
-                                      (((u & 7) ^ (kt & 7)) << 4)) =
+            *reinterpret_cast<uint4*>(smem + S::kOffP + (it % PB) * S::kPOne + (u >> 3) * S::kPChunk +
+                                      kt * 128 + (((u & 7) ^ (kt & 7)) << 4)) =
                 make_uint4(pk[4 * x], pk[4 * x + 1], pk[4 * x + 2], pk[4 * x + 3]);
           }
         }
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
+        if (lane == 0) mbar_arrive(p_full + it % PB);
       }
       if (!ok) break;
       // ---- the segment's partial
@@ -1182,15 +1210,16 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
         smax[q4 * N + r0 + c * 32 + lane] = across_lanes<true>(v, lane);
       }
       const bool any_taken = soft_any<kSoft>(taken);
-      ok = wait_warp(pv_done, (it - 1) & 1);
+      ok = wait_pv(it - 1);
       if (ok) {
         tc_fence_after();
         const int64_t item = head * p.nrb + sp.rb;
         float* pp = p.part + (static_cast<int64_t>(blockIdx.x) + item) * N * part_stride<D>();
         if (tid < sp.rows) {
           float* row = pp + tid * part_stride<D>();
-          row[D] = -nref[tid];
-          row[D + 1] = (smax[tid] + smax[N + tid]) + (smax[2 * N + tid] + smax[3 * N + tid]);
+          const float sum = (smax[tid] + smax[N + tid]) + (smax[2 * N + tid] + smax[3 * N + tid]);
+          row[D] = sum == 0.0f ? -INFINITY : -nref[tid];  // a row that sees nothing here
+          row[D + 1] = sum;
           row[D + 2] = any_taken ? 1.0f : 0.0f;
         }
         if (D == 128 || q4 < 2) {  // thread = output dim
