@@ -355,12 +355,19 @@ __global__ void __launch_bounds__(kBThreads)
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int nlists = W * nchunk, entries = nlists * K;
   const uint64_t* mine = lists + static_cast<int64_t>(b) * entries;
+  for (int w = tid; w < W; w += kBThreads) {
+    const float sc = scores[b * W + w];
+    s_score[w] = sc == sc ? sc : -INFINITY;
+    s_done[w] = done != nullptr && done[b * W + w] != 0;
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the chunks' kernel has completed
+  const bool all = entries <= kMergeAll;  // few enough to rank as they are
+  const uint64_t own = all && tid < entries ? mine[tid] : 0ull;  // in flight with the sums
+  __syncthreads();
   // a row's maximum and sum over its chunks: one warp per row
 #pragma unroll 1
   for (int w = warp; w < W; w += kBThreads / 32) {
     const int row = b * W + w;
-    const float sc = scores[row];
     float m = -INFINITY, sum = 0.0f;
 #pragma unroll 1
     for (int c0 = 0; c0 < nchunk; c0 += 32) {
@@ -375,16 +382,12 @@ __global__ void __launch_bounds__(kBThreads)
       m = mm;
     }
     if (lane == 0) {
-      const float s = sc == sc ? sc : -INFINITY;
       s_max[w] = m;
-      s_base[w] = static_cast<double>(s) - static_cast<double>(logf(sum));
-      s_score[w] = s;
-      s_done[w] = done != nullptr && done[row] != 0;
+      s_base[w] = s_score[w] - static_cast<double>(logf(sum));
     }
   }
   __syncthreads();
-  auto entry = [&](int l, int i) -> Total {  // list l, entry i of all
-    const uint64_t key = mine[i];
+  auto total = [&](int l, uint64_t key) -> Total {  // of a key of list l
     if (key == 0ull) return Total{0ull, ~0u, 0u};
     const uint32_t u = static_cast<uint32_t>(key >> 32);
     const int w = l / nchunk;
@@ -393,6 +396,7 @@ __global__ void __launch_bounds__(kBThreads)
       t = s_done[w] ? s_score[w] : s_base[w] + (static_cast<double>(unordered(u)) - s_max[w]);
     return Total{ordered64(t), static_cast<uint32_t>(w) * V + ~static_cast<uint32_t>(key), 0u};
   };
+  auto entry = [&](int l, int i) { return total(l, mine[i]); };  // entry i of all
   auto put = [&](int k, const Total& x) {
     const int w = static_cast<int>(x.f / static_cast<uint32_t>(V));
     const int tok = static_cast<int>(x.f) - w * V;
@@ -412,8 +416,8 @@ __global__ void __launch_bounds__(kBThreads)
       if (rank < K) put(rank, x);
     }
   };
-  if (entries <= kMergeAll) {  // few enough to rank as they are
-    if (tid < entries) s_cand[tid] = entry(tid / K, tid);
+  if (all) {
+    if (tid < entries) s_cand[tid] = total(tid / K, own);
     __syncthreads();
     rank_all(entries);
     return;

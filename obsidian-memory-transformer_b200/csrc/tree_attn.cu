@@ -54,6 +54,7 @@ namespace {
 
 constexpr int kTcTile = 128;      // cache positions per tile of the tcgen05 kernel
 constexpr int kTBatch = 512;      // sequences per launch
+constexpr int kScanWords = 3 * (kTBatch + 2);  // what tree_scan leaves
 constexpr int kTMaxGrid = 256;    // CTAs that share the tiles, whatever the device
 constexpr int kTMaxTokens = 64;   // drafted tokens (one 64-bit ancestor mask)
 constexpr float kTRaise = 8.0f;   // log2 of the largest probability before the reference is raised
@@ -99,7 +100,8 @@ __device__ __forceinline__ int row_blocks(const TreeParams& p, int n) {
   return (p.G * n + p.rb - 1) / p.rb;
 }
 
-// First tile of every sequence in the batch's list (one warp).
+// First tile of every sequence in the batch's list, and the sequences' lengths and
+// token counts after it ([kTBatch + 2] words each), by one warp.
 __device__ __forceinline__ void tree_scan(const TreeParams& p, uint32_t* base, int lane) {
   uint32_t carry = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
@@ -109,6 +111,8 @@ __device__ __forceinline__ void tree_scan(const TreeParams& p, uint32_t* base, i
       int len, n;
       tree_seq(p, b, len, n);
       w = static_cast<uint32_t>(p.kvh) * row_blocks(p, n) * tiles_of(p, len, n);
+      base[kTBatch + 2 + b] = static_cast<uint32_t>(len);
+      base[2 * (kTBatch + 2) + b] = static_cast<uint32_t>(n);
     }
     uint32_t s = w;
 #pragma unroll
@@ -144,7 +148,8 @@ __device__ __forceinline__ TreeSpan tree_find(const TreeParams& p, const uint32_
   }
   TreeSpan s;
   s.b = lo;
-  tree_seq(p, lo, s.len, s.n);
+  s.len = static_cast<int>(base[kTBatch + 2 + lo]);
+  s.n = static_cast<int>(base[2 * (kTBatch + 2) + lo]);
   s.tiles = tiles_of(p, s.len, s.n);
   const int nrb = row_blocks(p, s.n);
   const uint32_t at = w - base[lo];
@@ -330,13 +335,13 @@ struct MmaSmem {
   static constexpr int kTile = kKeys * kRow;               // K or V tile
   static constexpr int kMergeRow = D + 4;                  // output, max, sum
   static constexpr int kMerge = kWarps * kRows * kMergeRow * 4;
-  static constexpr int kFit = (214 * 1024 - kMerge) / kTile;
+  static constexpr int kFit = (212 * 1024 - kMerge) / kTile;
   static constexpr int kSlots = kFit > 8 ? 8 : kFit;
   static_assert(kTile % 1024 == 0 && kSlots >= 4, "swizzle atoms; K and V of two tiles");
   static constexpr int kOffMerge = kSlots * kTile;         // [warps][rows]
   static constexpr int kOffMask = kOffMerge + kMerge;  // [warps][rows]
   static constexpr int kOffBase = kOffMask + kWarps * kRows * 8;
-  static constexpr int kOffBar = kOffBase + (kTBatch + 2) * 4;
+  static constexpr int kOffBar = kOffBase + kScanWords * 4;
   static constexpr int kOffFlag = kOffBar + 2 * kSlots * 8;
   static constexpr int kBytes = kOffFlag + 128 + 1024;
   static_assert(kBytes <= 232448, "shared memory of one CTA");
@@ -777,13 +782,13 @@ struct TcSmem {
   static constexpr int kP = kPs * kPOne;
   static constexpr int kOffP = kQ;
   static constexpr int kOffRing = kOffP + kP;
-  static constexpr int kLeft = 222 * 1024 - kOffRing;
+  static constexpr int kLeft = 217 * 1024 - kOffRing;
   static constexpr int kSlots = kLeft / kTile > 8 ? 8 : kLeft / kTile;
   static constexpr int kOffMax = kOffRing + kSlots * kTile;  // [4][N] maxima / sums
   static constexpr int kOffRef = kOffMax + 4 * N * 4;        // [N] -reference, [N] factor
   static constexpr int kOffMask = kOffRef + 2 * N * 4;       // [softmax warps][rows] ancestor sets
   static constexpr int kOffBase = kOffMask + 4 * N * 8;
-  static constexpr int kOffBar = (kOffBase + (kTBatch + 2) * 4 + 7) / 8 * 8;
+  static constexpr int kOffBar = (kOffBase + kScanWords * 4 + 7) / 8 * 8;
   static constexpr int kBars = 2 * kSlots + 10;
   static constexpr int kOffFlag = kOffBar + kBars * 8;
   static constexpr int kBytes = kOffFlag + 48 + 1024;
@@ -1257,7 +1262,7 @@ constexpr int kCWarps = 8;  // query rows per CTA
 template <class T, int D>
 __global__ void __launch_bounds__(32 * kCWarps) tree_combine_kernel(const TreeParams p) {
   constexpr int DL = D / 32;
-  __shared__ uint32_t base[kTBatch + 2];
+  __shared__ uint32_t base[kScanWords];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (warp == 0) tree_scan(p, base, lane);
   __syncthreads();
@@ -1269,9 +1274,12 @@ __global__ void __launch_bounds__(32 * kCWarps) tree_combine_kernel(const TreePa
   const int bh = row / R, r = row - bh * R;
   const int b = bh / p.kvh, h = bh - b * p.kvh;
   const int t = r / p.G, head = h * p.G + (r - t * p.G);
-  int len, n;
-  const bool valid = tree_seq(p, b, len, n);
-  if (!valid && h == 0 && r == 0 && lane == 0) atomicExch(p.err, kErrBadCacheLen);
+  const int len = static_cast<int>(base[kTBatch + 2 + b]);
+  const int n = static_cast<int>(base[2 * (kTBatch + 2) + b]);
+  if (h == 0 && r == 0 && lane == 0) {
+    int x, y;
+    if (!tree_seq(p, b, x, y)) atomicExch(p.err, kErrBadCacheLen);
+  }
   float acc[DL], m = -INFINITY, l = 0.0f;
 #pragma unroll
   for (int i = 0; i < DL; ++i) acc[i] = 0.0f;
