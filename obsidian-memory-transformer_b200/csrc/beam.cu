@@ -128,13 +128,14 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 && PER == kPer ? 4 :
   __shared__ uint4 s_slot[kBThreads * NV];  // vectors of the threads that hold candidates
   __shared__ int s_owner[kBThreads];
   __shared__ int s_count, s_slots;
+  grid_wait();
+  grid_release();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / nchunk, chunk = blockIdx.x - row * nchunk;
   const int b = row / W, w = row - b * W;
   const int c0 = chunk * kChunk, c1 = min(V, c0 + kChunk);
   const int64_t item = blockIdx.x;
   uint64_t* list = lists + item * K;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- load: 16-byte vectors of the row's aligned span, all in flight at once; then the
   // vectors that the chunk's ends cut, element by element (-inf where there is none:
@@ -352,6 +353,7 @@ __global__ void __launch_bounds__(kBThreads)
   __shared__ uint32_t s_key[kMergeKeys];
   __shared__ uint32_t s_lim[2 * kBThreads / 32];
   __shared__ int s_count[2];
+  grid_release();
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int nlists = W * nchunk, entries = nlists * K;
   const uint64_t* mine = lists + static_cast<int64_t>(b) * entries;
@@ -360,7 +362,7 @@ __global__ void __launch_bounds__(kBThreads)
     s_score[w] = sc == sc ? sc : -INFINITY;
     s_done[w] = done != nullptr && done[b * W + w] != 0;
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the chunks' kernel has completed
+  grid_wait();  // the chunks' kernel has completed
   const bool all = entries <= kMergeAll;  // few enough to rank as they are
   const uint64_t own = all && tid < entries ? mine[tid] : 0ull;  // in flight with the sums
   __syncthreads();
@@ -576,10 +578,10 @@ extern "C" ltm_status ltm_beam_select(const void* logits, ltm_dtype dtype, int64
     dispatch_dtype(dtype, [&](auto tag) {
       using T = decltype(tag);
       auto go = [&](auto per_c) {
-        beam_chunk_kernel<T, decltype(per_c)::value><<<static_cast<unsigned>(items), kBThreads, 0,
-                                                       st>>>(
-            static_cast<const T*>(logits), batch_stride, beam_stride, scores, done, end_token, W,
-            V, K, nchunk, groups, stats, lists);
+        launch_dependent(beam_chunk_kernel<T, decltype(per_c)::value>,
+                         dim3(static_cast<unsigned>(items)), kBThreads, 0, st,
+                         static_cast<const T*>(logits), batch_stride, beam_stride, scores, done,
+                         end_token, W, V, K, nchunk, groups, stats, lists);
       };
       if constexpr (sizeof(T) == 2) {
         if (per == kPerMany) return go(std::integral_constant<int, kPerMany>{});

@@ -258,9 +258,11 @@ void allow_smem(K kernel, int bytes) {
   allow_smem_of(reinterpret_cast<const void*>(kernel), bytes);
 }
 
-// Launches a kernel that starts by waiting (griddepcontrol.wait) for the kernel
-// before it on the stream: its CTAs may be scheduled once every CTA of that
-// kernel has executed griddepcontrol.launch_dependents or ended.
+// Launches a kernel whose every CTA starts by waiting (grid_wait) for what is before
+// it on the stream: its CTAs may be scheduled once every CTA of the kernel before has
+// called grid_release or ended, which hides the launch (and what it does before the
+// wait: it must not touch memory that earlier kernels write, unless they are
+// complete when the kernel before releases).
 template <class... P, class... A>
 void launch_dependent(void (*kernel)(P...), dim3 grid, int block, size_t smem, cudaStream_t stream,
                       A... args) {
@@ -275,6 +277,13 @@ void launch_dependent(void (*kernel)(P...), dim3 grid, int block, size_t smem, c
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   LTM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+}
+
+__device__ __forceinline__ void grid_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void grid_release() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // ------------------------------------------------------- PTX: sync/timing --

@@ -146,6 +146,8 @@ __global__ void __launch_bounds__(kWarps * 32)
   constexpr int G = D / kVals;        // lanes per row
   constexpr int RP = 32 / G;          // rows per warp and step
   constexpr int TOK = RP * kRowsFly;  // tokens per warp
+  grid_wait();
+  grid_release();
   const int lane = threadIdx.x & 31;
   const int hv = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);  // K heads, then V heads
   if (hv >= 2 * heads) return;
@@ -226,6 +228,8 @@ __global__ void __launch_bounds__(kWarps * 32)
   constexpr int G = D / V;
   constexpr int RP = 32 / G;
   constexpr int ROWS = RP * kReadFly;
+  grid_wait();
+  grid_release();
   const int lane = threadIdx.x & 31;
   const int bh = blockIdx.x;
   const int i0 = (blockIdx.y * kWarps + (threadIdx.x >> 5)) * ROWS;
@@ -305,6 +309,8 @@ __global__ void __launch_bounds__(256)
                          const int* __restrict__ first, const int* __restrict__ lens, int W,
                          int heads, int64_t P, int parts, int* err) {
   __shared__ int src[WMAX];
+  grid_wait();
+  grid_release();
   const int bh = blockIdx.x / parts, part = blockIdx.x % parts;
   const int b = bh / heads, h = bh % heads;
   int mine = threadIdx.x;
@@ -396,10 +402,10 @@ extern "C" ltm_status ltm_kv_cache_append(const void* k, const int64_t* k_stride
       by_head_dim(head_dim, [&](auto d_c) {
         constexpr int D = decltype(d_c)::value;
         auto go = [&](auto q_c) {
-          cache_append_kernel<E, D, decltype(q_c)::value><<<grid, warps * 32, 0, st>>>(
-              static_cast<const E*>(k), sk, static_cast<const E*>(v), sv, k_cache, v_cache,
-              k_scale, v_scale, max_positions, cache_lens, num_tokens, T, kv_heads, tgroups,
-              device_error_ptr());
+          launch_dependent(cache_append_kernel<E, D, decltype(q_c)::value>, grid, warps * 32, 0, st,
+                           static_cast<const E*>(k), sk, static_cast<const E*>(v), sv, k_cache,
+                           v_cache, k_scale, v_scale, max_positions, cache_lens, num_tokens, T,
+                           kv_heads, tgroups, device_error_ptr());
         };
         if constexpr (std::is_same<E, float>::value) {
           go(std::true_type{});
@@ -437,9 +443,9 @@ extern "C" ltm_status ltm_kv_cache_read(const void* cache, const float* scale, l
       by_head_dim(head_dim, [&](auto d_c) {
         constexpr int D = decltype(d_c)::value;
         auto go = [&](auto q_c) {
-          cache_read_kernel<O, D, decltype(q_c)::value><<<grid, kWarps * 32, 0, st>>>(
-              cache, scale, max_positions, first, cache_lens, kv_heads, n,
-              static_cast<O*>(out));
+          launch_dependent(cache_read_kernel<O, D, decltype(q_c)::value>, grid, kWarps * 32, 0, st,
+                           cache, scale, max_positions, first, cache_lens, kv_heads, n,
+                           static_cast<O*>(out));
         };
         if constexpr (std::is_same<O, float>::value) {
           go(std::true_type{});
@@ -494,9 +500,9 @@ extern "C" ltm_status ltm_kv_cache_reorder(void* const* caches, const int64_t* r
       LTM_REQUIRE(gx < (1ll << 31), "too many heads");
       const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(n));
       auto go = [&](auto w_c) {
-        cache_reorder_kernel<decltype(w_c)::value><<<grid, 256, 0, st>>>(
-            p, beams, first, cache_lens, W, kv_heads, max_positions, static_cast<int>(nx),
-            device_error_ptr());
+        launch_dependent(cache_reorder_kernel<decltype(w_c)::value>, grid, 256, 0, st, p, beams,
+                         first, cache_lens, W, kv_heads, max_positions, static_cast<int>(nx),
+                         device_error_ptr());
       };
       if (W <= 4) go(std::integral_constant<int, 4>{});
       else if (W <= 8) go(std::integral_constant<int, 8>{});

@@ -307,9 +307,6 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return *reinterpret_cast<uint32_t*>(&h);
   }
 }
-__device__ __forceinline__ void launch_dependents() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
 template <int THREADS>
 __device__ __forceinline__ void cons_sync() {
   asm volatile("barrier.cta.sync 1, %0;" ::"n"(THREADS) : "memory");
@@ -387,9 +384,10 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
+  grid_wait();
   if (warp == 0) tree_scan(p, base, lane);
   __syncthreads();
-  launch_dependents();
+  grid_release();
   const uint32_t total = base[p.B];
   const uint32_t shares = min(total, gridDim.x);
   if (blockIdx.x >= shares) return;
@@ -880,11 +878,12 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
     __syncwarp();
     tmem_alloc(tslot, kCols);
   }
+  grid_wait();
   if (warp == 0) tree_scan(p, base, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  launch_dependents();
+  grid_release();
   const uint32_t tmem = *tslot, tO = tmem + 2 * N;
   const uint32_t total = base[p.B];
   const uint32_t shares = min(total, gridDim.x);
@@ -1264,13 +1263,17 @@ __global__ void __launch_bounds__(32 * kCWarps) tree_combine_kernel(const TreePa
   constexpr int DL = D / 32;
   __shared__ uint32_t base[kScanWords];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  grid_release();
   if (warp == 0) tree_scan(p, base, lane);
   __syncthreads();
   const uint32_t total = base[p.B];
   const uint32_t shares = min(total, static_cast<uint32_t>(p.grid));
   const int R = p.G * p.T;
   const int row = blockIdx.x * kCWarps + warp;
-  if (row >= p.B * p.kvh * R) return;
+  if (row >= p.B * p.kvh * R) {
+    grid_wait();
+    return;
+  }
   const int bh = row / R, r = row - bh * R;
   const int b = bh / p.kvh, h = bh - b * p.kvh;
   const int t = r / p.G, head = h * p.G + (r - t * p.G);
@@ -1283,7 +1286,7 @@ __global__ void __launch_bounds__(32 * kCWarps) tree_combine_kernel(const TreePa
   float acc[DL], m = -INFINITY, l = 0.0f;
 #pragma unroll
   for (int i = 0; i < DL; ++i) acc[i] = 0.0f;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the partials are complete
+  grid_wait();  // the partials are complete
   if (t < n) {
     const int rb = r / p.rb, tiles = tiles_of(p, len, n), nrb = row_blocks(p, n);
     const uint32_t t0 = base[b] + (static_cast<uint32_t>(h) * nrb + rb) * tiles;
@@ -1375,7 +1378,8 @@ void launch_mma(TreeParams p, cudaStream_t st) {
   make_tma_2d(&tv, p.vc, dt, Q8 ? 1 : 2, rows, D, D, S::kBox / (Q8 ? 1 : 2), S::kKeys, sw);
   auto kern = tree_mma_kernel<T, D, Q8, NR>;
   allow_smem(kern, S::kBytes);
-  kern<<<p.grid, 32 * (S::kWarps + 1), S::kBytes, st>>>(tk, tv, p);
+  launch_dependent(kern, dim3(static_cast<unsigned>(p.grid)), 32 * (S::kWarps + 1), S::kBytes, st,
+                   tk, tv, p);
   check_launch("tree_mma_kernel", st);
   launch_combine<T, D>(p, st);
 }
@@ -1390,7 +1394,8 @@ void launch_tc(TreeParams p, cudaStream_t st) {
   make_tma_2d(&tv, p.vc, tma_dtype_of<T>(), 2, rows, D, D, 64, kTcTile);
   auto kern = tree_tc_kernel<T, D, N>;
   allow_smem(kern, S::kBytes);
-  kern<<<p.grid, 128 + 128 * S::kGroups, S::kBytes, st>>>(tk, tv, p);
+  launch_dependent(kern, dim3(static_cast<unsigned>(p.grid)), 128 + 128 * S::kGroups, S::kBytes,
+                   st, tk, tv, p);
   check_launch("tree_tc_kernel", st);
   launch_combine<T, D>(p, st);
 }
