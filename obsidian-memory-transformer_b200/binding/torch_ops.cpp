@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -101,6 +102,24 @@ class Call {
     return t;
   }
   void* stream() const { return static_cast<void*>(raw_); }
+  // Workspace of the allocator's, given back to the call's stream when the launches are
+  // queued.
+  class Workspace {
+   public:
+    Workspace(size_t bytes, cudaStream_t stream)
+        : p_(bytes ? c10::cuda::CUDACachingAllocator::raw_alloc_with_stream(bytes, stream)
+                   : nullptr) {}
+    ~Workspace() {
+      if (p_ != nullptr) c10::cuda::CUDACachingAllocator::raw_delete(p_);
+    }
+    Workspace(const Workspace&) = delete;
+    Workspace& operator=(const Workspace&) = delete;
+    void* get() const { return p_; }
+
+   private:
+    void* p_;
+  };
+  Workspace workspace(size_t bytes) const { return Workspace(bytes, raw_); }
 
  private:
   c10::Device device_;
@@ -262,12 +281,12 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                       size32(d), &bytes));
     Call c(q, a[9]);
     const at::Tensor out = given ? *given : c.empty(q.sizes(), q.scalar_type());
-    const at::Tensor ws = c.empty({static_cast<int64_t>(bytes)}, at::kByte);
+    const Call::Workspace ws = c.workspace(bytes);
     done(ltm_tree_attention(q.data_ptr(), sq, kc.data_ptr(), vc.data_ptr(), ptr_as<float>(ks),
                             ptr_as<float>(vs), kc.size(2), ptr_as<int32_t>(&lens),
                             ptr_as<int32_t>(num), ptr_as<int32_t>(parents), out.data_ptr(),
                             rows_strides(out, "out"), size32(B), size32(T), size32(heads),
-                            size32(kc.size(1)), size32(d), dt, ws.data_ptr(), bytes, c.stream()));
+                            size32(kc.size(1)), size32(d), dt, ws.get(), bytes, c.stream()));
     return given ? Py_NewRef(a[8]) : THPVariable_Wrap(out);
   });
 }
@@ -297,12 +316,12 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor tokens = c.empty({B, K}, at::kInt);
     at::Tensor out_fin;
     if (fin != nullptr) out_fin = c.empty({B, K}, at::kBool);
-    const at::Tensor ws = c.empty({static_cast<int64_t>(bytes)}, at::kByte);
+    const Call::Workspace ws = c.workspace(bytes);
     done(ltm_beam_select(logits.data_ptr(), dt, logits.stride(0), logits.stride(1),
                          ptr_as<float>(&scores), ptr_as<uint8_t>(fin), end, size32(B), size32(W),
                          size32(V), K, ptr_as<float>(&best), ptr_as<int32_t>(&beams),
                          ptr_as<int32_t>(&tokens), fin ? ptr_as<uint8_t>(&out_fin) : nullptr,
-                         ws.data_ptr(), bytes, c.stream()));
+                         ws.get(), bytes, c.stream()));
     PyObject* r = PyTuple_New(fin ? 4 : 3);
     if (r == nullptr) throw Refused{};
     PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(best));
