@@ -19,7 +19,7 @@
 //
 // Two kernels contract the tiles, by the rows G * T that share a cached head:
 //
-// * tree_mma_kernel, up to 16 rows (and int8 caches): warp 0 streams K and V
+// * tree_mma_kernel, up to 16 rows: warp 0 streams K and V
 //   tiles by TMA into a ring of swizzled slots; the consumer warps contract them on
 //   mma.sync m16n8k16 with the keys as M (a decode step's few rows are the 8 or 16
 //   columns; a 128-row tcgen05 tile would idle).  A warp takes 16 keys at a time
@@ -32,11 +32,20 @@
 //   thread) and 11 beyond (168), 16-bit ones 8.  A tile is 16 keys for every warp:
 //   each warp waits for every load in turn (a warp that skipped tiles could take a
 //   barrier's phase for the one before).
-// * tree_tc_kernel, more rows of a 16-bit cache: tcgen05, keys as the 128 lanes:
-//   S^T [128 keys x N rows] = K Q^T and O^T [D x N] += V^T P, N = 32, 64 or 128 rows.
-//   K and V tiles are used as they lie (K-major and M-major operands), the
-//   softmax work grows with the rows, and a thread owns a key: its mask test and
-//   the clean-up of rows past the end are its own.
+// * tree_tc_kernel, more rows: tcgen05, keys as the 128 lanes:
+//   S^T [128 keys x N rows] = K Q^T and O^T [D x N] += V^T P, N = 32, 64 or (16-bit
+//   caches) 128 rows.  K and V tiles are used as they lie (K-major and M-major
+//   operands), the softmax work grows with the rows, and a thread owns a key: its mask
+//   test, its scales and the clean-up of rows past the end are its own.  int8 codes
+//   become f16 tiles in shared memory first.
+//
+// Measured, cold caches, contexts of equal length.  Read-bound: 16-bit, one row per
+// head of 128 dims, 32 x 8 heads x 16384 positions 0.46 ms (7.0 TB/s); int8, one row,
+// 0.52 ms for 3.2 GB (6.4 TB/s; 5.5 TB/s once the clock has dropped under load).  int8
+// conversions bound 9 to 16 rows (4.1 TB/s, 128 dims; tcgen05's blocks of 32 rows reach
+// 2.7).  tree_tc_kernel is bound by its softmax: 1.0, 1.2 and 2.05 us per tile of 128
+// positions with 32, 64 and 128 rows of 64 dims (int8: 1.25 and 1.66; 128 dims 1.8 and
+// 2.45), where reading a 16-bit tile takes 0.7 us of 64 dims, 1.4 of 128.
 //
 // In both, a row's reference maximum is only raised when a score exceeds it by more
 // than 2^8.  A non-finite value of a drafted token must not
@@ -768,8 +777,10 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
 // ------------------------------------------------------------ tcgen05 kernel --
 // Shared memory: Q [N rows x D] (K-major), P [128 keys x N] (N contiguous; twice up to 64
 // rows, so that P(j + 1) is written while P(j) is contracted), a ring
-// of 128-position K and V tiles, all in 128-byte-swizzled chunks of 64 columns.
-template <int D, int N>
+// of 128-position K and V tiles, all in 128-byte-swizzled chunks of 64 columns.  int8
+// caches: two or four warps fill that ring from a ring of code tiles.
+
+template <int D, int N, bool Q8>
 struct TcSmem {
   static constexpr int kTile = kTcTile * D * 2;        // K or V tile
   static constexpr int kQChunk = N * 128;             // N rows x 64 dims
@@ -780,19 +791,29 @@ struct TcSmem {
   static constexpr int kP = kPs * kPOne;
   static constexpr int kOffP = kQ;
   static constexpr int kOffRing = kOffP + kP;
-  static constexpr int kLeft = 217 * 1024 - kOffRing;
-  static constexpr int kSlots = kLeft / kTile > 8 ? 8 : kLeft / kTile;
-  static constexpr int kOffMax = kOffRing + kSlots * kTile;  // [4][N] maxima / sums
-  static constexpr int kOffRef = kOffMax + 4 * N * 4;        // [N] -reference, [N] factor
-  static constexpr int kOffMask = kOffRef + 2 * N * 4;       // [softmax warps][rows] ancestor sets
+  static constexpr int kLeft = 214 * 1024 - kOffRing;
+  static constexpr int kFit = kLeft / kTile;
+  static constexpr int kSlots = Q8 ? (D == 64 ? 6 : 3) : kFit > 8 ? 8 : kFit;
+  static constexpr int kCodes = Q8 ? kTcTile * D : 0;        // K or V tile of codes
+  static constexpr int kSlots8 = !Q8 ? 0 : D == 64 ? 8 : 4;
+  static constexpr int kOffCodes = kOffRing + kSlots * kTile;
+  static_assert(kSlots * kTile + kSlots8 * kCodes <= kLeft && kSlots >= 3, "ring");
+  static constexpr int kOffMax = kOffCodes + kSlots8 * kCodes;  // [2][4][N] maxima / sums
+  static constexpr int kOffRef = kOffMax + 8 * N * 4;        // [6][N] per row, see the kernel
+  static constexpr int kOffMask = kOffRef + 6 * N * 4;       // [softmax warps][rows] ancestor sets
   static constexpr int kOffBase = kOffMask + 4 * N * 8;
   static constexpr int kOffBar = (kOffBase + kScanWords * 4 + 7) / 8 * 8;
-  static constexpr int kBars = 2 * kSlots + 10;
+  static constexpr int kBars = 2 * kSlots + 2 * kSlots8 + 10;
   static constexpr int kOffFlag = kOffBar + kBars * 8;
-  static constexpr int kBytes = kOffFlag + 48 + 1024;
   // softmax: groups of four warps, each with 32 rows, or with 64 of 128 (four groups would
   // leave 96 registers a thread: 2.1 -> 3.0 us a tile)
   static constexpr int kRows = N <= 64 ? 32 : 64, kGroups = N / kRows;
+  // int8: warps 2, 3 convert, and two more, but not with 64 rows of 64 dims: the 13th warp
+  // costs the softmax registers (168 -> 128; 2.26 us a tile against 1.66), which 128 dims,
+  // bound by the conversion, are worth (2.44 us against 2.84)
+  static constexpr int kConv = N == 64 && D == 64 ? 2 : 4;
+  static constexpr int kThreads = 128 + 128 * kGroups + (Q8 ? 32 * (kConv - 2) : 0);
+  static constexpr int kBytes = kOffFlag + 48 + 1024;
   static_assert(kBytes <= 232448, "shared memory of one CTA");
 };
 
@@ -833,22 +854,31 @@ __device__ __forceinline__ void soft_sync() {
 // warp 0: TMA producer (K(0), V(0), K(1), ... into the ring); warp 1: TMEM and
 // the MMAs, in the order S(0), S(1), O(0), S(2), O(1), ... within a head's
 // segment; warps 4-7 (and 8-11 for the upper half of 64 or 128 rows): softmax,
-// thread = key = TMEM lane.  TMEM: S^T twice, O^T.  The softmax reads its rows of S
-// twice, 32 at a time (for the vote, then for the exponentials), instead of holding them.
-template <class T, int D, int N>
-__global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
+// thread = key = TMEM lane.  TMEM: S^T twice, O^T.  With 128 rows the softmax reads its
+// 64 rows of S twice, 32 at a time (for the vote, then for the exponentials).  int8
+// caches: warps 2, 3 (and the last two) turn the codes into f16 tiles (exact); a thread's key
+// has its K scale on the scores and its V scale on the probabilities, as in tree_mma_kernel.
+template <class T, int D, int N, bool Q8>
+__global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const TreeParams p) {
-  using S = TcSmem<D, N>;
-  constexpr int NS = S::kSlots;
+  using S = TcSmem<D, N, Q8>;
+  constexpr int NS = S::kSlots, N8 = S::kSlots8;
+  static_assert(!Q8 || S::kRows == 32, "int8: 32 rows a softmax group");
   constexpr int RW = S::kRows, NC = RW / 32, kSoft = 128 * S::kGroups, PB = S::kPs;
   constexpr uint32_t kCols = N <= 32 ? 128 : N <= 64 ? 256 : 512;  // 3 N columns
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   float* smax = reinterpret_cast<float*>(smem + S::kOffMax);
-  float* nref = reinterpret_cast<float*>(smem + S::kOffRef);  // -reference (0: none yet)
+  // per row: -reference (0: none yet), the rescaling of the sums; int8: the scores'
+  // factor, the reference with the V scale, the rescaling of O, 2^(reference - that one)
+  float* nref = reinterpret_cast<float*>(smem + S::kOffRef);
   float* fact = nref + N;
+  float* srow = fact + N;
+  float* eref = srow + N;
+  float* facto = eref + N;
+  float* frow = facto + N;
   uint32_t* base = reinterpret_cast<uint32_t*>(smem + S::kOffBase);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kOffBar);
   uint64_t* empty = full + NS;
@@ -858,6 +888,8 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
   uint64_t* p_full = s_free + 2;  // [2], as is pv_done: by P buffer
   uint64_t* pv_done = p_full + 2;
   uint64_t* drained = pv_done + 2;
+  uint64_t* full8 = drained + 1;  // the ring of code tiles
+  uint64_t* empty8 = full8 + N8;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kOffFlag);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + S::kOffFlag) + 1;
   int* wait_ok = reinterpret_cast<int*>(tslot) + 1;  // [softmax warps]
@@ -867,7 +899,8 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
     for (int i = 0; i < S::kBars; ++i) {
       const bool per_warp = full + i == q_full || full + i == s_free || full + i == s_free + 1 ||
                             full + i == p_full || full + i == p_full + 1;
-      mbar_init(full + i, per_warp ? kSoft / 32 : 1);
+      const bool conv = Q8 && (i < NS || (full + i >= empty8 && full + i < empty8 + N8));
+      mbar_init(full + i, per_warp ? kSoft / 32 : conv ? S::kConv : 1);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -895,6 +928,11 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
 
   if (warp == 0) {
     if (lane == 0) {
+      // into the ring of tiles, or of code tiles
+      constexpr int NP = Q8 ? N8 : NS, kBytes = Q8 ? S::kCodes : S::kTile;
+      constexpr int kBoxes = Q8 ? 1 : D / 64;
+      uint64_t* pfull = Q8 ? full8 : full;
+      uint64_t* pempty = Q8 ? empty8 : empty;
       int it = 0;  // ring slots used
       bool ok = true;
       for (uint32_t w = w0; ok && w < w1;) {
@@ -903,17 +941,17 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
         const int row = static_cast<int>((static_cast<int64_t>(s.b) * p.kvh + s.h) * p.P) +
                         s.tile * kTcTile;
         for (int t = 0; ok && t < 2 * nt; ++t) {
-          const int st = it % NS;
-          if (!mbar_wait_bounded(empty + st, ((it / NS) & 1) ^ 1, abort_flag, p.err,
+          const int st = it % NP;
+          if (!mbar_wait_bounded(pempty + st, ((it / NP) & 1) ^ 1, abort_flag, p.err,
                                  kErrWaitEmpty)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(full + st, S::kTile);
-          uint8_t* dst = smem + S::kOffRing + st * S::kTile;
+          mbar_arrive_expect_tx(pfull + st, kBytes);
+          uint8_t* dst = smem + (Q8 ? S::kOffCodes : S::kOffRing) + st * kBytes;
 #pragma unroll
-          for (int x = 0; x < D / 64; ++x)
-            tma_load_2d(dst + x * kTcTile * 128, (t & 1) ? &tmV : &tmK, full + st, x * 64,
+          for (int x = 0; x < kBoxes; ++x)
+            tma_load_2d(dst + x * kTcTile * 128, (t & 1) ? &tmV : &tmK, pfull + st, x * 64,
                         row + (t >> 1) * kTcTile);
           ++it;
         }
@@ -921,13 +959,13 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
       }
       if (!ok) {  // let the copies in flight land before the CTA exits
         volatile int never = 0;
-        for (int j = (it > NS ? it - NS : 0); j < it; ++j)
-          mbar_wait_bounded(full + j % NS, (j / NS) & 1, &never, p.err, kErrWaitOther);
+        for (int j = (it > NP ? it - NP : 0); j < it; ++j)
+          mbar_wait_bounded(pfull + j % NP, (j / NP) & 1, &never, p.err, kErrWaitOther);
       }
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr bool kBF = std::is_same<T, __nv_bfloat16>::value;
+      constexpr bool kBF = std::is_same<T, __nv_bfloat16>::value && !Q8;
       constexpr uint32_t idS = idesc_f16(128, N, kBF);
       // A = V^T: M (dims) contiguous; B = P: N (rows) contiguous
       constexpr uint32_t idO = idesc_f16(128, N, kBF, true) | (1u << 15);
@@ -989,7 +1027,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
         mbar_wait_bounded(drained, 0, &never, p.err, kErrWaitOther);
       }
     }
-  } else if (warp >= 4) {
+  } else if (warp >= 4 && warp < 4 + kSoft / 32) {
     // ---- softmax: key `kt` of every tile, rows r0 .. r0 + RW
     const int sw = warp - 4, q4 = warp & 3, kt = q4 * 32 + lane, tid = threadIdx.x - 128;
     const int r0 = (sw >> 2) * RW;
@@ -1027,6 +1065,26 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
           v[i] = r < sp.rows ? __ldg(reinterpret_cast<const uint4*>(qp) + x)
                              : make_uint4(0, 0, 0, 0);
         }
+        if constexpr (Q8) {
+          // f16, each row scaled by a power of two (undone by srow); the row's U units
+          // lie in U neighbouring lanes
+#pragma unroll
+          for (int i = 0; i < NQ; ++i) {
+            const T* e = reinterpret_cast<const T*>(&v[i]);
+            float am = 0.0f;
+#pragma unroll
+            for (int y = 0; y < 8; ++y) am = fmaxf(am, fabsf(to_f32(e[y])));
+#pragma unroll
+            for (int o = 1; o < U; o <<= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+            const float qs = query_scale(am);
+            uint32_t f[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              f[y] = pack16<false>(to_f32(e[2 * y]) * qs, to_f32(e[2 * y + 1]) * qs);
+            v[i] = make_uint4(f[0], f[1], f[2], f[3]);
+            if ((tid + i * kSoft) % U == 0) srow[(tid + i * kSoft) / U] = p.sl2 / qs;
+          }
+        }
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
           const int r = (tid + i * kSoft) / U, x = (tid + i * kSoft) % U;
@@ -1040,6 +1098,18 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
       float l[RW];
 #pragma unroll
       for (int i = 0; i < RW; ++i) l[i] = 0.0f;
+      // the scales of this thread's key, loaded two tiles ahead
+      float ks_next[2], vs_next[2];
+      auto load_scales = [&](int t, int slot) {
+        const int key = (sp.tile + t) * kTcTile + kt;
+        const bool in = key < sp.len + sp.n;
+        ks_next[slot] = in ? __ldg(p.ks + head * p.P + key) : 0.0f;
+        vs_next[slot] = in ? __ldg(p.vs + head * p.P + key) : 0.0f;
+      };
+      if constexpr (Q8) {
+        load_scales(0, 0);
+        load_scales(1, 1);
+      }
 
       for (int t = 0; t < nt; ++t, ++it) {
         const int at = (sp.tile + t) * kTcTile + kt - sp.len;  // this key's place in the draft
@@ -1053,11 +1123,32 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
 #pragma unroll 8
             for (int i = 0; i < RW; ++i) seen |= (mask[i] >> at & 1ull) << i;
         }
+        float ksc = 1.0f, vsc = 1.0f, lvs = 0.0f;
+        if constexpr (Q8) {
+          ksc = ks_next[0];
+          asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lvs) : "f"(vs_next[0]));
+          vsc = fminf(vs_next[0], 3.0e38f);
+          ks_next[0] = ks_next[1];
+          vs_next[0] = vs_next[1];
+          load_scales(t + 2, 1);
+        }
         bool got = wait_warp(s_full + (it & 1), (it >> 1) & 1);
         tc_fence_after();
         auto scores = [&](int c, uint32_t (&s)[32]) {
           tmem_ld_32x32b_x32(tmem + (it & 1) * N + lane_off + r0 + c * 32, s);
           tmem_wait_ld_tie(s);
+          if constexpr (Q8) {  // the row's factor, then the key's (last where nothing is masked)
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 y = *reinterpret_cast<const float4*>(srow + r0 + c * 32 + i);
+              const float y4[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                s[i + x] = __float_as_uint(__uint_as_float(s[i + x]) * y4[x]);
+                if (tail) s[i + x] = __float_as_uint(__uint_as_float(s[i + x]) * ksc);
+              }
+            }
+          }
           if (tail) {
             const uint32_t bits = static_cast<uint32_t>(seen >> (32 * c));
 #pragma unroll
@@ -1065,7 +1156,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
               if (!(bits >> i & 1u)) s[i] = __float_as_uint(-INFINITY);
           }
         };  // scores of 32 rows
-        if (tail && got && sw < 4) {  // this thread's V row, once it has landed
+        if (!Q8 && tail && got && sw < 4) {  // this thread's V row, once it has landed
           const int slot = 2 * it + 1;
           got = wait_warp(full + slot % NS, (slot / NS) & 1);
           if (got && at >= 0) {
@@ -1078,6 +1169,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
         }
         // ---- does a score pass its row's reference by more than the margin?  With 32 rows
         // the exponentials are taken at once and looked at afterwards
+        const float unit = !Q8 ? p.sl2 : tail ? 1.0f : ksc;  // scores to log2 units
         auto expo = [&](uint32_t (&x)[32], int c) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
@@ -1085,12 +1177,33 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
             const float n4[4] = {nr.x, nr.y, nr.z, nr.w};
 #pragma unroll
             for (int y = 0; y < 4; ++y)
-              x[i + y] = __float_as_uint(
-                  ex2_approx(fmaf(__uint_as_float(x[i + y]), p.sl2, n4[y])));
+              x[i + y] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(x[i + y]), unit, n4[y])));
           }
         };
+        // int8: p * v's scale goes into P, against its own reference: at most 2^8
+        // (a scale NaN counts as 3e38 and becomes an infinity in P)
+        uint32_t pk[16];
+        auto weigh = [&](const uint32_t (&x)[32]) -> float {
+          float top = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 y = *reinterpret_cast<const float4*>(frow + r0 + i);
+            const float y4[4] = {y.x, y.y, y.z, y.w};
+            float z[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              z[j] = __uint_as_float(x[i + j]) * y4[j] * vsc;
+              top = fmaxf(top, z[j]);
+            }
+            pk[i / 2] = pack16<false>(z[0], z[1]);
+            pk[i / 2 + 1] = pack16<false>(z[2], z[3]);
+          }
+          return top;
+        };
         uint32_t e[32];  // NC == 1: the tile's exponentials
-        bool need = first || !got;
+        // int8: always where drafted keys are, so that no row's result hangs on the scales of
+        // keys that it does not see
+        bool need = first || !got || (Q8 && tail);
         if (!need) {
           float top = -INFINITY;
           if constexpr (NC == 1) {
@@ -1098,6 +1211,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
             expo(e, 0);
 #pragma unroll
             for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(e[i]));
+            if constexpr (Q8) top = fmaxf(top, weigh(e));
             need = top > kTMost;
           } else {
 #pragma unroll
@@ -1124,7 +1238,13 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
               scores(c, s);
               float v[32];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(s[i]);
+              for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(s[i]) * unit;
+              if constexpr (Q8) {
+                float x[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x[i] = v[i] + lvs;
+                smax[(4 + q4) * N + r0 + c * 32 + lane] = across_lanes<false>(x, lane);
+              }
               smax[q4 * N + r0 + c * 32 + lane] = across_lanes<false>(v, lane);
             }
           }
@@ -1139,12 +1259,21 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
           }
           if (tid < N) {
             const float top = fmaxf(fmaxf(smax[tid], smax[N + tid]),
-                                    fmaxf(smax[2 * N + tid], smax[3 * N + tid])) * p.sl2;
+                                    fmaxf(smax[2 * N + tid], smax[3 * N + tid]));
             const float old = first ? -INFINITY : -nref[tid];
             const float now = fmaxf(old, top);
             // a row without a score above -inf keeps 0: its probabilities are 0 (or NaN)
             nref[tid] = now == -INFINITY ? 0.0f : -now;
             fact[tid] = first ? 0.0f : ex2_approx(old - now);
+            if constexpr (Q8) {
+              const float* m = smax + 4 * N + tid;
+              const float old_e = first ? -INFINITY : eref[tid];
+              const float now_e = fmaxf(old_e, fmaxf(fmaxf(m[0], m[N]), fmaxf(m[2 * N], m[3 * N])));
+              eref[tid] = now_e;
+              facto[tid] = old_e == -INFINITY ? 0.0f : ex2_approx(old_e - now_e);
+              // capped: p, at most 2^8, times it stays finite
+              frow[tid] = now_e == -INFINITY ? 0.0f : ex2_approx(fminf(now - now_e, 119.0f));
+            }
           }
           soft_sync<kSoft>();
           // O is final up to the tile before; rescale it and the sums (where the wait
@@ -1159,7 +1288,8 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
                 const float f = fact[r0 + c * 32 + i];
-                ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
+                const float fo = Q8 ? facto[r0 + c * 32 + i] : f;
+                ov[i] = __float_as_uint(__uint_as_float(ov[i]) * fo);
                 l[c * 32 + i] *= f;
               }
               tmem_st_32x32b_x32(tO + lane_off + r0 + c * 32, ov);
@@ -1169,12 +1299,12 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
           if constexpr (NC == 1) {
             scores(0, e);
             expo(e, 0);
+            if constexpr (Q8) weigh(e);
           }
         }
         // ---- probabilities, their sums, and P (16 bits, this key's row)
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          uint32_t pk[16];
           if constexpr (NC > 1) scores(c, e);
           if (c == NC - 1) {
             tc_fence_before();
@@ -1187,7 +1317,7 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
             const float a = __uint_as_float(e[i]), b = __uint_as_float(e[i + 1]);
             l[c * 32 + i] += a;
             l[c * 32 + i + 1] += b;
-            pk[i / 2] = pack16<std::is_same<T, __nv_bfloat16>::value>(a, b);
+            if constexpr (!Q8) pk[i / 2] = pack16<std::is_same<T, __nv_bfloat16>::value>(a, b);
           }
           // this P buffer is free once the tile that was in it has been contracted
           if (c == 0 && it >= PB) wait_pv(it - PB);
@@ -1213,6 +1343,9 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
         for (int i = 0; i < 32; ++i) v[i] = l[c * 32 + i];
         smax[q4 * N + r0 + c * 32 + lane] = across_lanes<true>(v, lane);
       }
+      if constexpr (Q8) {  // O back to the scores' own reference
+        if (tid < N) smax[4 * N + tid] = eref[tid] == -INFINITY ? 0.0f : ex2_approx(eref[tid] + nref[tid]);
+      }
       const bool any_taken = soft_any<kSoft>(taken);
       ok = wait_pv(it - 1);
       if (ok) {
@@ -1235,7 +1368,8 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (r0 + c * 32 + i < sp.rows)
-                pp[(r0 + c * 32 + i) * part_stride<D>() + kt] = __uint_as_float(ov[i]);
+                pp[(r0 + c * 32 + i) * part_stride<D>() + kt] =
+                    __uint_as_float(ov[i]) * (Q8 ? smax[4 * N + r0 + c * 32 + i] : 1.0f);
           }
         }
         tc_fence_before();
@@ -1243,6 +1377,54 @@ __global__ void __launch_bounds__(128 + 128 * TcSmem<D, N>::kGroups, 1)
       // nref, smax and O are used again by the next segment only after this
       if (soft_any<kSoft>(!ok)) ok = false;
       w += nt;
+    }
+  } else if constexpr (Q8) {
+    // ---- codes to f16 tiles
+    const int ct = (warp < 4 ? warp - 2 : warp - 2 - kSoft / 32) * 32 + lane;
+    constexpr int U = D / 16, NU = kTcTile * U / (32 * S::kConv);  // 16-code units per row / thread
+    const int nloads = 2 * static_cast<int>(w1 - w0);
+    auto wait_conv = [&](uint64_t* bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu,
+                        mbar_wait_bounded(bar, parity, abort_flag, p.err, kErrWaitOther));
+    };
+    for (int it = 0; it < nloads; ++it) {
+      const int s8 = it % N8, st = it % NS;
+      if (!wait_conv(full8 + s8, (it / N8) & 1)) break;
+      const uint8_t* src = smem + S::kOffCodes + s8 * S::kCodes;
+      uint4 x[NU];
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        const int u = ct + i * 32 * S::kConv, key = u / U, c = u % U;
+        const int at = D == 128 ? key * 128 + ((c ^ (key & 7)) << 4)
+                                : key * 64 + ((c ^ ((key >> 1) & 3)) << 4);
+        x[i] = *reinterpret_cast<const uint4*>(src + at);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty8 + s8);
+      if (!wait_conv(empty + st, ((it / NS) & 1) ^ 1)) break;
+      uint8_t* dst = smem + S::kOffRing + st * S::kTile;
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        const int u = ct + i * 32 * S::kConv, key = u / U, c = u % U;
+        const uint32_t wd[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        uint32_t f[8];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const uint32_t z = wd[y] ^ 0x80808080u;
+          f[2 * y] = codes_f16(z, 0x4140);
+          f[2 * y + 1] = codes_f16(z, 0x4342);
+        }
+        // the upper chunk's units in the other order: no bank conflicts between the chunks
+        const bool swap = (c >> 2) & 1;
+        uint8_t* row = dst + (c >> 2) * kTcTile * 128 + key * 128;
+        const int w0u = ((c & 3) * 2 + swap) ^ (key & 7), w1u = ((c & 3) * 2 + !swap) ^ (key & 7);
+        const uint4 lo = make_uint4(f[0], f[1], f[2], f[3]), hi = make_uint4(f[4], f[5], f[6], f[7]);
+        *reinterpret_cast<uint4*>(row + (w0u << 4)) = swap ? hi : lo;
+        *reinterpret_cast<uint4*>(row + (w1u << 4)) = swap ? lo : hi;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full + st);
     }
   }
 
@@ -1332,13 +1514,15 @@ __global__ void __launch_bounds__(32 * kCWarps) tree_combine_kernel(const TreePa
 }
 
 // ---------------------------------------------------------------- launchers --
-// Rows of a block.  Up to 16 rows go to mma.sync in one block, int8 caches in blocks of 16.  More rows of a 16-bit cache go
-// to tcgen05 in the smallest block that holds them (at most 128).
+// Rows of a block.  Up to 16 rows go to mma.sync; more to tcgen05, in the smallest block
+// that holds them, of at most 128 rows (64 for int8 caches).  17 int8 rows of 128 dims, 8 x
+// 32 heads x 16384 positions: 0.40 ms in one block, about 0.52 in two of mma.sync; 12 rows
+// 0.26 ms on mma.sync, 0.40 on tcgen05.
 int block_rows(int rows, bool q8) {
   if (rows <= 8) return 8;
-  if (rows <= kMRows || q8) return kMRows;
+  if (rows <= kMRows) return kMRows;
   if (rows <= 32) return 32;
-  return rows <= 64 ? 64 : 128;
+  return rows <= 64 || q8 ? 64 : 128;
 }
 
 size_t tree_slots(int B, int T, int G, int kvh, int grid, int rb, int& nrb) {
@@ -1384,18 +1568,21 @@ void launch_mma(TreeParams p, cudaStream_t st) {
   launch_combine<T, D>(p, st);
 }
 
-template <class T, int D, int N>
+template <class T, int D, int N, bool Q8>
 void launch_tc(TreeParams p, cudaStream_t st) {
-  using S = TcSmem<D, N>;
+  using S = TcSmem<D, N, Q8>;
   set_tiles(p, kTcTile);
   const uint64_t rows = static_cast<uint64_t>(p.B) * p.kvh * p.P;
   CUtensorMap tk, tv;
-  make_tma_2d(&tk, p.kc, tma_dtype_of<T>(), 2, rows, D, D, 64, kTcTile);
-  make_tma_2d(&tv, p.vc, tma_dtype_of<T>(), 2, rows, D, D, 64, kTcTile);
-  auto kern = tree_tc_kernel<T, D, N>;
+  const CUtensorMapDataType dt = Q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : tma_dtype_of<T>();
+  const CUtensorMapSwizzle sw =
+      Q8 && D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  make_tma_2d(&tk, p.kc, dt, Q8 ? 1 : 2, rows, D, D, Q8 ? D : 64, kTcTile, sw);
+  make_tma_2d(&tv, p.vc, dt, Q8 ? 1 : 2, rows, D, D, Q8 ? D : 64, kTcTile, sw);
+  auto kern = tree_tc_kernel<T, D, N, Q8>;
   allow_smem(kern, S::kBytes);
-  launch_dependent(kern, dim3(static_cast<unsigned>(p.grid)), 128 + 128 * S::kGroups, S::kBytes,
-                   st, tk, tv, p);
+  launch_dependent(kern, dim3(static_cast<unsigned>(p.grid)), S::kThreads, S::kBytes, st, tk, tv,
+                   p);
   check_launch("tree_tc_kernel", st);
   launch_combine<T, D>(p, st);
 }
@@ -1500,10 +1687,12 @@ extern "C" ltm_status ltm_tree_attention(
           launch_mma<E, D, Q, 1>(p, st);
         } else if (rb == kMRows) {
           launch_mma<E, D, Q, 2>(p, st);
+        } else if (rb == 32) {
+          launch_tc<E, D, 32, Q>(p, st);
+        } else if (rb == 64) {
+          launch_tc<E, D, 64, Q>(p, st);
         } else if constexpr (!Q) {
-          if (rb == 32) launch_tc<E, D, 32>(p, st);
-          else if (rb == 64) launch_tc<E, D, 64>(p, st);
-          else launch_tc<E, D, 128>(p, st);
+          launch_tc<E, D, 128, false>(p, st);
         }
       };
       auto by_q = [&](auto t_c, auto d_c) {

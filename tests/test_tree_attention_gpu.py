@@ -121,6 +121,42 @@ def test_tree_matches_reference(ltm, dt, cache, B, T, heads, kvh, d, lens):
     assert ltm.device_error() == 0
 
 
+@pytest.mark.parametrize("dt,cache,T,G,d", [("bf16", "int8", 9, 2, 128), ("f16", "int8", 16, 4, 64),
+                                           ("bf16", "int8", 64, 1, 64), ("f16", "int8", 11, 6, 128),
+                                           ("f16", "same", 8, 4, 128), ("bf16", "same", 40, 3, 64)])
+def test_many_rows_over_a_long_context(ltm, dt, cache, T, G, d):
+    """18 to 120 rows per cached head with contexts cut over many CTAs: keys that grow
+    towards the end (the references rise), V scales that span 2^6, query heads of very
+    different sizes.  Scores have a deviation of at most 1, so that of a row's p * scale
+    only those below 2^-14 of the largest (f16: 2^-25 off, not a relative 2^-11) make up
+    less than that share of the sum: check's bound holds as it is."""
+    import torch
+    B, kvh = 3, 4
+    lens = [12345, 0, 777]
+    P = max(lens) + T + 5
+    q, k, v, ks, vs, vk, vv = make(B, T, kvh * G, kvh, d, P, dt, cache, lens, 31 * T + G)
+    mag = 2.0 ** (6 * torch.arange(kvh * G, device="cuda") / (kvh * G) - 7)
+    q = (q.float() * mag[None, None, :, None]).to(q.dtype)
+    rise = torch.linspace(0.25, 2.0, P, device="cuda")[None, None, :]
+    size = 2.0 ** (6 * torch.rand((B, kvh, P), generator=torch.Generator().manual_seed(3)).cuda()
+                   - 3).round()
+    for b in range(B):
+        e = lens[b] + T
+        if cache == "int8":
+            ks[b, :, :e] = (ks[b] * rise[0])[:, :e]
+            vs[b, :, :e] = (vs[b] * size[b])[:, :e]
+            vk[b, :, :e] = (k[b].double() * ks[b].double()[..., None])[:, :e]
+            vv[b, :, :e] = (v[b].double() * vs[b].double()[..., None])[:, :e]
+        else:
+            k[b, :, :e] = (vk[b].float() * rise[0][..., None]).to(k.dtype)[:, :e]
+            vk[b, :, :e] = k[b, :, :e].double()
+    par = tree(B, T, 2)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    got = ltm.tree_attention(q, k, v, torch.tensor(lens, **i32), torch.tensor(par, **i32), ks, vs)
+    o, a = reference(q, vk, vv, lens, [T] * B, par)
+    check(got, o, a, dt, cache)
+
+
 @pytest.mark.parametrize("cache", ["same", "int8"])
 def test_long_context_over_many_ctas(ltm, cache):
     """Contexts long enough that several CTAs share a head, next to empty and
