@@ -285,7 +285,8 @@ LTM_API ltm_status ltm_memory_store_noalloc(void* memory, const void* keys, int6
  *   s = max_d |x_d| / 127 ;  q_d = clamp(round_half_away(x_d / s), -127, 127)
  *   per token and head (s == 0 => q = 0); a row with an infinity or a NaN gets
  *   s = NaN and q = 0, so that whatever reads it gets NaN.
- * Positions outside the written ones keep their bytes. */
+ * Positions outside the written ones keep their bytes.  The caches (and scales)
+ * overlap neither one another nor k and v. */
 LTM_API ltm_status ltm_kv_cache_append(const void* k, const int64_t* k_strides, const void* v,
                                        const int64_t* v_strides, ltm_dtype dtype, void* k_cache,
                                        void* v_cache, float* k_scale, float* v_scale,
@@ -298,7 +299,7 @@ LTM_API ltm_status ltm_kv_cache_append(const void* k, const int64_t* k_strides, 
  * q * s of an int8 cache (one fp32 product, rounded to out_dtype), or a copy of a
  * 16-bit cache of out_dtype (scale NULL).  Positions outside
  * [0, min(max_positions, cache_lens[b])) (cache_lens: device int32 [B] or NULL)
- * give zeros. */
+ * give zeros.  out does not overlap the cache. */
 LTM_API ltm_status ltm_kv_cache_read(const void* cache, const float* scale, ltm_dtype out_dtype,
                                      int64_t max_positions, const int32_t* first,
                                      const int32_t* cache_lens, int B, int kv_heads, int head_dim,
@@ -318,7 +319,8 @@ LTM_API ltm_status ltm_kv_cache_read(const void* cache, const float* scale, ltm_
  * b * s[0] + t * s[1] + h * s[2] (multiples of 8 elements), f16 / bf16; int8
  * caches serve both.  Tokens t >= num_tokens[b], and those of a skipped
  * sequence, get zeros.  What the cache holds at positions that a token does not
- * see never reaches its output, NaN and infinities included.
+ * see never reaches its output, NaN and infinities included.  o does not overlap
+ * the caches.
  * workspace: device memory of ltm_tree_attention_workspace bytes, 16-byte
  * aligned, that nothing else uses until the call's work is done. */
 LTM_API ltm_status ltm_tree_attention_workspace(int B, int T, int num_heads, int kv_heads,
@@ -358,7 +360,7 @@ LTM_API ltm_status ltm_beam_select(const void* logits, ltm_dtype dtype, int64_t 
  * their slot are not touched.  caches: host array of n_caches device pointers to
  * [B * W, kv_heads, max_positions, row] tensors, row_bytes[i] bytes per row
  * (a multiple of 4: K or V rows of any type, or an int8 cache's scales),
- * each listed once.  W <= 32.  A request whose beams hold an index outside
+ * none overlapping another.  W <= 32.  A request whose beams hold an index outside
  * [0, W), or whose range is not inside the cache, is left as it is and the device
  * error word set to 6. */
 LTM_API ltm_status ltm_kv_cache_reorder(void* const* caches, const int64_t* row_bytes,

@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -169,9 +170,29 @@ void check_pair(const at::Tensor& k, const at::Tensor& v, Opt ks, Opt vs) {
   if (k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type())
     bad("k_cache and v_cache must have one shape and type");
 }
-const int64_t* rows_strides(const at::Tensor& t, const char* what) {
-  if (t.stride(3) != 1) bad(std::string(what) + " must have unit stride in head_dim");
-  return t.strides().data();
+// Strides of a 4-dimensional tensor's first three dimensions; those of one entry
+// count as 0, whatever the tensor says.
+struct RowStrides {
+  int64_t s[3];
+  RowStrides(const at::Tensor& t, const char* what) {
+    if (t.stride(3) != 1) bad(std::string(what) + " must have unit stride in head_dim");
+    for (int i = 0; i < 3; ++i) s[i] = t.size(i) == 1 ? 0 : t.stride(i);
+  }
+};
+
+// Whether the spans of two tensors' elements meet.
+bool meet(const at::Tensor& a, const at::Tensor& b) {
+  auto end = [](const at::Tensor& t) {
+    int64_t last = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return static_cast<const char*>(t.data_ptr()) + last * static_cast<int64_t>(t.element_size());
+  };
+  return a.numel() > 0 && b.numel() > 0 && static_cast<const char*>(a.data_ptr()) < end(b) &&
+         static_cast<const char*>(b.data_ptr()) < end(a);
+}
+void apart(const at::Tensor& a, std::initializer_list<Opt> others, const char* msg) {
+  for (Opt t : others)
+    if (t != nullptr && meet(a, *t)) bad(msg);
 }
 
 template <class F>
@@ -207,10 +228,11 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       bad("the caches must be int8 or have k's type");
     check_index(&lens, {B});
     check_index(num, {B});
-    const int64_t *sk = rows_strides(k, "k"), *sv = rows_strides(v, "v");
+    const RowStrides sk(k, "k"), sv(v, "v");
+    for (Opt t : {&k, &v}) apart(*t, {&kc, &vc, ks, vs}, "k and v must not overlap the caches");
     const ltm_dtype dt = dtype_of(k.scalar_type());
     Call c(k, a[8]);
-    done(ltm_kv_cache_append(k.data_ptr(), sk, v.data_ptr(), sv, dt, kc.data_ptr(), vc.data_ptr(),
+    done(ltm_kv_cache_append(k.data_ptr(), sk.s, v.data_ptr(), sv.s, dt, kc.data_ptr(), vc.data_ptr(),
                              ptr_as<float>(ks), ptr_as<float>(vs), kc.size(2),
                              ptr_as<int32_t>(&lens), ptr_as<int32_t>(num), size32(B), size32(T),
                              size32(h), size32(d), c.stream()));
@@ -247,6 +269,7 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (given != nullptr && (given->sizes() != at::IntArrayRef(shape, 4) ||
                              given->scalar_type() != type || !given->is_contiguous()))
       bad("out must be contiguous [B, kv_heads, length, head_dim] of the read type");
+    if (given != nullptr) apart(*given, {&cache, scale}, "out must not overlap the cache");
     Call c(cache, a[7]);
     const at::Tensor out = given ? *given : c.empty(at::IntArrayRef(shape, 4), type);
     done(ltm_kv_cache_read(cache.data_ptr(), ptr_as<float>(scale), dt, P, ptr_as<int32_t>(first),
@@ -274,18 +297,24 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check_index(parents, {B, T});
     if (given != nullptr && (given->sizes() != q.sizes() || given->scalar_type() != q.scalar_type()))
       bad("out must have q's shape and type");
-    const int64_t* sq = rows_strides(q, "q");
+    if (given != nullptr) {
+      apart(*given, {&kc, &vc, ks, vs}, "out must not overlap the caches");
+      if (at::has_internal_overlap(*given) == at::MemOverlap::Yes)
+        bad("elements of out share memory");
+    }
+    const RowStrides sq(q, "q");
     const ltm_dtype dt = dtype_of(q.scalar_type());
     size_t bytes = 0;
     done(ltm_tree_attention_workspace(size32(B), size32(T), size32(heads), size32(kc.size(1)),
                                       size32(d), &bytes));
     Call c(q, a[9]);
     const at::Tensor out = given ? *given : c.empty(q.sizes(), q.scalar_type());
+    const RowStrides so(out, "out");
     const Call::Workspace ws = c.workspace(bytes);
-    done(ltm_tree_attention(q.data_ptr(), sq, kc.data_ptr(), vc.data_ptr(), ptr_as<float>(ks),
+    done(ltm_tree_attention(q.data_ptr(), sq.s, kc.data_ptr(), vc.data_ptr(), ptr_as<float>(ks),
                             ptr_as<float>(vs), kc.size(2), ptr_as<int32_t>(&lens),
                             ptr_as<int32_t>(num), ptr_as<int32_t>(parents), out.data_ptr(),
-                            rows_strides(out, "out"), size32(B), size32(T), size32(heads),
+                            so.s, size32(B), size32(T), size32(heads),
                             size32(kc.size(1)), size32(d), dt, ws.get(), bytes, c.stream()));
     return given ? Py_NewRef(a[8]) : THPVariable_Wrap(out);
   });
@@ -297,7 +326,7 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor &logits = tensor(a[0]), &scores = tensor(a[1]);
     Opt fin = tensor_or_none(a[3]);
     check_device(logits, {&scores, fin});
-    if (logits.dim() != 3 || logits.stride(2) != 1)
+    if (logits.dim() != 3 || (logits.size(2) > 1 && logits.stride(2) != 1))
       bad("logits must be [B, W, V] with unit stride in V");
     const int64_t B = logits.size(0), W = logits.size(1), V = logits.size(2);
     if (scores.scalar_type() != at::kFloat || scores.sizes() != at::IntArrayRef({B, W}) ||

@@ -17,7 +17,10 @@
 //
 // All three kernels are bound by memory.  Rows are handled by groups of lanes
 // that hold 16 bytes each, several rows per lane in flight.
+#include <algorithm>
 #include <type_traits>
+#include <utility>
+#include <vector>
 
 #include "block.cuh"
 
@@ -355,6 +358,11 @@ void check_dims(int B, int heads, int head_dim, int64_t P) {
   LTM_REQUIRE(P < (1ll << 31), "max_positions exceeds int32");
 }
 
+bool overlap(const void* a, const void* b, size_t bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + bytes && y < x + bytes;
+}
+
 template <class F>
 void by_head_dim(int D, F&& f) {
   if (D == 64) f(std::integral_constant<int, 64>{});
@@ -387,6 +395,10 @@ extern "C" ltm_status ltm_kv_cache_append(const void* k, const int64_t* k_stride
     check_rows(v, v_strides, dtype_size(dtype), "v");
     LTM_REQUIRE(((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) &
                  15) == 0, "the caches must be 16-byte aligned");
+    const size_t rows = static_cast<size_t>(B) * kv_heads * max_positions;
+    LTM_REQUIRE(!overlap(k_cache, v_cache, rows * head_dim * (q8 ? 1 : dtype_size(dtype))) &&
+                    !(q8 && overlap(k_scale, v_scale, rows * 4)),
+                "the K and V caches overlap");
     const RowStrides sk{k_strides[0], k_strides[1], k_strides[2]};
     const RowStrides sv{v_strides[0], v_strides[1], v_strides[2]};
     const int tok = 32 / (head_dim / kVals) * kRowsFly;
@@ -472,16 +484,20 @@ extern "C" ltm_status ltm_kv_cache_reorder(void* const* caches, const int64_t* r
     if (n_caches == 0 || B == 0) return;
     LTM_REQUIRE(caches && row_bytes && beams, "NULL pointer");
     int64_t widest = 0;
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans(n_caches);
     for (int i = 0; i < n_caches; ++i) {
       LTM_REQUIRE(caches[i] != nullptr, "NULL pointer");
       LTM_REQUIRE(row_bytes[i] > 0 && row_bytes[i] % 4 == 0 && row_bytes[i] <= 4096,
                   "row bytes must be a multiple of 4, at most 4096");
       const uintptr_t a = reinterpret_cast<uintptr_t>(caches[i]);
       LTM_REQUIRE(a % (row_bytes[i] % 16 == 0 ? 16 : 4) == 0, "a cache is not aligned to its rows");
-      for (int j = 0; j < i; ++j)
-        LTM_REQUIRE(caches[j] != caches[i], "the same cache is listed twice");
+      spans[i] = {a, a + static_cast<uintptr_t>(B) * W * kv_heads * max_positions * row_bytes[i]};
       if (row_bytes[i] > widest) widest = row_bytes[i];
     }
+    std::sort(spans.begin(), spans.end());
+    for (int i = 1; i < n_caches; ++i)
+      LTM_REQUIRE(spans[i].first >= spans[i - 1].second,
+                  "caches overlap (each may be listed once)");
     const cudaStream_t st = as_stream(stream);
     for (int i0 = 0; i0 < n_caches; i0 += kMaxReorder) {
       const int n = n_caches - i0 < kMaxReorder ? n_caches - i0 : kMaxReorder;

@@ -1666,6 +1666,8 @@ extern "C" ltm_status ltm_tree_attention(
       const int64_t heads0 = static_cast<int64_t>(b0) * kv_heads;
       LTM_REQUIRE(static_cast<int64_t>(p.B) * kv_heads * max_positions < (1ll << 31),
                   "cache rows exceed int32");
+      LTM_REQUIRE(static_cast<int64_t>(p.B) * num_heads * T < (1ll << 31) - kCWarps,
+                  "query rows exceed int32");
       p.rb = rb;
       const size_t slots = tree_slots(p.B, T, G, kv_heads, kTMaxGrid, rb, p.nrb);
       LTM_REQUIRE(workspace_bytes >= slots * rb * (head_dim + 4) * sizeof(float),
