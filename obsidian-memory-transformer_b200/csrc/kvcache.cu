@@ -15,8 +15,11 @@
 // (python_bindings/src/main.cpp:101-135); the quantizer's formula is that of
 // src/core/quantization/quantizer.cu:94-142 with a row per token and head.
 //
-// All three kernels are bound by memory.  Rows are handled by groups of lanes
-// that hold 16 bytes each, several rows per lane in flight.
+// Rows are handled by groups of lanes that hold 16 bytes each, several rows per lane in
+// flight.  Measured (cold caches): the int8 write of 4 x 8192 tokens, 32 heads of 128 dims
+// (bf16), 165 us for 0.81 GB (4.9 TB/s; arithmetic: 14 instructions a value); reading
+// either cache back 72 us for 0.40 GB (5.6 TB/s); the reorder of 32 beams' caches 476 us,
+// at the copy bandwidth.
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -29,7 +32,7 @@ namespace {
 
 constexpr int kWarps = 8;    // warps per CTA of the write and read kernels
 constexpr int kVals = 16;    // values of a row per lane
-constexpr int kRowsFly = 2;  // rows in flight per lane group (write)
+constexpr int kRowsFly = 4;  // rows in flight per lane group (write)
 constexpr int kReadFly = 4;  // rows in flight per lane group (read)
 
 struct RowStrides {
@@ -54,57 +57,73 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
-// Scale and codes of one row: 16 values per lane, packed to four words.  All 32
-// lanes call it (lanes without a row pass zeros).  abs_bits: the row's largest
-// |x| as bits, where an infinity or a NaN compares above every finite value.
-//
-// The scale is the IEEE quotient amax / 127, by Markstein's correction of the
-// product with the rounded reciprocal (q = a y, q + (a - 127 q) y with fused
-// multiply-adds; compared with the division for every mantissa on the CPU); amax
-// below 2^-100, where the correction could underflow, is divided.
-// The quotients are estimated with an approximate reciprocal (relative error
-// 2^-23, another 2^-24 by the product) and rounded by adding 1.5 * 2^23: an
-// estimate of |t| <= 127.5 is off by at most 2.3e-5, the IEEE quotient by 0.8e-5,
-// so both round alike unless the estimate is within 2^-14 of a tie; such values
-// (6% of the warps' rows have one) take the division and round half away from zero.
-__device__ __forceinline__ float quant_row16(const float (&v)[kVals], uint32_t abs_bits,
-                                             uint32_t (&code)[kVals / 4]) {
-  constexpr float kShift = 12582912.0f;            // 1.5 * 2^23
-  constexpr float kTie = 0.5f - 6.103515625e-5f;   // 0.5 - 2^-14
+// prmt with its sign modes: selector nibble 8 | i gives byte i's sign, eight times.
+__device__ __forceinline__ uint32_t signs_of(uint32_t lo, uint32_t hi, uint32_t sel) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(lo), "r"(hi), "r"(sel));
+  return r;
+}
+
+// Scale of a row from its largest |x|: the IEEE quotient amax / 127, by Markstein's
+// correction of the product with the rounded reciprocal (q = a y, q + (a - 127 q) y with
+// fused multiply-adds; compared with the division for every mantissa on the CPU); small
+// amax, where the correction could underflow, is divided.
+constexpr float kTiny = 8.0779357e-28f;  // 2^-90
+__device__ __forceinline__ float row_scale(float amax) {
   constexpr float kY = 1.0f / 127.0f;
-  const float amax = __uint_as_float(abs_bits);
-  const bool bad = abs_bits >= 0x7f800000u, tiny = amax < 7.9e-31f;
   float s = amax * kY;
   s = fmaf(fmaf(-s, 127.0f, amax), kY, s);
-  if (tiny) s = __fdiv_rn(amax, 127.0f);
-  const float inv = (bad || tiny) ? 0.0f : rcp_approx(s);
-  const uint64_t inv2 = f2_pack(inv, inv), shift2 = f2_pack(kShift, kShift);
-  float big[kVals], off[kVals];
-  float far = 0.0f;  // the largest distance from the rounded value
+  if (amax < kTiny) s = __fdiv_rn(amax, 127.0f);
+  return s;
+}
+
+// What the codes of a row take from it.
+struct RowQuant {
+  uint64_t inv, ms;  // 1 / s (approximate) and -s, twice
+  float up;          // 2^50 / s
+  uint32_t keep;     // all ones, or 0: zero codes
+};
+
+// Codes of four values of a row, in magnitudes (a) and signs (a byte of ones for each
+// negative value): the IEEE quotient q = RN(a / s) rounded half up, without a division.
+//
+// n = floor(a / s) or, just above an integer, one less, from an approximate reciprocal
+// (off by at most 2e-5); then the code is n + 1 where q >= c = n + 1/2, else n.  RN ties
+// to even and c is even, so q >= c iff a / s >= (c + c') / 2, c' the float below c:
+//   w = (a - c s) + (a - c' s) >= 0 .
+// Near the threshold both differences are exact as fused multiply-adds for s >= 2^-97: a
+// and c s are multiples of 2^(e-24) (s in [2^e, 2^(e+1))) that differ by less than
+// 2^-14 s, and a - c' s, a multiple of 2^(e+k-46) for c in [2^k, 2^(k+1)), is there about
+// s 2^(k-24); so w, where it is negative, is at most -2^(e-47), and 1 + 2^50 w / s,
+// clamped to [0, 1], is the step.  Farther away the signs are certain.  c' is RN(c -
+// 2^-24 c): c is a power of two only as 1/2, otherwise 2^-24 c lies between half a unit
+// and one.
+// (Dividing where the estimate is near a tie cost 250 us for a prompt of 4 x 8192 tokens,
+// 32 heads of 128: most warps of 16-bit rows hold a tie.)
+__device__ __forceinline__ uint32_t quant4(const float (&a)[4], uint32_t neg, const RowQuant& r) {
+  constexpr float kShift = 12582912.0f;  // 1.5 * 2^23: the sum's low byte is the integer
+  constexpr float kBelow = 1.0f - 5.9604644775390625e-8f;  // 1 - 2^-24
+  const uint64_t shift2 = f2_pack(kShift, kShift), half2 = f2_pack(0.5f, 0.5f);
+  const uint64_t mhalf2 = f2_pack(-0.5f, -0.5f), below2 = f2_pack(kBelow, kBelow);
+  float big[4];
 #pragma unroll
-  for (int i = 0; i < kVals; i += 2) {
-    const uint64_t t = f2_mul(f2_pack(v[i], v[i + 1]), inv2);
-    const uint64_t b = f2_add(t, shift2);
-    f2_unpack(f2_sub(t, f2_sub(b, shift2)), off[i], off[i + 1]);
-    f2_unpack(b, big[i], big[i + 1]);
-    far = fmaxf(far, fmaxf(fabsf(off[i]), fabsf(off[i + 1])));
+  for (int i = 0; i < 4; i += 2) {
+    const uint64_t a2 = f2_pack(a[i], a[i + 1]);
+    const uint64_t b = f2_add(f2_fma(a2, r.inv, mhalf2), shift2);
+    const uint64_t c = f2_add(f2_sub(b, shift2), half2);
+    float w0, w1;
+    f2_unpack(f2_add(f2_fma(c, r.ms, a2), f2_fma(f2_mul(c, below2), r.ms, a2)), w0, w1);
+    float s0, s1;
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(s0) : "f"(w0), "f"(r.up), "f"(1.0f));
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(s1) : "f"(w1), "f"(r.up), "f"(1.0f));
+    f2_unpack(f2_add(b, f2_pack(s0, s1)), big[i], big[i + 1]);
   }
-  const bool divide = tiny && s > 0.0f;
-  if ((far >= kTie || divide) && !bad) {
-#pragma unroll
-    for (int i = 0; i < kVals; ++i)
-      if (divide || fabsf(off[i]) >= kTie) {
-        const float r = fminf(fmaxf(roundf(__fdiv_rn(v[i], s)), -127.0f), 127.0f);
-        big[i] = r + kShift;
-      }
-  }
-#pragma unroll
-  for (int i = 0; i < kVals / 4; ++i) {  // the low byte holds the code
-    const uint32_t lo = __byte_perm(__float_as_uint(big[4 * i]), __float_as_uint(big[4 * i + 1]), 0x0040);
-    const uint32_t hi = __byte_perm(__float_as_uint(big[4 * i + 2]), __float_as_uint(big[4 * i + 3]), 0x0040);
-    code[i] = bad ? 0u : __byte_perm(lo, hi, 0x5410);
-  }
-  return bad ? __int_as_float(0x7fc00000) : s;
+  const uint32_t m =  // magnitudes, at most 127 each
+      __byte_perm(__byte_perm(__float_as_uint(big[0]), __float_as_uint(big[1]), 0x0040),
+                  __byte_perm(__float_as_uint(big[2]), __float_as_uint(big[3]), 0x0040), 0x5410);
+  // byte-wise (m ^ neg) - neg without carries between bytes
+  return (((m ^ neg) & (r.keep & 0x7f7f7f7fu)) + (neg & (r.keep & 0x01010101u))) ^
+         (neg & (r.keep & 0x80808080u));
 }
 
 // Bits of the largest |x| of a 16-byte vector.
@@ -130,15 +149,45 @@ __device__ __forceinline__ uint32_t widen_bits(uint32_t m) {
   }
 }
 
-// New tokens into the caches.  Bound by memory (input read once, codes and scales
-// written once).  A lane holds 16 values of a row (two or four 16-byte pieces a
+// |x| and signs (a byte of ones where negative) of values 4g .. 4g + 3 of a lane.
+template <class T, int NP>
+__device__ __forceinline__ void magnitudes(const uint4 (&raw)[NP], int g, float (&a)[4],
+                                           uint32_t& neg) {
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t x[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = fabsf(__uint_as_float(x[i]));
+    neg = __byte_perm(signs_of(x[0], x[1], 0x00fb), signs_of(x[2], x[3], 0x00fb), 0x5410);
+  } else {
+    const uint4& r = raw[g / 2];
+    const uint32_t x[2] = {g % 2 ? r.z : r.x, g % 2 ? r.w : r.y};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t y = x[i] & 0x7fff7fffu;
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y));
+        a[2 * i] = f.x;
+        a[2 * i + 1] = f.y;
+      } else {
+        a[2 * i] = __uint_as_float(y << 16);
+        a[2 * i + 1] = __uint_as_float(y & 0xffff0000u);
+      }
+    }
+    neg = signs_of(x[0], x[1], 0xfdb9);
+  }
+}
+
+// New tokens into the caches: input read once, codes and scales written once.  The int8
+// write is bound by its arithmetic (70% of the issue slots, 57% of the integer pipe; 4
+// rows in flight, because a warp's fixed part is 125 instructions: 322 -> 307 us with the
+// reads of both caches, from 388 with divisions), the 16-bit one by memory.  A lane holds 16 values of a row (two or four 16-byte pieces a
 // group's width apart, so that loads and stores are contiguous over the group),
 // a group of D / 16 lanes a row; a warp takes kRowsFly * 32 / group
 // consecutive tokens of one head, K or V, so that its int8 rows are one
 // contiguous block and its scales whole 32-byte sectors; neighbouring warps take
 // neighbouring heads of the same tokens: the reads cover whole projection rows.
 template <class T, int D, bool Q8>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 ? 4 : 2)
     cache_append_kernel(const T* __restrict__ k, RowStrides sk, const T* __restrict__ v,
                         RowStrides sv, void* __restrict__ kc, void* __restrict__ vc,
                         float* __restrict__ ks, float* __restrict__ vs, int64_t P,
@@ -179,16 +228,12 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int t = tg * TOK + j * RP + sub;
     if (tg * TOK + j * RP >= n) break;  // uniform over the warp
     if constexpr (Q8) {
-      float x[kVals];
       uint32_t m = 0;
 #pragma unroll
       for (int q = 0; q < NP; ++q) {
         const uint32_t a = abs_max_bits<T>(raw[j][q]);
         if constexpr (sizeof(T) == 4) m = max(m, a);
         else m = __vmaxu2(m, a);
-        const T* e = reinterpret_cast<const T*>(&raw[j][q]);
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[q * N + i] = to_f32(e[i]);
       }
 #pragma unroll
       for (int o = G / 2; o > 0; o >>= 1) {
@@ -196,8 +241,36 @@ __global__ void __launch_bounds__(kWarps * 32)
         if constexpr (sizeof(T) == 4) m = max(m, a);
         else m = __vmaxu2(m, a);
       }
+      const uint32_t abs_bits = widen_bits<T>(m);
+      const bool bad = abs_bits >= 0x7f800000u;  // an infinity or a NaN
+      const float amax = __uint_as_float(abs_bits);
+      const bool tiny = amax < kTiny;
+      float s = row_scale(amax);
+      const float inv = rcp_approx(s);
+      const RowQuant rq{f2_pack(inv, inv), f2_pack(-s, -s), inv * 1.125899906842624e15f,
+                        bad || tiny ? 0u : ~0u};
       uint32_t code[kVals / 4];
-      const float s = quant_row16(x, widen_bits<T>(m), code);
+#pragma unroll
+      for (int g = 0; g < kVals / 4; ++g) {
+        float a[4];
+        uint32_t neg;
+        magnitudes<T>(raw[j], g, a, neg);
+        code[g] = quant4(a, neg, rq);
+      }
+      if (tiny && s > 0.0f) {  // divided
+#pragma unroll
+        for (int g = 0; g < kVals / 4; ++g) {
+          float a[4];
+          uint32_t neg;
+          magnitudes<T>(raw[j], g, a, neg);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int c = static_cast<int>(fminf(roundf(__fdiv_rn(a[i], s)), 127.0f));
+            code[g] |= static_cast<uint32_t>((neg >> (8 * i) & 1u ? -c : c) & 0xff) << (8 * i);
+          }
+        }
+      }
+      if (bad) s = __int_as_float(0x7fc00000);
       if (t < n) {
         int8_t* dst = static_cast<int8_t*>(is_v ? vc : kc) + (row0 + t) * D + gl * N;
 #pragma unroll

@@ -62,6 +62,38 @@ def test_append_int8_bit_exact(ltm, dt, B, T, h, d, P):
     assert ltm.device_error() == 0
 
 
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+def test_append_rounds_like_the_division(ltm, dt):
+    """Values at and next to the ties of every row's scale: rows whose largest values
+    take every bf16 mantissa (and some of every other type's), values that are
+    (n + 1/2) * amax / 127 moved by a few units in the last place, either sign, over many
+    magnitudes."""
+    import torch
+    T, h, d = 128, 16, 128
+    g = torch.Generator().manual_seed(1)
+    top = (1 + torch.arange(T) / 128)[:, None] * (2.0 ** (8 * torch.arange(h) - 100).double())[None]
+    if dt != "bf16":
+        top = top * (1 + torch.rand((T, h), generator=g, dtype=torch.float64) / 200)
+    if dt == "f16":
+        top = top * 2.0 ** 100 / 2.0 ** (8 * torch.arange(h) - torch.arange(h) % 13 + 3).double()
+    n = torch.randint(0, 127, (T, h, d), generator=g).double() + 0.5
+    x = (n / 127 * top.to(torch_dtype(dt)).double()[..., None]).to(torch_dtype(dt))
+    bits = torch.int32 if dt == "f32" else torch.int16
+    step = torch.randint(-2, 3, (T, h, d), generator=g)
+    x = (x.view(bits) + step.to(bits)).view(torch_dtype(dt))
+    x[:, :, 5] = top.to(torch_dtype(dt))
+    x = torch.minimum(x, x[:, :, 5:6]) * (1 - 2 * torch.randint(0, 2, (T, h, d), generator=g)).to(x.dtype)
+    x = x[None].cuda()
+    kc = torch.zeros((1, h, T, d), dtype=torch.int8, device="cuda")
+    vc, ks = kc.clone(), torch.zeros((1, h, T), device="cuda")
+    vs = ks.clone()
+    ltm.kv_cache_append(x, -x, kc, vc, torch.zeros(1, dtype=torch.int32, device="cuda"), ks, vs)
+    for y, c, s in ((x, kc, ks), (-x, vc, vs)):
+        q, sc = quant_rows(y.float().cpu().numpy().transpose(0, 2, 1, 3))
+        assert np.array_equal(s.cpu().numpy(), sc)
+        assert np.array_equal(c.cpu().numpy(), q)
+
+
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
 @pytest.mark.parametrize("d", [64, 128])
 def test_append_same_type_copies(ltm, dt, d):
