@@ -83,6 +83,7 @@ struct TreeParams {
   const int* parents;
   int B, T, G, kvh, nrb, rb;  // nrb: row blocks per cached head, of rb rows
   int tile;                   // positions per tile
+  float inv_g;                // 1 / G
   int64_t P;
   float sl2;
   float* part;
@@ -102,15 +103,25 @@ __device__ __forceinline__ bool tree_seq(const TreeParams& p, int b, int& len, i
   return ok;
 }
 
+// TILE, RB: p.tile and p.rb where the kernel knows them (integer divisions by a variable
+// are most of what finding a tile costs), else 0.
+template <int TILE>
 __device__ __forceinline__ int tiles_of(const TreeParams& p, int len, int n) {
-  return n > 0 ? (len + n - 1) / p.tile + 1 : 0;
+  return n > 0 ? (len + n - 1) / (TILE ? TILE : p.tile) + 1 : 0;
 }
+template <int RB>
 __device__ __forceinline__ int row_blocks(const TreeParams& p, int n) {
-  return (p.G * n + p.rb - 1) / p.rb;
+  const int rb = RB ? RB : p.rb;
+  return (p.G * n + rb - 1) / rb;
+}
+// x / G for 0 <= x < 2^13 (G <= 64: (x + 1/2) / G is 2^-7 away from every integer)
+__device__ __forceinline__ int over_g(const TreeParams& p, int x) {
+  return static_cast<int>((static_cast<float>(x) + 0.5f) * p.inv_g);
 }
 
 // First tile of every sequence in the batch's list, and the sequences' lengths and
 // token counts after it ([kTBatch + 2] words each), by one warp.
+template <int TILE, int RB>
 __device__ __forceinline__ void tree_scan(const TreeParams& p, uint32_t* base, int lane) {
   uint32_t carry = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
@@ -119,7 +130,7 @@ __device__ __forceinline__ void tree_scan(const TreeParams& p, uint32_t* base, i
     if (b < p.B) {
       int len, n;
       tree_seq(p, b, len, n);
-      w = static_cast<uint32_t>(p.kvh) * row_blocks(p, n) * tiles_of(p, len, n);
+      w = static_cast<uint32_t>(p.kvh) * row_blocks<RB>(p, n) * tiles_of<TILE>(p, len, n);
       base[kTBatch + 2 + b] = static_cast<uint32_t>(len);
       base[2 * (kTBatch + 2) + b] = static_cast<uint32_t>(n);
     }
@@ -148,6 +159,7 @@ __device__ __forceinline__ uint32_t share_of(uint32_t tile, uint32_t total, uint
 struct TreeSpan {
   int b, h, rb, len, n, rows, tile, tiles;  // tile: index within the head's keys
 };
+template <int TILE, int RB>
 __device__ __forceinline__ TreeSpan tree_find(const TreeParams& p, const uint32_t* base, uint32_t w) {
   int lo = 0, hi = p.B;  // base[lo] <= w < base[hi]
   while (hi - lo > 1) {
@@ -159,14 +171,14 @@ __device__ __forceinline__ TreeSpan tree_find(const TreeParams& p, const uint32_
   s.b = lo;
   s.len = static_cast<int>(base[kTBatch + 2 + lo]);
   s.n = static_cast<int>(base[2 * (kTBatch + 2) + lo]);
-  s.tiles = tiles_of(p, s.len, s.n);
-  const int nrb = row_blocks(p, s.n);
+  s.tiles = tiles_of<TILE>(p, s.len, s.n);
+  const int nrb = row_blocks<RB>(p, s.n);
   const uint32_t at = w - base[lo];
   const uint32_t item = at / s.tiles;
   s.tile = static_cast<int>(at - item * s.tiles);
-  s.h = static_cast<int>(item / nrb);
+  s.h = static_cast<int>(nrb == 1 ? item : item / nrb);
   s.rb = static_cast<int>(item - s.h * nrb);
-  s.rows = min(p.rb, p.G * s.n - s.rb * p.rb);
+  s.rows = min(RB, p.G * s.n - s.rb * RB);
   return s;
 }
 
@@ -182,9 +194,10 @@ __device__ __forceinline__ void tree_masks(const TreeParams& p, int b, int n, in
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int t = lane + 32 * i;
-    m[i] = 1ull << t;
-    up[i] = t - 1;
+    m[i] = (2ull << t) - 1;  // a chain
+    up[i] = -1;
     if (p.parents != nullptr) {
+      m[i] = 1ull << t;
       up[i] = t < n ? p.parents[static_cast<int64_t>(b) * p.T + t] : -1;
       if (up[i] >= t || up[i] < -1) {
         bad = true;
@@ -194,7 +207,7 @@ __device__ __forceinline__ void tree_masks(const TreeParams& p, int b, int n, in
   }
   if (bad) atomicExch(p.err, kErrBadParent);
 #pragma unroll 1
-  for (int reach = 1; reach < n; reach *= 2) {
+  for (int reach = 1; reach < n && p.parents != nullptr; reach *= 2) {
     unsigned long long a[2];
     int nx[2];
 #pragma unroll
@@ -216,7 +229,7 @@ __device__ __forceinline__ void tree_masks(const TreeParams& p, int b, int n, in
   __syncwarp();  // the sets of the segment before have been read
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int r = lane + 32 * i, tok = (row0 + r) / p.G;
+    const int r = lane + 32 * i, tok = over_g(p, row0 + r);
     const unsigned long long m0 = __shfl_sync(0xffffffffu, m[0], tok & 31);
     const unsigned long long m1 = __shfl_sync(0xffffffffu, m[1], tok & 31);
     if (r < rows) mask[r] = tok >= n ? 0ull : tok < 32 ? m0 : m1;
@@ -224,33 +237,32 @@ __device__ __forceinline__ void tree_masks(const TreeParams& p, int b, int n, in
   __syncwarp();
 }
 
-// Whether a 16-bit value of a word is not finite: exponent bits all ones.
+// Bit 15 of each half of a word whose 16-bit value is not finite (its exponent bits are
+// all ones).
 template <class T>
 __device__ __forceinline__ uint32_t non_finite_halves(uint32_t w) {
-  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  uint32_t keep = 0xffffffffu;
-  if ((w & kExp) == kExp) keep &= 0xffff0000u;
-  if (((w >> 16) & kExp) == kExp) keep &= 0x0000ffffu;
-  return keep;
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  constexpr uint32_t kOne = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+  return ((w & kExp) + kOne) & 0x80008000u;
+}
+template <class T>
+__device__ __forceinline__ uint32_t non_finite_in(const uint4& x) {
+  return non_finite_halves<T>(x.x) | non_finite_halves<T>(x.y) | non_finite_halves<T>(x.z) |
+         non_finite_halves<T>(x.w);
+}
+template <class T>
+__device__ __forceinline__ uint32_t finite_of(uint32_t w) {
+  return w & ~((non_finite_halves<T>(w) >> 15) * 0xffffu);
 }
 // One 16-byte unit of a tile's V row: zeroed (`drop`: nothing is there), or
 // without its non-finite values (a drafted token); returns whether any was found.
 template <class T>
 __device__ __forceinline__ bool clean_unit(uint8_t* at, bool drop) {
-  uint4 x = *reinterpret_cast<const uint4*>(at);
-  uint32_t keep[4] = {0u, 0u, 0u, 0u};
-  if (!drop) {
-    keep[0] = non_finite_halves<T>(x.x);
-    keep[1] = non_finite_halves<T>(x.y);
-    keep[2] = non_finite_halves<T>(x.z);
-    keep[3] = non_finite_halves<T>(x.w);
-    if ((keep[0] & keep[1] & keep[2] & keep[3]) == 0xffffffffu) return false;
-  }
-  x.x &= keep[0];
-  x.y &= keep[1];
-  x.z &= keep[2];
-  x.w &= keep[3];
-  *reinterpret_cast<uint4*>(at) = x;
+  const uint4 x = *reinterpret_cast<const uint4*>(at);
+  if (!drop && non_finite_in<T>(x) == 0u) return false;
+  *reinterpret_cast<uint4*>(at) =
+      drop ? make_uint4(0u, 0u, 0u, 0u)
+           : make_uint4(finite_of<T>(x.x), finite_of<T>(x.y), finite_of<T>(x.z), finite_of<T>(x.w));
   return !drop;
 }
 
@@ -394,7 +406,7 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
     tma_prefetch_desc(&tmV);
   }
   grid_wait();
-  if (warp == 0) tree_scan(p, base, lane);
+  if (warp == 0) tree_scan<S::kKeys, ROWS>(p, base, lane);
   __syncthreads();
   grid_release();
   const uint32_t total = base[p.B];
@@ -409,7 +421,7 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
       int it = 0;
       bool ok = true;
       for (uint32_t w = w0; ok && w < w1;) {
-        const TreeSpan s = tree_find(p, base, w);
+        const TreeSpan s = tree_find<S::kKeys, ROWS>(p, base, w);
         const int nt = min(static_cast<int>(w1 - w), s.tiles - s.tile);
         const int row = static_cast<int>((static_cast<int64_t>(s.b) * p.kvh + s.h) * p.P) +
                         s.tile * S::kKeys;
@@ -445,7 +457,7 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
   unsigned long long* mask = reinterpret_cast<unsigned long long*>(smem + S::kOffMask) + cw * ROWS;
   int it = 0, seg = 0;  // the CTA's tiles so far; parity of its segments
   for (uint32_t w = w0; w < w1; seg ^= 1) {
-    const TreeSpan sp = tree_find(p, base, w);
+    const TreeSpan sp = tree_find<S::kKeys, ROWS>(p, base, w);
     const int nt = min(static_cast<int>(w1 - w), sp.tiles - sp.tile);
     const int64_t head = static_cast<int64_t>(sp.b) * p.kvh + sp.h;
     const int keys = sp.len + sp.n;
@@ -468,8 +480,8 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
     float qinv[NR][2];  // of rows 2c, 2c + 1
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
-      const int r = nr * 8 + g, rr = sp.rb * p.rb + r;
-      const int t = rr / p.G, gg = rr - t * p.G;
+      const int r = nr * 8 + g, rr = sp.rb * ROWS + r;
+      const int t = over_g(p, rr), gg = rr - t * p.G;
       const T* qp = static_cast<const T*>(p.q) + sp.b * p.qb + t * p.qt +
                     (static_cast<int64_t>(sp.h) * p.G + gg) * p.qh;
       const bool live = r < sp.rows;
@@ -505,7 +517,7 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
       }
     }
     if ((sp.tile + nt) * S::kKeys > sp.len)
-      tree_masks(p, sp.b, sp.n, sp.rb * p.rb, ROWS, mask, lane);
+      tree_masks(p, sp.b, sp.n, sp.rb * ROWS, ROWS, mask, lane);
     // o[nr][u]: dims of 16-byte-pair u (rows of the A tile) x rows 2c, 2c + 1
     float o[NR][NU][4], l[NR][2], mref[NR][2], eref[NR][2], frow[NR][2];
 #pragma unroll
@@ -741,7 +753,7 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
     for (int k = 0; k < NW; ++k) all_ok &= wait_ok[k] != 0;
     if (!all_ok) return;  // a wait ran out: every consumer leaves here
     const int64_t item = head * p.nrb + sp.rb;
-    float* pp = p.part + (static_cast<int64_t>(blockIdx.x) + item) * p.rb * part_stride<D>();
+    float* pp = p.part + (static_cast<int64_t>(blockIdx.x) + item) * ROWS * part_stride<D>();
     for (int i = ct; i < sp.rows * (D / 4); i += NW * 32) {
       const int r = i / (D / 4), d = (i % (D / 4)) * 4;
       const float* in = merge + r * S::kMergeRow;
@@ -791,29 +803,31 @@ struct TcSmem {
   static constexpr int kP = kPs * kPOne;
   static constexpr int kOffP = kQ;
   static constexpr int kOffRing = kOffP + kP;
-  static constexpr int kLeft = 214 * 1024 - kOffRing;
+  // 128 rows: the sums by the tensor core, behind the ring 16 keys x 64 ones
+  static constexpr bool kSum = N == 128 && !Q8;
+  static constexpr int kOnes = kSum ? 2048 : 0;
+  static constexpr int kLeft = 212 * 1024 - kOffRing;
   static constexpr int kFit = kLeft / kTile;
   static constexpr int kSlots = Q8 ? (D == 64 ? 6 : 3) : kFit > 8 ? 8 : kFit;
   static constexpr int kCodes = Q8 ? kTcTile * D : 0;        // K or V tile of codes
   static constexpr int kSlots8 = !Q8 ? 0 : D == 64 ? 8 : 4;
   static constexpr int kOffCodes = kOffRing + kSlots * kTile;
   static_assert(kSlots * kTile + kSlots8 * kCodes <= kLeft && kSlots >= 3, "ring");
-  static constexpr int kOffMax = kOffCodes + kSlots8 * kCodes;  // [2][4][N] maxima / sums
+  static constexpr int kOffOnes = kOffCodes + kSlots8 * kCodes;
+  static constexpr int kOffMax = kOffOnes + kOnes;  // [2][4][N] maxima / sums
   static constexpr int kOffRef = kOffMax + 8 * N * 4;        // [6][N] per row, see the kernel
   static constexpr int kOffMask = kOffRef + 6 * N * 4;       // [softmax warps][rows] ancestor sets
   static constexpr int kOffBase = kOffMask + 4 * N * 8;
   static constexpr int kOffBar = (kOffBase + kScanWords * 4 + 7) / 8 * 8;
   static constexpr int kBars = 2 * kSlots + 2 * kSlots8 + 10;
   static constexpr int kOffFlag = kOffBar + kBars * 8;
-  // softmax: groups of four warps, each with 32 rows, or with 64 of 128 (four groups would
-  // leave 96 registers a thread: 2.1 -> 3.0 us a tile)
-  static constexpr int kRows = N <= 64 ? 32 : 64, kGroups = N / kRows;
+  static constexpr int kRows = 32, kGroups = N / kRows;  // softmax: groups of four warps
   // int8: warps 2, 3 convert, and two more, but not with 64 rows of 64 dims: the 13th warp
   // costs the softmax registers (168 -> 128; 2.26 us a tile against 1.66), which 128 dims,
   // bound by the conversion, are worth (2.44 us against 2.84)
   static constexpr int kConv = N == 64 && D == 64 ? 2 : 4;
   static constexpr int kThreads = 128 + 128 * kGroups + (Q8 ? 32 * (kConv - 2) : 0);
-  static constexpr int kBytes = kOffFlag + 48 + 1024;
+  static constexpr int kBytes = kOffFlag + 80 + 1024;
   static_assert(kBytes <= 232448, "shared memory of one CTA");
 };
 
@@ -864,9 +878,9 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
                    const TreeParams p) {
   using S = TcSmem<D, N, Q8>;
   constexpr int NS = S::kSlots, N8 = S::kSlots8;
-  static_assert(!Q8 || S::kRows == 32, "int8: 32 rows a softmax group");
-  constexpr int RW = S::kRows, NC = RW / 32, kSoft = 128 * S::kGroups, PB = S::kPs;
-  constexpr uint32_t kCols = N <= 32 ? 128 : N <= 64 ? 256 : 512;  // 3 N columns
+  constexpr int RW = S::kRows, kSoft = 128 * S::kGroups, PB = S::kPs;
+  constexpr bool SUM = S::kSum;
+  constexpr uint32_t kCols = 4 * N;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -911,13 +925,21 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
     __syncwarp();
     tmem_alloc(tslot, kCols);
   }
+  if constexpr (SUM) {
+    if (warp >= 2 && warp < 4) {
+      constexpr uint32_t k1 = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
+      for (int i = threadIdx.x - 64; i < S::kOnes / 16; i += 64)
+        reinterpret_cast<uint4*>(smem + S::kOffOnes)[i] = make_uint4(k1, k1, k1, k1);
+      fence_proxy_async_smem();
+    }
+  }
   grid_wait();
-  if (warp == 0) tree_scan(p, base, lane);
+  if (warp == 0) tree_scan<kTcTile, N>(p, base, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   grid_release();
-  const uint32_t tmem = *tslot, tO = tmem + 2 * N;
+  const uint32_t tmem = *tslot, tO = tmem + 2 * N, tL = tO + N;
   const uint32_t total = base[p.B];
   const uint32_t shares = min(total, gridDim.x);
   uint32_t w0 = 0, w1 = 0;  // no tiles: every role falls through to the end
@@ -936,7 +958,7 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
       int it = 0;  // ring slots used
       bool ok = true;
       for (uint32_t w = w0; ok && w < w1;) {
-        const TreeSpan s = tree_find(p, base, w);
+        const TreeSpan s = tree_find<kTcTile, N>(p, base, w);
         const int nt = min(static_cast<int>(w1 - w), s.tiles - s.tile);
         const int row = static_cast<int>((static_cast<int64_t>(s.b) * p.kvh + s.h) * p.P) +
                         s.tile * kTcTile;
@@ -969,8 +991,7 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
       constexpr uint32_t idS = idesc_f16(128, N, kBF);
       // A = V^T: M (dims) contiguous; B = P: N (rows) contiguous
       constexpr uint32_t idO = idesc_f16(128, N, kBF, true) | (1u << 15);
-      // D = 64: the upper 64 lanes repeat the lower ones (chunk stride 0)
-      constexpr uint32_t kVChunk = D == 128 ? kTcTile * 128 : 0;
+      const uint32_t ones = smem_u32(smem + S::kOffOnes);
       const uint32_t aQ = smem_u32(smem), aP = smem_u32(smem + S::kOffP);
       const uint32_t ring = smem_u32(smem + S::kOffRing);
       int it = 0, seg = 0;  // tiles, segments so far
@@ -1002,15 +1023,21 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
         tc_fence_after();
         const uint32_t aV = ring + ((2 * j + 1) % NS) * S::kTile;
 #pragma unroll
-        for (int k = 0; k < kTcTile / 16; ++k)
-          tc_mma_f16(tO, make_desc_mnmajor_sw128(aV + k * 2048, kVChunk),
-                     make_desc_mnmajor_sw128(aP + pb * S::kPOne + k * 2048, S::kPChunk), idO, !first || k != 0);
+        for (int k = 0; k < kTcTile / 16; ++k) {
+          // D = 64: the upper 64 lanes are the ones' (or repeat the lower ones)
+          const uint32_t av = aV + k * 2048;
+          const uint32_t chunk = D == 128 ? kTcTile * 128 : SUM ? ones - av : 0u;
+          const uint64_t bP = make_desc_mnmajor_sw128(aP + pb * S::kPOne + k * 2048, S::kPChunk);
+          tc_mma_f16(tO, make_desc_mnmajor_sw128(av, chunk), bP, idO, !first || k != 0);
+          if constexpr (D == 128 && SUM)
+            tc_mma_f16(tL, make_desc_mnmajor_sw128(ones, 0), bP, idO, !first || k != 0);
+        }
         tc_commit(pv_done + pb);
         tc_commit(empty + (2 * j + 1) % NS);
         return true;
       };
       for (uint32_t w = w0; ok && w < w1; ++seg) {
-        const TreeSpan s = tree_find(p, base, w);
+        const TreeSpan s = tree_find<kTcTile, N>(p, base, w);
         const int nt = min(static_cast<int>(w1 - w), s.tiles - s.tile);
         ok = mbar_wait_bounded(q_full, seg & 1, abort_flag, p.err, kErrWaitFull);
         if (ok) ok = issue_s(it);
@@ -1044,27 +1071,27 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
     int it = 0;
     bool ok = true;
     for (uint32_t w = w0; ok && w < w1;) {
-      const TreeSpan sp = tree_find(p, base, w);
+      const TreeSpan sp = tree_find<kTcTile, N>(p, base, w);
       const int nt = min(static_cast<int>(w1 - w), sp.tiles - sp.tile);
       const int64_t head = static_cast<int64_t>(sp.b) * p.kvh + sp.h;
       bool taken = false;
-      if ((sp.tile + nt) * kTcTile > sp.len)
-        tree_masks(p, sp.b, sp.n, sp.rb * N + r0, RW, mask, lane);
       // Q into its swizzled chunks (the last scores of the segment before have been
-      // read, so its MMAs are done), all loads in flight together; rows past the
-      // block are zeros
+      // read, so its MMAs are done), all loads in flight together and with the masks; rows
+      // past the block are zeros
       {
         constexpr int U = D / 8, NQ = N * U / kSoft;  // 16-byte units per row / thread
         uint4 v[NQ];
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
           const int r = (tid + i * kSoft) / U, x = (tid + i * kSoft) % U;
-          const int rr = sp.rb * N + r, t = rr / p.G;
+          const int rr = sp.rb * N + r, t = over_g(p, rr);
           const T* qp = static_cast<const T*>(p.q) + sp.b * p.qb + t * p.qt +
                         (static_cast<int64_t>(sp.h) * p.G + (rr - t * p.G)) * p.qh;
           v[i] = r < sp.rows ? __ldg(reinterpret_cast<const uint4*>(qp) + x)
                              : make_uint4(0, 0, 0, 0);
         }
+        if ((sp.tile + nt) * kTcTile > sp.len)
+          tree_masks(p, sp.b, sp.n, sp.rb * N + r0, RW, mask, lane);
         if constexpr (Q8) {
           // f16, each row scaled by a power of two (undone by srow); the row's U units
           // lie in U neighbouring lanes
@@ -1095,9 +1122,9 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
-      float l[RW];
+      float l[SUM ? 1 : RW];
 #pragma unroll
-      for (int i = 0; i < RW; ++i) l[i] = 0.0f;
+      for (int i = 0; i < (SUM ? 1 : RW); ++i) l[i] = 0.0f;
       // the scales of this thread's key, loaded two tiles ahead
       float ks_next[2], vs_next[2];
       auto load_scales = [&](int t, int slot) {
@@ -1116,12 +1143,12 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
         const bool tail = (sp.tile + t + 1) * kTcTile > sp.len, first = t == 0;
         // the rows that see this key, as bits: all of a context key, of a drafted one those
         // whose token's set holds it
-        unsigned long long seen = ~0ull;
+        uint32_t seen = ~0u;
         if (tail && at >= 0) {
-          seen = 0ull;
+          seen = 0u;
           if (at < sp.n)
 #pragma unroll 8
-            for (int i = 0; i < RW; ++i) seen |= (mask[i] >> at & 1ull) << i;
+            for (int i = 0; i < RW; ++i) seen |= static_cast<uint32_t>(mask[i] >> at & 1ull) << i;
         }
         float ksc = 1.0f, vsc = 1.0f, lvs = 0.0f;
         if constexpr (Q8) {
@@ -1134,13 +1161,13 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
         }
         bool got = wait_warp(s_full + (it & 1), (it >> 1) & 1);
         tc_fence_after();
-        auto scores = [&](int c, uint32_t (&s)[32]) {
-          tmem_ld_32x32b_x32(tmem + (it & 1) * N + lane_off + r0 + c * 32, s);
+        auto scores = [&](uint32_t (&s)[32]) {
+          tmem_ld_32x32b_x32(tmem + (it & 1) * N + lane_off + r0, s);
           tmem_wait_ld_tie(s);
           if constexpr (Q8) {  // the row's factor, then the key's (last where nothing is masked)
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              const float4 y = *reinterpret_cast<const float4*>(srow + r0 + c * 32 + i);
+              const float4 y = *reinterpret_cast<const float4*>(srow + r0 + i);
               const float y4[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
               for (int x = 0; x < 4; ++x) {
@@ -1150,30 +1177,41 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
             }
           }
           if (tail) {
-            const uint32_t bits = static_cast<uint32_t>(seen >> (32 * c));
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (!(bits >> i & 1u)) s[i] = __float_as_uint(-INFINITY);
+              if (!(seen >> i & 1u)) s[i] = __float_as_uint(-INFINITY);
           }
-        };  // scores of 32 rows
+        };
         if (!Q8 && tail && got && sw < 4) {  // this thread's V row, once it has landed
           const int slot = 2 * it + 1;
           got = wait_warp(full + slot % NS, (slot / NS) & 1);
           if (got && at >= 0) {
             uint8_t* tv = smem + S::kOffRing + (slot % NS) * S::kTile;
-#pragma unroll 4
-            for (int u = 0; u < D / 8; ++u)
-              taken |= clean_unit<T>(tv + (u >> 3) * kTcTile * 128 + kt * 128 +
-                                         (((u & 7) ^ (kt & 7)) << 4), at >= sp.n);
+            auto unit = [&](int u) {
+              return tv + (u >> 3) * kTcTile * 128 + kt * 128 + (((u & 7) ^ (kt & 7)) << 4);
+            };
+            if (at >= sp.n) {
+#pragma unroll
+              for (int u = 0; u < D / 8; ++u)
+                *reinterpret_cast<uint4*>(unit(u)) = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+              uint32_t any = 0u;
+#pragma unroll
+              for (int u = 0; u < D / 8; ++u)
+                any |= non_finite_in<T>(*reinterpret_cast<const uint4*>(unit(u)));
+              if (any != 0u)
+#pragma unroll 1
+                for (int u = 0; u < D / 8; ++u) taken |= clean_unit<T>(unit(u), false);
+            }
           }
         }
-        // ---- does a score pass its row's reference by more than the margin?  With 32 rows
-        // the exponentials are taken at once and looked at afterwards
+        // ---- does a score pass its row's reference by more than the margin?  The
+        // exponentials are taken at once and looked at afterwards
         const float unit = !Q8 ? p.sl2 : tail ? 1.0f : ksc;  // scores to log2 units
-        auto expo = [&](uint32_t (&x)[32], int c) {
+        auto expo = [&](uint32_t (&x)[32]) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            const float4 nr = *reinterpret_cast<const float4*>(nref + r0 + c * 32 + i);
+            const float4 nr = *reinterpret_cast<const float4*>(nref + r0 + i);
             const float n4[4] = {nr.x, nr.y, nr.z, nr.w};
 #pragma unroll
             for (int y = 0; y < 4; ++y)
@@ -1200,53 +1238,33 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
           }
           return top;
         };
-        uint32_t e[32];  // NC == 1: the tile's exponentials
+        uint32_t e[32];
         // int8: always where drafted keys are, so that no row's result hangs on the scales of
         // keys that it does not see
         bool need = first || !got || (Q8 && tail);
         if (!need) {
           float top = -INFINITY;
-          if constexpr (NC == 1) {
-            scores(0, e);
-            expo(e, 0);
+          scores(e);
+          expo(e);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(e[i]));
-            if constexpr (Q8) top = fmaxf(top, weigh(e));
-            need = top > kTMost;
-          } else {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-              uint32_t s[32];
-              scores(c, s);
-#pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                const float4 nr = *reinterpret_cast<const float4*>(nref + r0 + c * 32 + i);
-                top = fmaxf(top, fmaxf(fmaf(__uint_as_float(s[i]), p.sl2, nr.x),
-                                       fmaf(__uint_as_float(s[i + 1]), p.sl2, nr.y)));
-                top = fmaxf(top, fmaxf(fmaf(__uint_as_float(s[i + 2]), p.sl2, nr.z),
-                                       fmaf(__uint_as_float(s[i + 3]), p.sl2, nr.w)));
-              }
-            }
-            need = top > kTRaise;
-          }
+          for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(e[i]));
+          if constexpr (Q8) top = fmaxf(top, weigh(e));
+          need = top > kTMost;
         }
         if (soft_any<kSoft>(need)) {
           if (got) {
+            uint32_t s[32];
+            scores(s);
+            float v[32];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-              uint32_t s[32];
-              scores(c, s);
-              float v[32];
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(s[i]) * unit;
+            if constexpr (Q8) {
+              float x[32];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(s[i]) * unit;
-              if constexpr (Q8) {
-                float x[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) x[i] = v[i] + lvs;
-                smax[(4 + q4) * N + r0 + c * 32 + lane] = across_lanes<false>(x, lane);
-              }
-              smax[q4 * N + r0 + c * 32 + lane] = across_lanes<false>(v, lane);
+              for (int i = 0; i < 32; ++i) x[i] = v[i] + lvs;
+              smax[(4 + q4) * N + r0 + lane] = across_lanes<false>(x, lane);
             }
+            smax[q4 * N + r0 + lane] = across_lanes<false>(v, lane);
           }
           if (lane == 0) wait_ok[sw] = got;
           soft_sync<kSoft>();
@@ -1280,54 +1298,50 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
           // runs out, the next vote ends the segment)
           if (!first && wait_pv(it - 1)) {
             tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
+            auto rescale = [&](uint32_t at, const float* by) {
               uint32_t ov[32];
-              tmem_ld_32x32b_x32(tO + lane_off + r0 + c * 32, ov);
+              tmem_ld_32x32b_x32(at + lane_off + r0, ov);
               tmem_wait_ld_tie(ov);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float f = fact[r0 + c * 32 + i];
-                const float fo = Q8 ? facto[r0 + c * 32 + i] : f;
-                ov[i] = __float_as_uint(__uint_as_float(ov[i]) * fo);
-                l[c * 32 + i] *= f;
-              }
-              tmem_st_32x32b_x32(tO + lane_off + r0 + c * 32, ov);
+              for (int i = 0; i < 32; ++i)
+                ov[i] = __float_as_uint(__uint_as_float(ov[i]) * by[r0 + i]);
+              tmem_st_32x32b_x32(at + lane_off + r0, ov);
+            };
+            rescale(tO, Q8 ? facto : fact);
+            if constexpr (!SUM) {
+#pragma unroll
+              for (int i = 0; i < RW; ++i) l[i] *= fact[r0 + i];
+            } else if (D == 128 && q4 == 0) {
+              rescale(tL, fact);
             }
             tmem_wait_st();
           }
-          if constexpr (NC == 1) {
-            scores(0, e);
-            expo(e, 0);
-            if constexpr (Q8) weigh(e);
-          }
+          scores(e);
+          expo(e);
+          if constexpr (Q8) weigh(e);
         }
-        // ---- probabilities, their sums, and P (16 bits, this key's row)
+        // ---- P: 16 bits, this key's row
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free + (it & 1));  // S may be overwritten
+        if constexpr (!SUM) {
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          if constexpr (NC > 1) scores(c, e);
-          if (c == NC - 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_free + (it & 1));  // S may be overwritten
-          }
-          if constexpr (NC > 1) expo(e, c);
+          for (int i = 0; i < 32; ++i) l[i] += __uint_as_float(e[i]);
+        }
+        if constexpr (!Q8) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float a = __uint_as_float(e[i]), b = __uint_as_float(e[i + 1]);
-            l[c * 32 + i] += a;
-            l[c * 32 + i + 1] += b;
-            if constexpr (!Q8) pk[i / 2] = pack16<std::is_same<T, __nv_bfloat16>::value>(a, b);
-          }
-          // this P buffer is free once the tile that was in it has been contracted
-          if (c == 0 && it >= PB) wait_pv(it - PB);
+          for (int i = 0; i < 32; i += 2)
+            pk[i / 2] = pack16<std::is_same<T, __nv_bfloat16>::value>(__uint_as_float(e[i]),
+                                                                      __uint_as_float(e[i + 1]));
+        }
+        // this P buffer is free once the tile that was in it has been contracted
+        if (it >= PB) wait_pv(it - PB);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int u = (r0 + c * 32) / 8 + x;
-            *reinterpret_cast<uint4*>(smem + S::kOffP + (it % PB) * S::kPOne + (u >> 3) * S::kPChunk +
-                                      kt * 128 + (((u & 7) ^ (kt & 7)) << 4)) =
-                make_uint4(pk[4 * x], pk[4 * x + 1], pk[4 * x + 2], pk[4 * x + 3]);
-          }
+        for (int x = 0; x < 4; ++x) {
+          const int u = r0 / 8 + x;
+          *reinterpret_cast<uint4*>(smem + S::kOffP + (it % PB) * S::kPOne + (u >> 3) * S::kPChunk +
+                                    kt * 128 + (((u & 7) ^ (kt & 7)) << 4)) =
+              make_uint4(pk[4 * x], pk[4 * x + 1], pk[4 * x + 2], pk[4 * x + 3]);
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -1336,41 +1350,45 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
       }
       if (!ok) break;
       // ---- the segment's partial
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        float v[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = l[c * 32 + i];
-        smax[q4 * N + r0 + c * 32 + lane] = across_lanes<true>(v, lane);
-      }
+      if constexpr (!SUM) smax[q4 * N + r0 + lane] = across_lanes<true>(l, lane);
       if constexpr (Q8) {  // O back to the scores' own reference
         if (tid < N) smax[4 * N + tid] = eref[tid] == -INFINITY ? 0.0f : ex2_approx(eref[tid] + nref[tid]);
       }
-      const bool any_taken = soft_any<kSoft>(taken);
       ok = wait_pv(it - 1);
+      if constexpr (SUM) {  // the ones' rows, alike in every lane
+        if (ok && q4 == (D == 128 ? 0 : 2)) {
+          tc_fence_after();
+          uint32_t lv[32];
+          tmem_ld_32x32b_x32((D == 128 ? tL : tO) + lane_off + r0, lv);
+          tmem_wait_ld_tie(lv);
+          float x = __uint_as_float(lv[0]);
+#pragma unroll
+          for (int i = 1; i < 32; ++i) x = lane == i ? __uint_as_float(lv[i]) : x;
+          smax[r0 + lane] = x;
+        }
+      }
+      const bool any_taken = soft_any<kSoft>(taken);
       if (ok) {
         tc_fence_after();
         const int64_t item = head * p.nrb + sp.rb;
         float* pp = p.part + (static_cast<int64_t>(blockIdx.x) + item) * N * part_stride<D>();
         if (tid < sp.rows) {
           float* row = pp + tid * part_stride<D>();
-          const float sum = (smax[tid] + smax[N + tid]) + (smax[2 * N + tid] + smax[3 * N + tid]);
+          const float sum = SUM ? smax[tid]
+                                : (smax[tid] + smax[N + tid]) + (smax[2 * N + tid] + smax[3 * N + tid]);
           row[D] = sum == 0.0f ? -INFINITY : -nref[tid];  // a row that sees nothing here
           row[D + 1] = sum;
           row[D + 2] = any_taken ? 1.0f : 0.0f;
         }
         if (D == 128 || q4 < 2) {  // thread = output dim
+          uint32_t ov[32];
+          tmem_ld_32x32b_x32(tO + lane_off + r0, ov);
+          tmem_wait_ld_tie(ov);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            uint32_t ov[32];
-            tmem_ld_32x32b_x32(tO + lane_off + r0 + c * 32, ov);
-            tmem_wait_ld_tie(ov);
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (r0 + c * 32 + i < sp.rows)
-                pp[(r0 + c * 32 + i) * part_stride<D>() + kt] =
-                    __uint_as_float(ov[i]) * (Q8 ? smax[4 * N + r0 + c * 32 + i] : 1.0f);
-          }
+          for (int i = 0; i < 32; ++i)
+            if (r0 + i < sp.rows)
+              pp[(r0 + i) * part_stride<D>() + kt] =
+                  __uint_as_float(ov[i]) * (Q8 ? smax[4 * N + r0 + i] : 1.0f);
         }
         tc_fence_before();
       }
@@ -1446,7 +1464,7 @@ __global__ void __launch_bounds__(32 * kCWarps) tree_combine_kernel(const TreePa
   __shared__ uint32_t base[kScanWords];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   grid_release();
-  if (warp == 0) tree_scan(p, base, lane);
+  if (warp == 0) tree_scan<0, 0>(p, base, lane);
   __syncthreads();
   const uint32_t total = base[p.B];
   const uint32_t shares = min(total, static_cast<uint32_t>(p.grid));
@@ -1470,7 +1488,7 @@ __global__ void __launch_bounds__(32 * kCWarps) tree_combine_kernel(const TreePa
   for (int i = 0; i < DL; ++i) acc[i] = 0.0f;
   grid_wait();  // the partials are complete
   if (t < n) {
-    const int rb = r / p.rb, tiles = tiles_of(p, len, n), nrb = row_blocks(p, n);
+    const int rb = r / p.rb, tiles = tiles_of<0>(p, len, n), nrb = row_blocks<0>(p, n);
     const uint32_t t0 = base[b] + (static_cast<uint32_t>(h) * nrb + rb) * tiles;
     const uint32_t c0 = share_of(t0, total, shares), c1 = share_of(t0 + tiles - 1, total, shares);
     const int64_t item = static_cast<int64_t>(bh) * p.nrb + rb;
@@ -1654,6 +1672,7 @@ extern "C" ltm_status ltm_tree_attention(
     p.oh = o_strides[2];
     p.T = T;
     p.G = G;
+    p.inv_g = 1.0f / static_cast<float>(G);
     p.kvh = kv_heads;
     p.P = max_positions;
     p.sl2 = 1.4426950408889634f / sqrtf(static_cast<float>(head_dim));
