@@ -148,12 +148,17 @@ __device__ __forceinline__ void tree_scan(const TreeParams& p, uint32_t* base, i
 
 // The list is shared by min(grid, total) CTAs, so that no share is empty: the
 // partials of a head are those of consecutive CTAs.
-__device__ __forceinline__ uint32_t share_start(uint32_t c, uint32_t total, uint32_t grid) {
-  return static_cast<uint32_t>(static_cast<uint64_t>(c) * total / grid);
-}
-__device__ __forceinline__ uint32_t share_of(uint32_t tile, uint32_t total, uint32_t grid) {
-  return static_cast<uint32_t>((static_cast<uint64_t>(tile + 1) * grid - 1) / total);
-}
+// The first total % shares of them take a tile more than the others.
+struct Shares {
+  uint32_t each, more;
+  __device__ __forceinline__ Shares(uint32_t total, uint32_t shares)
+      : each(shares ? total / shares : 0u), more(total - each * shares) {}
+  __device__ __forceinline__ uint32_t start(uint32_t c) const { return c * each + min(c, more); }
+  __device__ __forceinline__ uint32_t of(uint32_t tile) const {
+    const uint32_t head = more * (each + 1);
+    return tile < head ? tile / (each + 1) : more + (tile - head) / each;
+  }
+};
 
 // Where tile w of the list lies.
 struct TreeSpan {
@@ -412,8 +417,8 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
   const uint32_t total = base[p.B];
   const uint32_t shares = min(total, gridDim.x);
   if (blockIdx.x >= shares) return;
-  const uint32_t w0 = share_start(blockIdx.x, total, shares);
-  const uint32_t w1 = share_start(blockIdx.x + 1, total, shares);
+  const Shares share(total, shares);
+  const uint32_t w0 = share.start(blockIdx.x), w1 = share.start(blockIdx.x + 1);
 
   if (warp == 0) {
     // ---- producer: K(0), V(0), K(1), ... into the ring
@@ -944,8 +949,9 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
   const uint32_t shares = min(total, gridDim.x);
   uint32_t w0 = 0, w1 = 0;  // no tiles: every role falls through to the end
   if (blockIdx.x < shares) {
-    w0 = share_start(blockIdx.x, total, shares);
-    w1 = share_start(blockIdx.x + 1, total, shares);
+    const Shares share(total, shares);
+    w0 = share.start(blockIdx.x);
+    w1 = share.start(blockIdx.x + 1);
   }
 
   if (warp == 0) {
@@ -1490,7 +1496,8 @@ __global__ void __launch_bounds__(32 * kCWarps) tree_combine_kernel(const TreePa
   if (t < n) {
     const int rb = r / p.rb, tiles = tiles_of<0>(p, len, n), nrb = row_blocks<0>(p, n);
     const uint32_t t0 = base[b] + (static_cast<uint32_t>(h) * nrb + rb) * tiles;
-    const uint32_t c0 = share_of(t0, total, shares), c1 = share_of(t0 + tiles - 1, total, shares);
+    const Shares share(total, shares);
+    const uint32_t c0 = share.of(t0), c1 = share.of(t0 + tiles - 1);
     const int64_t item = static_cast<int64_t>(bh) * p.nrb + rb;
     const float* pr = p.part + ((c0 + item) * p.rb + (r - rb * p.rb)) * part_stride<D>();
     bool taken = false;
