@@ -39,13 +39,17 @@
 //   test, its scales and the clean-up of rows past the end are its own.  int8 codes
 //   become f16 tiles in shared memory first.
 //
-// Measured, cold caches, contexts of equal length.  Read-bound: 16-bit, one row per
-// head of 128 dims, 32 x 8 heads x 16384 positions 0.46 ms (7.0 TB/s); int8, one row,
-// 0.52 ms for 3.2 GB (6.4 TB/s; 5.5 TB/s once the clock has dropped under load).  int8
-// conversions bound 9 to 16 rows (4.1 TB/s, 128 dims; tcgen05's blocks of 32 rows reach
-// 2.7).  tree_tc_kernel is bound by its softmax: 1.0, 1.2 and 2.05 us per tile of 128
-// positions with 32, 64 and 128 rows of 64 dims (int8: 1.25 and 1.66; 128 dims 1.8 and
-// 2.45), where reading a 16-bit tile takes 0.7 us of 64 dims, 1.4 of 128.
+// Measured (bf16 queries, calls back to back).  Read-bound: one row per head of 128 dims
+// over a 16-bit cache, 16 x 32 heads x 8192 to 16384 positions, 0.46 ms for 3.2 GB (6.9
+// TB/s); int8, 64 x 32 heads x 4096 to 8192, 0.51 ms for 3.3 GB, 0.60 once the clock has
+// dropped under load (5.6 TB/s).  The int8 conversions bound 9 to 16 rows (8 x 32
+// heads x 16384 positions of 128 dims 0.26 ms, 4.1 TB/s).  tree_tc_kernel reads a 16-bit
+// tile of 128 positions in 0.7 us (64 dims) or 1.4 us (128 dims); with 32, 64 and 128 rows it
+// takes 0.98, 1.26 and 1.84 us for 64 dims, 1.40, 1.45 and 2.2 us for 128: up to 64 rows of
+// 128 dims are read-bound, the others bound by the softmax's latencies (exponentials,
+// votes, barriers).  int8: 1.25 and 1.66 us for 32 and 64 rows of 64 dims, 1.8 and 2.45 us
+// for 128.  A segment's start and end cost 7 to 9 us (half of it queries, masks and the
+// tail's clean-up; 13 before those were overlapped and rid of divisions).
 //
 // In both, a row's reference maximum is only raised when a score exceeds it by more
 // than 2^8.  A non-finite value of a drafted token must not
@@ -872,11 +876,15 @@ __device__ __forceinline__ void soft_sync() {
 
 // warp 0: TMA producer (K(0), V(0), K(1), ... into the ring); warp 1: TMEM and
 // the MMAs, in the order S(0), S(1), O(0), S(2), O(1), ... within a head's
-// segment; warps 4-7 (and 8-11 for the upper half of 64 or 128 rows): softmax,
-// thread = key = TMEM lane.  TMEM: S^T twice, O^T.  With 128 rows the softmax reads its
-// 64 rows of S twice, 32 at a time (for the vote, then for the exponentials).  int8
-// caches: warps 2, 3 (and the last two) turn the codes into f16 tiles (exact); a thread's key
-// has its K scale on the scores and its V scale on the probabilities, as in tree_mma_kernel.
+// segment; from warp 4 on, four warps for every 32 rows: softmax, thread = key = TMEM
+// lane, a tile's 32 exponentials in registers.  TMEM: S^T twice, O^T.  With 128 rows that
+// leaves a thread 96 registers, too few for its 32 sums as well: they are those of P's
+// 16-bit values, contracted with ones (rows 64-127 of O^T for 64 dims, an accumulator of
+// their own for 128), which saves reading S twice: 27 tokens of 4 heads a cached head,
+// 55 -> 50 us.  (Up to 64 rows the sums stay in fp32 registers: contracting them cost 5%.)
+// int8 caches: warps 2, 3 (and the last two) turn the codes into f16 tiles (exact); a thread's
+// key has its K scale on the scores and its V scale on the probabilities, as in
+// tree_mma_kernel.
 template <class T, int D, int N, bool Q8>
 __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
