@@ -109,6 +109,27 @@ __device__ __noinline__ uint4 cut_vector(const T* r, int x, int c0, int c1) {
   return *reinterpret_cast<const uint4*>(e);
 }
 
+// Ranks of n values by counting those before each, by the whole CTA; up to 32 lanes share
+// one value's comparisons (the comparisons of one thread after the other would be most of
+// a short list's time).
+template <class Get, class Before, class Put>
+__device__ __forceinline__ void rank_in_place(int n, Get&& get, Before&& before, Put&& put) {
+  int g = 1;
+  while (g < 32 && 2 * g * n <= kBThreads) g *= 2;
+  const int tid = threadIdx.x, sub = tid & (g - 1), own = tid / g;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += kBThreads / g) {
+    const int i = i0 + own;
+    const auto x = get(i < n ? i : n - 1);
+    int rank = 0;
+#pragma unroll 4
+    for (int j = sub; j < n; j += g) rank += before(get(j), x);
+#pragma unroll 1
+    for (int o = g / 2; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (sub == 0 && i < n) put(rank, x);
+  }
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct BeamPartial {
@@ -269,13 +290,11 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 && PER == kPer ? 4 :
   __syncthreads();
   const int n = s_count;
   if (n <= kMaxCand) {
-    for (int i = tid; i < n; i += kBThreads) {
-      const uint64_t mine = s_cand[i];
-      int rank = 0;
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) rank += s_cand[j] > mine;
-      if (rank < K) list[rank] = mine;
-    }
+    rank_in_place(
+        n, [&](int i) { return s_cand[i]; }, [](uint64_t a, uint64_t b) { return a > b; },
+        [&](int rank, uint64_t x) {
+          if (rank < K) list[rank] = x;
+        });
     for (int i = n + tid; i < K; i += kBThreads) list[i] = 0ull;
     return;
   }
@@ -414,14 +433,12 @@ __global__ void __launch_bounds__(kBThreads)
     if (out_done) out_done[o] = s_done[w] || tok == end;
   };
   auto rank_all = [&](int n) {
-#pragma unroll 1
-    for (int i = tid; i < n; i += kBThreads) {
-      const Total x = s_cand[i];
-      int rank = 0;
-#pragma unroll 2
-      for (int j = 0; j < n; ++j) rank += before(s_cand[j], x);
-      if (rank < K) put(rank, x);
-    }
+    rank_in_place(
+        n, [&](int i) { return s_cand[i]; },
+        [](const Total& a, const Total& b) { return before(a, b); },
+        [&](int rank, const Total& x) {
+          if (rank < K) put(rank, x);
+        });
   };
   if (all) {
     if (tid < entries) s_cand[tid] = total(tid / K, own);
