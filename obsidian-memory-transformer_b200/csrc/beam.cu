@@ -9,7 +9,7 @@
 // is NaN counts as -inf.
 //
 // Every logit is read once (the bound): beam_chunk_kernel gives each CTA up to
-// 8192 logits of one row, held in registers.  It takes the chunk's maximum, the
+// 8192 or 16384 logits of one row, held in shared memory.  It takes the chunk's maximum, the
 // sum of exponentials, and its K best by filtering: the smallest of n >= K group
 // maxima is a value that at least K logits reach, and usually few more do (about
 // n (1 + 1/2 + ... + 1/n) for n groups, 22 for 8), so only those are compacted and ranked.
@@ -97,16 +97,20 @@ __device__ __forceinline__ uint4 vec_none() {  // -inf everywhere
   return make_uint4(k, k, k, k);
 }
 
-// The vector of logits x .. x + N - 1 of a row, -inf for those outside [c0, c1).  Not
-// inlined: at most two threads of a chunk need it.
+// A 16-byte vector of shared memory with -inf at the elements whose token, t0 for the
+// first, lies outside [c0, c1).
 template <class T>
-__device__ __noinline__ uint4 cut_vector(const T* r, int x, int c0, int c1) {
+__device__ __noinline__ void cut_vector(uint4* v, int t0, int c0, int c1) {
   constexpr int N = 16 / sizeof(T);
-  T e[N];
-#pragma unroll
+  T* e = reinterpret_cast<T*>(v);
+#pragma unroll 1
   for (int j = 0; j < N; ++j)
-    e[j] = x + j >= c0 && x + j < c1 ? r[x + j] : from_f32<T>(-INFINITY);
-  return *reinterpret_cast<const uint4*>(e);
+    if (t0 + j < c0 || t0 + j >= c1) e[j] = from_f32<T>(-INFINITY);
+}
+
+__device__ __forceinline__ void copy_vector(uint4* dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src)
+               : "memory");
 }
 
 // Ranks of n values by counting those before each, by the whole CTA; up to 32 lanes share
@@ -138,20 +142,24 @@ struct BeamPartial {
 
 // Workspace: [rows, nchunk] BeamPartial, then [rows, nchunk, K] sorted keys
 // (ordered logit << 32 | ~token; 0 = none).
+//
+// The chunk stays in shared memory (16-byte vectors of the row's aligned span; a thread
+// copies and works through its own, tid + i * 256), so that a thread needs few registers
+// and five CTAs share an SM: their loads, exponentials and filters overlap.
 template <class T, int PER>
-__global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 && PER == kPer ? 4 : 3)
+__global__ void __launch_bounds__(kBThreads, 5)
     beam_chunk_kernel(const T* __restrict__ logits, int64_t ldb, int64_t ldw,
                       const float* __restrict__ scores, const uint8_t* __restrict__ done, int end,
                       int W, int V, int K, int nchunk, int groups, BeamPartial* __restrict__ stats,
                       uint64_t* __restrict__ lists) {
   constexpr int N = 16 / sizeof(T);  // logits per vector
   constexpr int NV = PER / N;        // vectors per thread
-  constexpr int kChunk = kBThreads * PER;
+  constexpr int kChunk = kBThreads * PER, kVecs = kBThreads * NV;
+  __shared__ uint4 s_x[kVecs + 1];  // a misaligned chunk takes one vector more: thread 0's
   __shared__ float s_group[kBThreads];
   __shared__ float s_sum[kBThreads / 32];
   __shared__ uint64_t s_cand[kMaxCand];
   __shared__ uint64_t s_best[kBThreads / 32];
-  __shared__ uint4 s_slot[kBThreads * NV];  // vectors of the threads that hold candidates
   __shared__ int s_owner[kBThreads];
   __shared__ int s_count, s_slots;
   grid_wait();
@@ -163,21 +171,25 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 && PER == kPer ? 4 :
   const int64_t item = blockIdx.x;
   uint64_t* list = lists + item * K;
 
-  // ---- load: 16-byte vectors of the row's aligned span, all in flight at once; then the
-  // vectors that the chunk's ends cut, element by element (-inf where there is none:
-  // such elements are left out by their index below)
-  const T* r = logits + b * ldb + w * ldw;
-  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
-  // token of element j of vector i: t0 + i * 256 * N + j
-  const int t0 = c0 - shift + tid * N;
-  uint4 raw[NV];
+  // ---- load: whole vectors, in the first and last also what lies beside the chunk (it is
+  // in the same 16 bytes as logits of it), which is cut away afterwards
+  const uintptr_t at = reinterpret_cast<uintptr_t>(logits + b * ldb + w * ldw + c0);
+  const uint8_t* src = reinterpret_cast<const uint8_t*>(at & ~static_cast<uintptr_t>(15));
+  const int shift = static_cast<int>((at & 15) / sizeof(T));
+  const int t0 = c0 - shift;  // token of element 0
+  const int nvec = (c1 - t0 + N - 1) / N;
+  const bool more = tid == 0 && nvec > kVecs;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int x = t0 + i * kBThreads * N;
-    if (x >= c0 && x + N <= c1) raw[i] = __ldg(reinterpret_cast<const uint4*>(r + x));
+    const int v = tid + i * kBThreads;
+    if (v < nvec) copy_vector(s_x + v, src + v * 16);
+    else s_x[v] = vec_none<T>();
   }
+  if (more) copy_vector(s_x + kVecs, src + kVecs * 16);
+  asm volatile("cp.async.commit_group;" ::: "memory");
   const float score = scores[row];
   const bool is_done = done != nullptr && done[row] != 0;
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (is_done || !(score > -INFINITY)) {
     // no logit matters: the end token (if this chunk has it), then the lowest tokens
     const bool has = is_done && score > -INFINITY && end >= c0 && end < c1;
@@ -198,27 +210,20 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 && PER == kPer ? 4 :
     return;
   }
   if (tid == 0) s_count = s_slots = 0;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int x = t0 + i * kBThreads * N;
-    if (!(x >= c0 && x + N <= c1)) {
-      raw[i] = vec_none<T>();
-      if (x < c1 && x + N > c0) raw[i] = cut_vector<T>(r, x, c0, c1);
-    }
-  }
-  // a misaligned row's last `shift` logits lie past the vectors: one per thread
-  const int xe = c0 - shift + kChunk + tid;
-  const bool has_extra = tid < shift && xe < c1;
-  float extra = has_extra ? to_f32(r[xe]) : -INFINITY;
+  if (tid == 0 && shift > 0) cut_vector<T>(s_x, t0, c0, c1);
+  if (more) cut_vector<T>(s_x + kVecs, t0 + kVecs * N, c0, c1);
+  else if ((nvec - 1) % kBThreads == tid && nvec <= kVecs)
+    cut_vector<T>(s_x + nvec - 1, t0 + (nvec - 1) * N, c0, c1);
 
   // Maximum, bound and sum.  The first pass takes the logits as they are; a NaN
   // or +inf among them makes the sum a NaN, and they are replaced before a second.
   float m, tau, tm;
   while (true) {
-    tm = extra;
-    uint4 vm = raw[0];
+    uint4 vm = s_x[tid];
 #pragma unroll
-    for (int i = 1; i < NV; ++i) vm = vec_max<T>(vm, raw[i]);
+    for (int i = 1; i < NV; ++i) vm = vec_max<T>(vm, s_x[tid + i * kBThreads]);
+    if (more) vm = vec_max<T>(vm, s_x[kVecs]);
+    tm = -INFINITY;
     {
       const T* e = reinterpret_cast<const T*>(&vm);
 #pragma unroll
@@ -239,38 +244,52 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 && PER == kPer ? 4 :
     m = unordered(__reduce_max_sync(0xffffffffu, ordered(fmaxf(g0, g1))));
     tau = unordered(__reduce_min_sync(0xffffffffu, ordered(fminf(g0, g1))));
     const float ref = m == -INFINITY ? 0.0f : m;
-    float sum = ex2_approx((extra - ref) * kLog2e);
+    const uint64_t ref2 = f2_pack(ref, ref), log2e2 = f2_pack(kLog2e, kLog2e);
+    uint64_t sum2 = 0ull;  // two sums
+    auto add = [&](const uint4& v) {
+      const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const T* e = reinterpret_cast<const T*>(&raw[i]);
+      for (int j = 0; j < N; j += 2) {
+        float x0, x1;
+        f2_unpack(f2_mul(f2_sub(f2_pack(to_f32(e[j]), to_f32(e[j + 1])), ref2), log2e2), x0, x1);
+        sum2 = f2_add(sum2, f2_pack(ex2_approx(x0), ex2_approx(x1)));
+      }
+    };
 #pragma unroll
-      for (int j = 0; j < N; ++j) sum += ex2_approx((to_f32(e[j]) - ref) * kLog2e);
-    }
+    for (int i = 0; i < NV; ++i) add(s_x[tid + i * kBThreads]);
+    if (more) add(s_x[kVecs]);
+    float sum, odd;
+    f2_unpack(sum2, sum, odd);
+    sum += odd;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_sum[warp] = sum;
     if (!__syncthreads_or(sum != sum)) break;
-    extra = logit_value<T>(extra);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      T* e = reinterpret_cast<T*>(&raw[i]);
-#pragma unroll
+    auto replace = [&](uint4* v) {
+      T* e = reinterpret_cast<T*>(v);
+#pragma unroll 1
       for (int j = 0; j < N; ++j) e[j] = from_f32<T>(logit_value<T>(to_f32(e[j])));
-    }
+    };
+#pragma unroll 1
+    for (int i = 0; i < NV; ++i) replace(s_x + tid + i * kBThreads);
+    if (more) replace(s_x + kVecs);
   }
-  // ---- the threads that hold a value at the bound hand theirs to the whole CTA
+  // ---- the threads that hold a value at the bound: their vectors, by the whole CTA
   auto offer = [&](float y, int x) {
     if (y >= tau && x >= c0 && x < c1) {
-      const int at = atomicAdd(&s_count, 1);
-      if (at < kMaxCand) s_cand[at] = list_key(y, x);
+      const int i = atomicAdd(&s_count, 1);
+      if (i < kMaxCand) s_cand[i] = list_key(y, x);
     }
   };
-  if (tm >= tau) {
-    const int at = atomicAdd(&s_slots, 1);
-    s_owner[at] = t0;
+  auto offer_vector = [&](int v) {
+    const uint4 x = s_x[v];
+    const T* e = reinterpret_cast<const T*>(&x);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) s_slot[at * NV + i] = raw[i];
-    if (has_extra) offer(extra, xe);
+    for (int j = 0; j < N; ++j) offer(to_f32(e[j]), t0 + v * N + j);
+  };
+  if (tm >= tau) {
+    s_owner[atomicAdd(&s_slots, 1)] = tid;
+    if (more) offer_vector(kVecs);
   }
   if (tid == 0) {
     float t = 0.0f;
@@ -279,46 +298,39 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 && PER == kPer ? 4 :
     stats[item] = BeamPartial{m, t};
   }
   __syncthreads();
-  const int nvec = s_slots * NV;
-  for (int i = tid; i < nvec; i += kBThreads) {
-    const uint4 v = s_slot[i];
-    const T* e = reinterpret_cast<const T*>(&v);
-    const int x = s_owner[i / NV] + (i % NV) * kBThreads * N;
-#pragma unroll
-    for (int j = 0; j < N; ++j) offer(to_f32(e[j]), x + j);
-  }
+  const int nown = s_slots * NV;
+#pragma unroll 1
+  for (int i = tid; i < nown; i += kBThreads)
+    offer_vector(s_owner[i / NV] + (i % NV) * kBThreads);
   __syncthreads();
   const int n = s_count;
   if (n <= kMaxCand) {
     rank_in_place(
-        n, [&](int i) { return s_cand[i]; }, [](uint64_t a, uint64_t b) { return a > b; },
+        n, [&](int i) { return s_cand[i]; }, [](uint64_t x, uint64_t y) { return x > y; },
         [&](int rank, uint64_t x) {
           if (rank < K) list[rank] = x;
         });
     for (int i = n + tid; i < K; i += kBThreads) list[i] = 0ull;
     return;
   }
-  // too many: the K best one after the other (each below the last one taken), from
-  // shared memory
-  uint4* mine = s_slot + tid * NV;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) mine[i] = raw[i];
+  // too many: the K best one after the other (each below the last one taken)
   uint64_t last = ~0ull;
 #pragma unroll 1
   for (int kk = 0; kk < K; ++kk) {
     uint64_t best = 0ull;
-    auto look = [&](float y, int x) {
-      const uint64_t full = list_key(y, x);
-      if (x >= c0 && x < c1 && full < last && full > best) best = full;
+    auto look = [&](int v) {
+      const uint4 q = s_x[v];
+      const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int x = t0 + v * N + j;
+        const uint64_t full = list_key(to_f32(e[j]), x);
+        if (x >= c0 && x < c1 && full < last && full > best) best = full;
+      }
     };
 #pragma unroll 1
-    for (int i = 0; i < NV; ++i) {
-      const uint4 v = mine[i];
-      const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-      for (int j = 0; j < N; ++j) look(to_f32(e[j]), t0 + i * kBThreads * N + j);
-    }
-    if (has_extra) look(extra, xe);
+    for (int i = 0; i < NV; ++i) look(tid + i * kBThreads);
+    if (more) look(kVecs);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
     __syncthreads();
