@@ -123,9 +123,11 @@ def test_tree_matches_reference(ltm, dt, cache, B, T, heads, kvh, d, lens):
 
 @pytest.mark.parametrize("dt,cache,T,G,d", [("bf16", "int8", 9, 2, 128), ("f16", "int8", 16, 4, 64),
                                            ("bf16", "int8", 64, 1, 64), ("f16", "int8", 11, 6, 128),
-                                           ("f16", "same", 8, 4, 128), ("bf16", "same", 40, 3, 64)])
+                                           ("f16", "same", 8, 4, 128), ("bf16", "same", 40, 3, 64),
+                                           ("f16", "same", 22, 4, 64), ("f16", "same", 25, 4, 128),
+                                           ("bf16", "same", 64, 4, 128), ("f16", "int8", 64, 2, 128)])
 def test_many_rows_over_a_long_context(ltm, dt, cache, T, G, d):
-    """18 to 120 rows per cached head with contexts cut over many CTAs: keys that grow
+    """18 to 256 rows per cached head with contexts cut over many CTAs: keys that grow
     towards the end (the references rise), V scales that span 2^6, query heads of very
     different sizes.  Scores have a deviation of at most 1, so that of a row's p * scale
     only those below 2^-14 of the largest (f16: 2^-25 off, not a relative 2^-11) make up
