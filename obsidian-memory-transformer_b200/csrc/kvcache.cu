@@ -84,12 +84,26 @@ struct RowQuant {
   uint32_t keep;     // all ones, or 0: zero codes
 };
 
+// Sum rounded down, two at a time.
+__device__ __forceinline__ uint64_t f2_add_down(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rm.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // Codes of four values of a row, in magnitudes (a) and signs (a byte of ones for each
 // negative value): the IEEE quotient q = RN(a / s) rounded half up, without a division.
 //
-// n = floor(a / s) or, just above an integer, one less, from an approximate reciprocal
-// (off by at most 2e-5); then the code is n + 1 where q >= c = n + 1/2, else n.  RN ties
-// to even and c is even, so q >= c iff a / s >= (c + c') / 2, c' the float below c:
+// 16-bit values: the product with the reciprocal, corrected once by its remainder, is the
+// quotient up to 2^-45, and floor((q - 1/2) + 1) the code (q - 1/2 is exact from 1/4 on;
+// below, the code is 0).  Compared on the CPU with the division for every mantissa of the
+// row's largest value, every smaller value down to 2^-8 of it, and reciprocals up to 2 units
+// in the last place off: all codes alike.
+//
+// fp32 values can come closer to a tie than that.  n = floor(a / s) or, just above an
+// integer, one less, from the reciprocal (off by at most 2e-5); then the code is n + 1
+// where q >= c = n + 1/2, else n.  RN ties to even and c is even, so q >= c iff
+// a / s >= (c + c') / 2, c' the float below c:
 //   w = (a - c s) + (a - c' s) >= 0 .
 // Near the threshold both differences are exact as fused multiply-adds for s >= 2^-97: a
 // and c s are multiples of 2^(e-24) (s in [2^e, 2^(e+1))) that differ by less than
@@ -98,25 +112,34 @@ struct RowQuant {
 // clamped to [0, 1], is the step.  Farther away the signs are certain.  c' is RN(c -
 // 2^-24 c): c is a power of two only as 1/2, otherwise 2^-24 c lies between half a unit
 // and one.
+//
 // (Dividing where the estimate is near a tie cost 250 us for a prompt of 4 x 8192 tokens,
 // 32 heads of 128: most warps of 16-bit rows hold a tie.)
+template <class T>
 __device__ __forceinline__ uint32_t quant4(const float (&a)[4], uint32_t neg, const RowQuant& r) {
   constexpr float kShift = 12582912.0f;  // 1.5 * 2^23: the sum's low byte is the integer
   constexpr float kBelow = 1.0f - 5.9604644775390625e-8f;  // 1 - 2^-24
-  const uint64_t shift2 = f2_pack(kShift, kShift), half2 = f2_pack(0.5f, 0.5f);
-  const uint64_t mhalf2 = f2_pack(-0.5f, -0.5f), below2 = f2_pack(kBelow, kBelow);
+  const uint64_t mhalf2 = f2_pack(-0.5f, -0.5f);
   float big[4];
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {
     const uint64_t a2 = f2_pack(a[i], a[i + 1]);
-    const uint64_t b = f2_add(f2_fma(a2, r.inv, mhalf2), shift2);
-    const uint64_t c = f2_add(f2_sub(b, shift2), half2);
-    float w0, w1;
-    f2_unpack(f2_add(f2_fma(c, r.ms, a2), f2_fma(f2_mul(c, below2), r.ms, a2)), w0, w1);
-    float s0, s1;
-    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(s0) : "f"(w0), "f"(r.up), "f"(1.0f));
-    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(s1) : "f"(w1), "f"(r.up), "f"(1.0f));
-    f2_unpack(f2_add(b, f2_pack(s0, s1)), big[i], big[i + 1]);
+    if constexpr (sizeof(T) == 2) {
+      const uint64_t q0 = f2_mul(a2, r.inv);
+      const uint64_t q = f2_fma(f2_fma(q0, r.ms, a2), r.inv, q0);
+      f2_unpack(f2_add_down(f2_add(q, mhalf2), f2_pack(kShift + 1.0f, kShift + 1.0f)), big[i],
+                big[i + 1]);
+    } else {
+      const uint64_t shift2 = f2_pack(kShift, kShift);
+      const uint64_t b = f2_add(f2_fma(a2, r.inv, mhalf2), shift2);
+      const uint64_t c = f2_add(f2_sub(b, shift2), f2_pack(0.5f, 0.5f));
+      const uint64_t below = f2_mul(c, f2_pack(kBelow, kBelow));
+      float w0, w1, s0, s1;
+      f2_unpack(f2_add(f2_fma(c, r.ms, a2), f2_fma(below, r.ms, a2)), w0, w1);
+      asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(s0) : "f"(w0), "f"(r.up), "f"(1.0f));
+      asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(s1) : "f"(w1), "f"(r.up), "f"(1.0f));
+      f2_unpack(f2_add(b, f2_pack(s0, s1)), big[i], big[i + 1]);
+    }
   }
   const uint32_t m =  // magnitudes, at most 127 each
       __byte_perm(__byte_perm(__float_as_uint(big[0]), __float_as_uint(big[1]), 0x0040),
@@ -255,7 +278,7 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 ? 4 : 2)
         float a[4];
         uint32_t neg;
         magnitudes<T>(raw[j], g, a, neg);
-        code[g] = quant4(a, neg, rq);
+        code[g] = quant4<T>(a, neg, rq);
       }
       if (tiny && s > 0.0f) {  // divided
 #pragma unroll
