@@ -33,7 +33,7 @@ namespace {
 constexpr int kWarps = 8;    // warps per CTA of the write and read kernels
 constexpr int kVals = 16;    // values of a row per lane
 constexpr int kRowsFly = 4;  // rows in flight per lane group (write)
-constexpr int kReadFly = 4;  // rows in flight per lane group (read)
+constexpr int kReadFly = 8;  // rows in flight per lane group (read)
 
 struct RowStrides {
   int64_t b, t, h;  // elements between batches, tokens, heads
@@ -316,14 +316,16 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 ? 4 : 2)
 }
 
 // Rows [first_b, first_b + n) of every head back as O values; positions
-// outside [0, min(P, len_b)) give zeros.  Bound by memory.  A lane holds 16 codes
-// (or 8 values of a 16-bit cache, copied).
+// outside [0, min(P, len_b)) give zeros.  Bound by memory.  A lane writes 16 bytes
+// (so that a warp's stores are contiguous) of the 4 or 8 codes, or the 8 values of a
+// 16-bit cache, that it holds of a row.
 template <class O, int D, bool Q8>
 __global__ void __launch_bounds__(kWarps * 32)
     cache_read_kernel(const void* __restrict__ cache, const float* __restrict__ scale, int64_t P,
                       const int* __restrict__ first, const int* __restrict__ lens, int heads,
                       int n, O* __restrict__ out) {
-  constexpr int V = Q8 ? 16 : 8;
+  constexpr int V = 16 / sizeof(O);
+  using Raw = std::conditional_t<!Q8, uint4, std::conditional_t<V == 8, uint2, uint32_t>>;
   constexpr int G = D / V;
   constexpr int RP = 32 / G;
   constexpr int ROWS = RP * kReadFly;
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int64_t p0 = first ? first[b] : 0;
   const int64_t end = lens ? min(P, static_cast<int64_t>(lens[b])) : P;
   const int sub = lane / G, gl = lane % G;
-  uint4 raw[kReadFly];
+  Raw raw[kReadFly];
   float s[kReadFly];
 #pragma unroll
   for (int j = 0; j < kReadFly; ++j) {
@@ -345,9 +347,9 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int64_t p = p0 + i;
     const bool live = i < n && p >= 0 && p < end;
     const int64_t row = bh * P + p;
-    raw[j] = live ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) +
-                                                         row * D * (Q8 ? 1 : 2)) + gl)
-                  : make_uint4(0, 0, 0, 0);
+    raw[j] = live ? __ldg(reinterpret_cast<const Raw*>(static_cast<const uint8_t*>(cache) +
+                                                       row * D * (Q8 ? 1 : 2)) + gl)
+                  : Raw{};
     s[j] = Q8 && live ? __ldg(scale + row) : 0.0f;
   }
 #pragma unroll
@@ -357,14 +359,10 @@ __global__ void __launch_bounds__(kWarps * 32)
     O* dst = out + (static_cast<int64_t>(bh) * n + i) * D + gl * V;
     if constexpr (Q8) {
       const int8_t* q = reinterpret_cast<const int8_t*>(&raw[j]);
-      constexpr int W = 16 / sizeof(O);  // values per 16-byte store
+      O y[V];
 #pragma unroll
-      for (int c = 0; c < V / W; ++c) {
-        O y[W];
-#pragma unroll
-        for (int u = 0; u < W; ++u) y[u] = from_f32<O>(static_cast<float>(q[c * W + u]) * s[j]);
-        reinterpret_cast<uint4*>(dst)[c] = *reinterpret_cast<const uint4*>(y);
-      }
+      for (int u = 0; u < V; ++u) y[u] = from_f32<O>(static_cast<float>(q[u]) * s[j]);
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(y);
     } else {
       *reinterpret_cast<uint4*>(dst) = raw[j];
     }
@@ -541,7 +539,7 @@ extern "C" ltm_status ltm_kv_cache_read(const void* cache, const float* scale, l
     if (!scale && out_dtype == LTM_DTYPE_F32) LTM_UNSUPPORTED("fp32 caches (int8, f16 or bf16)");
     LTM_REQUIRE(((reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
                 "the cache and the output must be 16-byte aligned");
-    const int rows = 32 / (head_dim / (scale ? 16 : 8)) * kReadFly * kWarps;  // per CTA
+    const int rows = 32 / (head_dim * static_cast<int>(dtype_size(out_dtype)) / 16) * kReadFly * kWarps;  // per CTA
     const int gy = (n + rows - 1) / rows;
     LTM_REQUIRE(static_cast<int64_t>(B) * kv_heads < (1ll << 31) && gy < (1 << 16), "too many rows");
     const dim3 grid(static_cast<unsigned>(B) * kv_heads, static_cast<unsigned>(gy));
