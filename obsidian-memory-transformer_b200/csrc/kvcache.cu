@@ -17,9 +17,9 @@
 //
 // Rows are handled by groups of lanes that hold 16 bytes each, several rows per lane in
 // flight.  Measured (cold caches): the int8 write of 4 x 8192 tokens, 32 heads of 128 dims
-// (bf16), 165 us for 0.81 GB (4.9 TB/s; arithmetic: 14 instructions a value); reading
-// either cache back 72 us for 0.40 GB (5.6 TB/s); the reorder of 32 beams' caches 476 us,
-// at the copy bandwidth.
+// (bf16), 147 us for 0.81 GB (5.5 TB/s; arithmetic: 11 instructions a value); reading
+// either cache back 62 us for 0.40 GB (6.5 TB/s, the copy bandwidth); the reorder of 32
+// beams' caches 474 us, at the copy bandwidth.
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -201,9 +201,9 @@ __device__ __forceinline__ void magnitudes(const uint4 (&raw)[NP], int g, float 
 }
 
 // New tokens into the caches: input read once, codes and scales written once.  The int8
-// write is bound by its arithmetic (70% of the issue slots, 57% of the integer pipe; 4
-// rows in flight, because a warp's fixed part is 125 instructions: 322 -> 307 us with the
-// reads of both caches, from 388 with divisions), the 16-bit one by memory.  A lane holds 16 values of a row (two or four 16-byte pieces a
+// write is bound by its arithmetic (67% of the issue slots, 62% of the integer pipe, 50% of
+// the DRAM; 4 rows in flight, because a warp's fixed part is 125 instructions: 2 rows cost
+// 16 us more), the 16-bit one by memory.  A lane holds 16 values of a row (two or four 16-byte pieces a
 // group's width apart, so that loads and stores are contiguous over the group),
 // a group of D / 16 lanes a row; a warp takes kRowsFly * 32 / group
 // consecutive tokens of one head, K or V, so that its int8 rows are one
