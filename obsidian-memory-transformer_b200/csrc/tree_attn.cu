@@ -47,8 +47,8 @@
 // tile of 128 positions in 0.7 us (64 dims) or 1.4 us (128 dims); with 32, 64 and 128 rows it
 // takes 0.98, 1.26 and 1.84 us for 64 dims, 1.40, 1.45 and 2.2 us for 128: up to 64 rows of
 // 128 dims are read-bound, the others bound by the softmax's latencies (exponentials,
-// votes, barriers).  int8: 1.25 and 1.66 us for 32 and 64 rows of 64 dims, 1.8 and 2.45 us
-// for 128.  A segment's start and end cost 7 to 9 us (half of it queries, masks and the
+// votes, barriers).  int8: 1.25 and 1.66 us for 32 and 64 rows of 64 dims, 1.53 and 2.45
+// us for 128.  A segment's start and end cost 7 to 9 us (half of it queries, masks and the
 // tail's clean-up; 13 before those were overlapped and rid of divisions).
 //
 // In both, a row's reference maximum is only raised when a score exceeds it by more
@@ -808,7 +808,10 @@ struct TcSmem {
   static constexpr int kQ = (D / 64) * kQChunk;
   static constexpr int kPChunk = kTcTile * 128;        // 128 keys x 64 rows
   static constexpr int kPOne = ((N + 63) / 64) * kPChunk;
-  static constexpr int kPs = N <= 64 ? 2 : 1;         // P buffers
+  // int8, 32 rows of 128 dims: a fourth slot of f16 tiles instead of the second P (1.80 ->
+  // 1.53 us a tile; 64 rows lose 2% by it)
+  static constexpr bool kFour = Q8 && D == 128 && N == 32;
+  static constexpr int kPs = N <= 64 && !kFour ? 2 : 1;  // P buffers
   static constexpr int kP = kPs * kPOne;
   static constexpr int kOffP = kQ;
   static constexpr int kOffRing = kOffP + kP;
@@ -817,9 +820,9 @@ struct TcSmem {
   static constexpr int kOnes = kSum ? 2048 : 0;
   static constexpr int kLeft = 212 * 1024 - kOffRing;
   static constexpr int kFit = kLeft / kTile;
-  static constexpr int kSlots = Q8 ? (D == 64 ? 6 : 3) : kFit > 8 ? 8 : kFit;
+  static constexpr int kSlots = Q8 ? (D == 64 ? 6 : kFour ? 4 : 3) : kFit > 8 ? 8 : kFit;
   static constexpr int kCodes = Q8 ? kTcTile * D : 0;        // K or V tile of codes
-  static constexpr int kSlots8 = !Q8 ? 0 : D == 64 ? 8 : 4;
+  static constexpr int kSlots8 = !Q8 ? 0 : D == 64 ? 8 : kFour ? 3 : 4;
   static constexpr int kOffCodes = kOffRing + kSlots * kTile;
   static_assert(kSlots * kTile + kSlots8 * kCodes <= kLeft && kSlots >= 3, "ring");
   static constexpr int kOffOnes = kOffCodes + kSlots8 * kCodes;
@@ -1549,8 +1552,8 @@ __global__ void __launch_bounds__(32 * kCWarps) tree_combine_kernel(const TreePa
 // ---------------------------------------------------------------- launchers --
 // Rows of a block.  Up to 16 rows go to mma.sync; more to tcgen05, in the smallest block
 // that holds them, of at most 128 rows (64 for int8 caches).  17 int8 rows of 128 dims, 8 x
-// 32 heads x 16384 positions: 0.40 ms in one block, about 0.52 in two of mma.sync; 12 rows
-// 0.26 ms on mma.sync, 0.40 on tcgen05.
+// 32 heads x 16384 positions: 0.34 ms in one block, about 0.52 in two of mma.sync; 12 rows
+// 0.26 ms on mma.sync.
 int block_rows(int rows, bool q8) {
   if (rows <= 8) return 8;
   if (rows <= kMRows) return kMRows;
