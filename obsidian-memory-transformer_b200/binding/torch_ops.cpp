@@ -7,6 +7,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -97,7 +98,7 @@ class Call {
     }
   }
   at::Tensor empty(at::IntArrayRef shape, at::ScalarType type) const {
-    at::Tensor t = at::empty(shape, at::TensorOptions().dtype(type).device(device_));
+    at::Tensor t(at::detail::empty_cuda(shape, type, device_, std::nullopt));  // no dispatch
     if (other_ && t.numel() > 0)
       t.record_stream(c10::cuda::getStreamFromExternal(raw_, device_.index()).unwrap());
     return t;

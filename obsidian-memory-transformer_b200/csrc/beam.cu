@@ -23,7 +23,7 @@
 // partly under them): the 33 MB take 5 us to read, the chunks are bound by their
 // instructions (65% of the issue slots; 20 a logit, half of them a chunk's fixed part:
 // maxima of groups, candidates, ranks) and their barriers.  With the logits in registers,
-// three CTAs per SM, it took 26.5 us.  One request of 4 beams: 9.4 us, of which the host
+// three CTAs per SM, it took 26.5 us.  One request of 4 beams: 8.5 us, of which the host
 // needs most to queue two kernels (6.4 us in a captured graph).
 //
 // The reference's generation loop samples on the host

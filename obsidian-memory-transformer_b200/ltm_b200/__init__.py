@@ -502,8 +502,8 @@ def kv_cache_append(k, v, k_cache, v_cache, cache_lens, k_scale=None, v_scale=No
     head_dim]: int8 with fp32 scales [B, kv_heads, max_positions] (k, v f32, f16
     or bf16), or of k's type (f16 / bf16).  cache_lens, num_tokens (how many of the
     T tokens a sequence has): int32 [B].  The lengths are not advanced."""
-    _ops().kv_cache_append(k, v, k_cache, v_cache, cache_lens, k_scale, v_scale, num_tokens,
-                                 stream)
+    (_ops_module or _ops()).kv_cache_append(k, v, k_cache, v_cache, cache_lens, k_scale, v_scale,
+                                            num_tokens, stream)
 
 
 def kv_cache_read(cache, scale, length: int, first=None, cache_lens=None, dtype=None, out=None,
@@ -513,7 +513,8 @@ def kv_cache_read(cache, scale, length: int, first=None, cache_lens=None, dtype=
     caches give code * scale in `dtype` (f32, f16 or bf16; f32 when None), other caches
     (scale None) their values.  Positions outside [0, cache_lens[b]) (int32 [B];
     max_positions when None) give zeros."""
-    return _ops().kv_cache_read(cache, scale, length, first, cache_lens, dtype, out, stream)
+    return (_ops_module or _ops()).kv_cache_read(cache, scale, length, first, cache_lens, dtype,
+                                                 out, stream)
 
 
 def tree_attention(q, k_cache, v_cache, cache_lens, parents=None, k_scale=None, v_scale=None,
@@ -527,8 +528,8 @@ def tree_attention(q, k_cache, v_cache, cache_lens, parents=None, k_scale=None, 
     have been appended (kv_cache_append).  parents: int32 [B, T], -1 for a root;
     None for a chain.  num_tokens: int32 [B], how many of the T tokens a sequence
     has (the others get zeros).  Returns [B, T, heads, head_dim]."""
-    return _ops().tree_attention(q, k_cache, v_cache, cache_lens, parents, k_scale, v_scale,
-                                       num_tokens, out, stream)
+    return (_ops_module or _ops()).tree_attention(q, k_cache, v_cache, cache_lens, parents, k_scale,
+                                                  v_scale, num_tokens, out, stream)
 
 
 def beam_select(logits, scores, num_out: int | None = None, done=None, end_token: int = -1,
@@ -539,7 +540,7 @@ def beam_select(logits, scores, num_out: int | None = None, done=None, end_token
     int32) of the K = num_out (W when None) best continuations, best first.  With
     `done` (bool [B, W]) finished beams continue as themselves with `end_token`
     and a fourth output [B, K] bool says which continuations are finished."""
-    return _ops().beam_select(logits, scores, num_out, done, end_token, stream)
+    return (_ops_module or _ops()).beam_select(logits, scores, num_out, done, end_token, stream)
 
 
 def kv_cache_reorder(caches, beams, cache_lens=None, first=None, stream=None) -> None:
@@ -549,7 +550,7 @@ def kv_cache_reorder(caches, beams, cache_lens=None, first=None, stream=None) ->
     max_positions, head_dim] tensors (K and V of all layers) and [B * W, kv_heads,
     max_positions] tensors (int8 caches' scales), each once; beams int32 [B, W];
     cache_lens, first: int32 [B] (max_positions and 0 when None)."""
-    _ops().kv_cache_reorder(caches, beams, cache_lens, first, stream)
+    (_ops_module or _ops()).kv_cache_reorder(caches, beams, cache_lens, first, stream)
 
 
 # --------------------------------------------------------------------- block --
