@@ -15,6 +15,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <optional>
 #include <string>
 #include <vector>
 
@@ -78,8 +79,11 @@ ltm_dtype dtype_of(at::ScalarType s) {
   }
 }
 
-// Device and stream of one call.  The tensors' device is the current one while
-// this lives; memory made for the call is safe on a stream that is not the current one.
+// Device and stream of one call.  The tensors' device and the call's stream are the current
+// ones while this lives.  Memory made for the call comes from the call's stream: a block of
+// the caller's current stream may still be read or written by work queued there, which the
+// call does not wait for.  The caller's stream is recorded as a user of the outputs, so that
+// they are not given out again while its work reads them.
 class Call {
  public:
   Call(const at::Tensor& first, PyObject* stream)
@@ -93,14 +97,13 @@ class Call {
       if (PyErr_Occurred()) throw Refused{};
       if (s != static_cast<void*>(raw_)) {
         raw_ = static_cast<cudaStream_t>(s);
-        other_ = true;
+        other_.emplace(c10::cuda::getStreamFromExternal(raw_, device_.index()).unwrap());
       }
     }
   }
   at::Tensor empty(at::IntArrayRef shape, at::ScalarType type) const {
     at::Tensor t(at::detail::empty_cuda(shape, type, device_, std::nullopt));  // no dispatch
-    if (other_ && t.numel() > 0)
-      t.record_stream(c10::cuda::getStreamFromExternal(raw_, device_.index()).unwrap());
+    if (other_ && t.numel() > 0) t.record_stream(stream_.unwrap());
     return t;
   }
   void* stream() const { return static_cast<void*>(raw_); }
@@ -126,9 +129,9 @@ class Call {
  private:
   c10::Device device_;
   c10::cuda::CUDAGuard guard_;
-  c10::cuda::CUDAStream stream_;
-  cudaStream_t raw_;
-  bool other_ = false;
+  c10::cuda::CUDAStream stream_;  // the caller's
+  cudaStream_t raw_;              // the call's
+  std::optional<c10::cuda::CUDAStreamGuard> other_;  // where they differ
 };
 
 void done(ltm_status st) {
