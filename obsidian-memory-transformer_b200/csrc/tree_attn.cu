@@ -647,7 +647,9 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
             }
             mref[nr][j] = a;
             eref[nr][j] = e;
-            if constexpr (Q8) frow[nr][j] = e == -INFINITY ? 0.0f : ex2_approx(a - e);
+            // finite: where the largest scores are those of keys with (nearly) no V scale, the
+            // factor may overflow, and times such a scale of 0 it would be a NaN
+            if constexpr (Q8) frow[nr][j] = e == -INFINITY ? 0.0f : ex2_approx(fminf(a - e, 126.0f));
           }
       }
       // ---- probabilities, transposed to the B fragment of the value product
