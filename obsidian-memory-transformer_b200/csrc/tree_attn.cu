@@ -666,9 +666,10 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
             l[nr][j] += pr[j];
             if constexpr (Q8) {
               // p * v's scale, against its own reference: at most 2^8.  The factor only
-              // overflows where p is 0.  A scale NaN becomes an infinity here, and a NaN by
-              // its row's zero codes; a row that does not see the key takes nothing of it.
-              pr[j] *= fminf(vsc[h] * frow[nr][j], 3.0e38f);
+              // overflows where p is 0.  A scale NaN makes a NaN of it, whatever p; a row that
+              // does not see the key takes nothing of it.
+              pr[j] = fmaf(pr[j], fminf(vsc[h] * frow[nr][j], 3.0e38f),
+                           vsc[h] != vsc[h] ? vsc[h] : 0.0f);
               if (tail && s == -INFINITY) pr[j] = 0.0f;
             }
           }
@@ -1170,9 +1171,11 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
             for (int i = 0; i < RW; ++i) seen |= static_cast<uint32_t>(mask[i] >> at & 1ull) << i;
         }
         float ksc = 1.0f, vsc = 1.0f, lvs = 0.0f;
+        bool no_scale = false;  // V's scale is a NaN
         if constexpr (Q8) {
           ksc = ks_next[0];
           asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lvs) : "f"(vs_next[0]));
+          no_scale = vs_next[0] != vs_next[0];
           vsc = fminf(vs_next[0], 3.0e38f);
           ks_next[0] = ks_next[1];
           vs_next[0] = vs_next[1];
@@ -1237,8 +1240,8 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
               x[i + y] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(x[i + y]), unit, n4[y])));
           }
         };
-        // int8: p * v's scale goes into P, against its own reference: at most 2^8
-        // (a scale NaN counts as 3e38 and becomes an infinity in P)
+        // int8: p * v's scale goes into P, against its own reference: at most 2^8 (a scale
+        // NaN counts as 3e38 until P is stored)
         uint32_t pk[16];
         auto weigh = [&](const uint32_t (&x)[32]) -> float {
           float top = 0.0f;
@@ -1352,6 +1355,11 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
           for (int i = 0; i < 32; i += 2)
             pk[i / 2] = pack16<std::is_same<T, __nv_bfloat16>::value>(__uint_as_float(e[i]),
                                                                       __uint_as_float(e[i + 1]));
+        }
+        if (Q8 && no_scale) {  // NaN for every row that sees the key, whatever its weight
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            pk[i / 2] |= (seen >> i & 1u) * 0x7fffu | (seen >> (i + 1) & 1u) * 0x7fff0000u;
         }
         // this P buffer is free once the tile that was in it has been contracted
         if (it >= PB) wait_pv(it - PB);

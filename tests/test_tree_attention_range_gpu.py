@@ -33,3 +33,32 @@ def test_zero_value_row_with_all_the_weight(ltm, far, d, T, G):
     got = ltm.tree_attention(q, k, v, lens, None, ks, vs).double()
     assert torch.isfinite(got).all()
     assert float(got.abs().max()) <= (n + T) * 1.27 * 2.0 ** (1 - far) + 2.0 ** -126
+
+
+@pytest.mark.parametrize("T,G", ROWS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("others", [0.0, 0.01, 1e30])
+@pytest.mark.parametrize("below", [0.0, 130.0])
+def test_nan_scale_reaches_every_token_that_sees_it(ltm, below, others, d, T, G):
+    """int8: a value row with the scale NaN (a row that held a NaN) whose key is seen gives
+    NaN, whatever its weight and the others' scales; a drafted one only to its descendants."""
+    import torch
+    n = 300
+    v = torch.full((1, 1, n + T, d), 100, dtype=torch.int8, device="cuda")
+    vs = torch.full((1, 1, n + T), others, device="cuda")
+    if others == 0:
+        v.zero_()
+    k = torch.zeros((1, 1, n + T, d), dtype=torch.int8, device="cuda")
+    ks = torch.ones((1, 1, n + T), device="cuda")
+    q = torch.full((1, T, G, d), 4.0, device="cuda").bfloat16()
+    lens = torch.full((1,), n, dtype=torch.int32, device="cuda")
+    for at, seen in ((150, range(T)), (n + T - 1, [T - 1])):
+        v2, vs2, k2, ks2 = v.clone(), vs.clone(), k.clone(), ks.clone()
+        v2[:, :, at] = 0
+        vs2[:, :, at] = float("nan")
+        k2[:, :, at] = -1
+        ks2[:, :, at] = below * math.log(2.0) * math.sqrt(d) / (d * 4.0)
+        got = ltm.tree_attention(q, k2, v2, lens, None, ks2, vs2)
+        for t in range(T):
+            bad = torch.isnan(got[0, t])
+            assert bad.all() if t in seen else not bad.any(), (at, t)
