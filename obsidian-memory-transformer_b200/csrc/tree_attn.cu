@@ -52,7 +52,8 @@
 // tail's clean-up; 13 before those were overlapped and rid of divisions).
 //
 // In both, a row's reference maximum is only raised when a score exceeds it by more
-// than 2^8.  A non-finite value of a drafted token must not
+// than 2^8.  Weights that go to the tensor core as f16 are held 2^7 higher (Raise), so that
+// the many small ones of a long context stay above its smallest numbers.  A non-finite value of a drafted token must not
 // reach the tokens that do not see it (0 * inf): it is taken out of the tile, and
 // the combine kernel adds it to the rows that do.
 //
@@ -70,8 +71,17 @@ constexpr int kTBatch = 512;      // sequences per launch
 constexpr int kScanWords = 3 * (kTBatch + 2);  // what tree_scan leaves
 constexpr int kTMaxGrid = 256;    // CTAs that share the tiles, whatever the device
 constexpr int kTMaxTokens = 64;   // drafted tokens (one 64-bit ancestor mask)
-constexpr float kTRaise = 8.0f;   // log2 of the largest probability before the reference is raised
-constexpr float kTMost = 256.0f;  // 2^kTRaise
+// A row's reference in log2 units: `lower` below its maximum when it is set, raised when a
+// score passes it by `at`.  Weights that stay in fp32 or become bf16 are at most 2^8.  f16
+// ends at 2^16, and below 2^-14 its steps are 2^-24 whatever the weight: with the largest
+// between 2^7 and 2^15, half such a step is at most 2^-32 of it (2^-25 with a reference at
+// the maximum: 65536 keys of 2^-26 each then vanished).
+template <bool F16>
+struct Raise {
+  static constexpr float lower = F16 ? 7.0f : 0.0f;
+  static constexpr float at = 8.0f + lower;
+  static constexpr float most = F16 ? 32768.0f : 256.0f;  // 2^at
+};
 
 struct TreeParams {
   const void* q;
@@ -391,6 +401,8 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
   constexpr int NS = S::kSlots, KS = D / 16, NU = D / 16, NW = S::kWarps;
   constexpr int ROWS = S::kRows;
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value && !Q8;  // type of the products
+  using RaiseS = Raise<!Q8 && !BF>;  // of the scores (int8: the sums' weights, in fp32)
+  using RaiseP = Raise<!BF>;         // of what goes to the tensor core
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -616,9 +628,9 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
             }
             acc[nr][2 * h + j] = s;
           }
-          need |= fmaxf(acc[nr][j], acc[nr][2 + j]) > mref[nr][j] + kTRaise;
+          need |= fmaxf(acc[nr][j], acc[nr][2 + j]) > mref[nr][j] + RaiseS::at;
           if constexpr (Q8)
-            need |= fmaxf(acc[nr][j] + lvs[0], acc[nr][2 + j] + lvs[1]) > eref[nr][j] + kTRaise;
+            need |= fmaxf(acc[nr][j] + lvs[0], acc[nr][2 + j] + lvs[1]) > eref[nr][j] + RaiseP::at;
         }
       if (__any_sync(0xffffffffu, need)) {
         // raise the references to the maxima (and rescale what is summed)
@@ -626,10 +638,10 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
         for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float a = fmaxf(mref[nr][j], fmaxf(acc[nr][j], acc[nr][2 + j]));
+            float a = fmaxf(mref[nr][j], fmaxf(acc[nr][j], acc[nr][2 + j]) - RaiseS::lower);
             float e = eref[nr][j];
             if constexpr (Q8)
-              e = fmaxf(e, fmaxf(acc[nr][j] + lvs[0], acc[nr][2 + j] + lvs[1]));
+              e = fmaxf(e, fmaxf(acc[nr][j] + lvs[0], acc[nr][2 + j] + lvs[1]) - RaiseP::lower);
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) {
               a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, x));
@@ -665,7 +677,7 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
             pr[j] = ex2_approx(s - (mref[nr][j] == -INFINITY ? 0.0f : mref[nr][j]));
             l[nr][j] += pr[j];
             if constexpr (Q8) {
-              // p * v's scale, against its own reference: at most 2^8.  The factor only
+              // p * v's scale, against its own reference: at most 2^15.  The factor only
               // overflows where p is 0.  A scale NaN makes a NaN of it, whatever p; a row that
               // does not see the key takes nothing of it.
               pr[j] = fmaf(pr[j], fminf(vsc[h] * frow[nr][j], 3.0e38f),
@@ -899,6 +911,8 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
   constexpr int NS = S::kSlots, N8 = S::kSlots8;
   constexpr int RW = S::kRows, kSoft = 128 * S::kGroups, PB = S::kPs;
   constexpr bool SUM = S::kSum;
+  using RaiseS = Raise<!Q8 && std::is_same<T, __half>::value>;
+  using RaiseP = Raise<Q8 || std::is_same<T, __half>::value>;
   constexpr uint32_t kCols = 4 * N;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -1240,7 +1254,7 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
               x[i + y] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(x[i + y]), unit, n4[y])));
           }
         };
-        // int8: p * v's scale goes into P, against its own reference: at most 2^8 (a scale
+        // int8: p * v's scale goes into P, against its own reference: at most 2^15 (a scale
         // NaN counts as 3e38 until P is stored)
         uint32_t pk[16];
         auto weigh = [&](const uint32_t (&x)[32]) -> float {
@@ -1270,8 +1284,8 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
           expo(e);
 #pragma unroll
           for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(e[i]));
-          if constexpr (Q8) top = fmaxf(top, weigh(e));
-          need = top > kTMost;
+          need = top > RaiseS::most;
+          if constexpr (Q8) need |= weigh(e) > RaiseP::most;
         }
         if (soft_any<kSoft>(need)) {
           if (got) {
@@ -1301,14 +1315,15 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
             const float top = fmaxf(fmaxf(smax[tid], smax[N + tid]),
                                     fmaxf(smax[2 * N + tid], smax[3 * N + tid]));
             const float old = first ? -INFINITY : -nref[tid];
-            const float now = fmaxf(old, top);
+            const float now = fmaxf(old, top - RaiseS::lower);
             // a row without a score above -inf keeps 0: its probabilities are 0 (or NaN)
             nref[tid] = now == -INFINITY ? 0.0f : -now;
             fact[tid] = first ? 0.0f : ex2_approx(old - now);
             if constexpr (Q8) {
               const float* m = smax + 4 * N + tid;
               const float old_e = first ? -INFINITY : eref[tid];
-              const float now_e = fmaxf(old_e, fmaxf(fmaxf(m[0], m[N]), fmaxf(m[2 * N], m[3 * N])));
+              const float now_e = fmaxf(old_e, fmaxf(fmaxf(m[0], m[N]), fmaxf(m[2 * N], m[3 * N])) -
+                                                   RaiseP::lower);
               eref[tid] = now_e;
               facto[tid] = old_e == -INFINITY ? 0.0f : ex2_approx(old_e - now_e);
               // capped: p, at most 2^8, times it stays finite
