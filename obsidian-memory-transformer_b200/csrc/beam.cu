@@ -369,6 +369,92 @@ constexpr int kMergeKeys = 8192;  // entries whose keys fit in shared memory
 constexpr int kMergeAll = 128;    // entries that are ranked without a bound
 constexpr int kMergeSlack = 24;   // continuations past K that are ranked rather than sorted out
 
+// What the merge knows of a request's rows.
+struct Rows {
+  double score[kMaxW], lse[kMaxW];  // score, log(sum of exp(logit - max))
+  float max[kMaxW];
+  uint8_t done[kMaxW];
+};
+
+// Total of a logit (ordered bits) of row w.
+__device__ __forceinline__ uint64_t total_bits(const Rows& r, int w, uint32_t u) {
+  double t = -INFINITY;
+  if (u > kNegInf && r.score[w] > -INFINITY)
+    t = r.done[w] ? r.score[w]
+                  : r.score[w] + ((static_cast<double>(unordered(u)) - r.max[w]) - r.lse[w]);
+  return ordered64(t);
+}
+
+// Writes continuation f = beam * V + token with the total t as the k-th of its request.
+struct Outputs {
+  float* scores;
+  int *beams, *tokens;
+  uint8_t* done;
+};
+__device__ __forceinline__ void write_out(const Outputs& o, const Rows& r, int64_t k, uint64_t t,
+                                          uint32_t f, int V, int end) {
+  const int w = static_cast<int>(f / static_cast<uint32_t>(V));
+  const int tok = static_cast<int>(f) - w * V;
+  o.scores[k] = static_cast<float>(unordered64(t));
+  o.beams[k] = w;
+  o.tokens[k] = tok;
+  if (o.done) o.done[k] = r.done[w] || tok == end;
+}
+
+// For a request with a row so far out that 64 bits may give different logits one total (a
+// score of fp32's lowest value, say, or a logit of +inf): a chunk's list, ordered by the
+// logits, then may lack continuations of a total that it holds.  Only those equal to the
+// K-th total matter (of greater ones there are fewer than K, so they are all in the lists),
+// and of those the lowest indices are the request's: the outputs from k0 + c on, c the number
+// of greater totals, are written anew from the logits, beam after beam.  By the whole CTA.
+constexpr float kFar = 16777216.0f;  // 2^24: steps of 2^-28
+template <class T>
+__device__ void ties_by_index(const T* logits, int64_t ldw, const Rows& r, const Outputs& o,
+                              int64_t k0, int W, int V, int K, int end) {
+  __shared__ int s_found[kBThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto total = [&](int w, int x) {
+    return total_bits(r, w, r.done[w] && x != end
+                                ? kNegInf : ordered(logit_value<T>(to_f32(logits[w * ldw + x]))));
+  };
+  __syncthreads();  // the outputs are written
+  const uint64_t tk = total(o.beams[k0 + K - 1], o.tokens[k0 + K - 1]);
+  if (tk == ordered64(-INFINITY)) return;  // equal logits (-inf) only
+  int at = __syncthreads_count(tid < K && total(o.beams[k0 + tid], o.tokens[k0 + tid]) > tk);
+#pragma unroll 1
+  for (int w = 0; w < W && at < K; ++w) {
+    if (!(r.score[w] > -INFINITY)) continue;
+    if (!r.done[w] && (r.max[w] == -INFINITY || total_bits(r, w, ordered(r.max[w])) < tk)) continue;
+#pragma unroll 1
+    for (int i0 = r.done[w] ? end : 0; i0 < (r.done[w] ? end + 1 : V) && at < K; i0 += kBThreads) {
+      const int i = i0 + tid;
+      const bool hit = i < V && total(w, i) == tk;
+      const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+      if (lane == 0) s_found[warp] = __popc(hits);
+      __syncthreads();
+      int mine = at + __popc(hits & ((1u << lane) - 1u));
+#pragma unroll 1
+      for (int x = 0; x < kBThreads / 32; ++x) {
+        if (x < warp) mine += s_found[x];
+        at += s_found[x];
+      }
+      if (hit && mine < K) write_out(o, r, k0 + mine, tk, static_cast<uint32_t>(w) * V + i, V, end);
+      __syncthreads();
+    }
+  }
+}
+__device__ __noinline__ void order_ties(const void* logits, ltm_dtype dtype, int64_t ldb,
+                                        int64_t ldw, const Rows& r, const Outputs& o, int W, int V,
+                                        int K, int end) {
+  const int64_t b = blockIdx.x, at = b * ldb;
+  if (dtype == LTM_DTYPE_F32)
+    ties_by_index(static_cast<const float*>(logits) + at, ldw, r, o, b * K, W, V, K, end);
+  else if (dtype == LTM_DTYPE_F16)
+    ties_by_index(static_cast<const __half*>(logits) + at, ldw, r, o, b * K, W, V, K, end);
+  else
+    ties_by_index(static_cast<const __nv_bfloat16*>(logits) + at, ldw, r, o, b * K, W, V, K, end);
+}
+
 // One CTA per request.  Its W * nchunk lists are sorted, so the best
 // d = ceil(K / lists) entries of every list hold K continuations, and the least of
 // those d-th entries is a total that at least K reach.  From there a bisection on
@@ -377,14 +463,13 @@ constexpr int kMergeSlack = 24;   // continuations past K that are ranked rather
 // shared memory does not take them (equal totals), the K best are taken one by
 // one.  Loops stay rolled: for one request the code's own fetch is most of the time.
 __global__ void __launch_bounds__(kBThreads)
-    beam_merge_kernel(const float* __restrict__ scores, const uint8_t* __restrict__ done, int end,
+    beam_merge_kernel(const void* logits, ltm_dtype dtype, int64_t ldb, int64_t ldw,
+                      const float* __restrict__ scores, const uint8_t* __restrict__ done, int end,
                       int W, int V, int K, int nchunk, const BeamPartial* stats,
-                      const uint64_t* lists, float* __restrict__ out_scores,
-                      int* __restrict__ out_beams, int* __restrict__ out_tokens,
-                      uint8_t* __restrict__ out_done) {
-  __shared__ double s_base[kMaxW], s_score[kMaxW];  // score - max - log(sum), score
-  __shared__ float s_max[kMaxW];
-  __shared__ uint8_t s_done[kMaxW];
+                      const uint64_t* lists,
+                      const __grid_constant__ Outputs out) {
+  __shared__ Rows rows;
+  __shared__ int s_far;  // a row is far out
   __shared__ Total s_cand[kMergeCand];
   __shared__ Total s_best[kBThreads / 32];
   __shared__ uint32_t s_key[kMergeKeys];
@@ -396,9 +481,10 @@ __global__ void __launch_bounds__(kBThreads)
   const uint64_t* mine = lists + static_cast<int64_t>(b) * entries;
   for (int w = tid; w < W; w += kBThreads) {
     const float sc = scores[b * W + w];
-    s_score[w] = sc == sc ? sc : -INFINITY;
-    s_done[w] = done != nullptr && done[b * W + w] != 0;
+    rows.score[w] = sc == sc ? sc : -INFINITY;
+    rows.done[w] = done != nullptr && done[b * W + w] != 0;
   }
+  if (tid == 0) s_far = 0;
   grid_wait();  // the chunks' kernel has completed
   const bool all = entries <= kMergeAll;  // few enough to rank as they are
   const uint64_t own = all && tid < entries ? mine[tid] : 0ull;  // in flight with the sums
@@ -421,29 +507,25 @@ __global__ void __launch_bounds__(kBThreads)
       m = mm;
     }
     if (lane == 0) {
-      s_max[w] = m;
-      s_base[w] = s_score[w] - static_cast<double>(logf(sum));
+      rows.max[w] = m;
+      rows.lse[w] = static_cast<double>(logf(sum));
+      const float out = fmaxf(fabsf(m), fabsf(static_cast<float>(rows.score[w])));
+      if (out >= kFar && out < INFINITY && !rows.done[w]) s_far = 1;
     }
   }
   __syncthreads();
   auto total = [&](int l, uint64_t key) -> Total {  // of a key of list l
     if (key == 0ull) return Total{0ull, ~0u, 0u};
-    const uint32_t u = static_cast<uint32_t>(key >> 32);
     const int w = l / nchunk;
-    double t = -INFINITY;
-    if (u > kNegInf && s_score[w] > -INFINITY)
-      t = s_done[w] ? s_score[w] : s_base[w] + (static_cast<double>(unordered(u)) - s_max[w]);
-    return Total{ordered64(t), static_cast<uint32_t>(w) * V + ~static_cast<uint32_t>(key), 0u};
+    return Total{total_bits(rows, w, static_cast<uint32_t>(key >> 32)),
+                 static_cast<uint32_t>(w) * V + ~static_cast<uint32_t>(key), 0u};
   };
   auto entry = [&](int l, int i) { return total(l, mine[i]); };  // entry i of all
   auto put = [&](int k, const Total& x) {
-    const int w = static_cast<int>(x.f / static_cast<uint32_t>(V));
-    const int tok = static_cast<int>(x.f) - w * V;
-    const int64_t o = static_cast<int64_t>(b) * K + k;
-    out_scores[o] = static_cast<float>(unordered64(x.t));
-    out_beams[o] = w;
-    out_tokens[o] = tok;
-    if (out_done) out_done[o] = s_done[w] || tok == end;
+    write_out(out, rows, static_cast<int64_t>(b) * K + k, x.t, x.f, V, end);
+  };
+  auto finish = [&] {
+    if (s_far) order_ties(logits, dtype, ldb, ldw, rows, out, W, V, K, end);
   };
   auto rank_all = [&](int n) {
     rank_in_place(
@@ -457,6 +539,7 @@ __global__ void __launch_bounds__(kBThreads)
     if (tid < entries) s_cand[tid] = total(tid / K, own);
     __syncthreads();
     rank_all(entries);
+    finish();
     return;
   }
   // ---- the bound: `low` is reached by at least K continuations
@@ -525,6 +608,7 @@ __global__ void __launch_bounds__(kBThreads)
       if (key_of(i) >= low) s_cand[atomicAdd(&s_count[0], 1)] = entry(i / K, i);
     __syncthreads();
     rank_all(n);
+    finish();
     return;
   }
   Total last{~0ull, 0u, 0u};
@@ -550,6 +634,7 @@ __global__ void __launch_bounds__(kBThreads)
     if (tid == 0) put(k, best);
     last = best;
   }
+  finish();
 }
 
 int chunks_of(int V, int per) { return (V + kBThreads * per - 1) / (kBThreads * per); }
@@ -625,10 +710,10 @@ extern "C" ltm_status ltm_beam_select(const void* logits, ltm_dtype dtype, int64
     });
     check_launch("beam_chunk_kernel", st);
     // launched while the chunks still run; it waits for their completion on the device
-    launch_dependent(beam_merge_kernel, dim3(static_cast<unsigned>(B)), kBThreads, 0, st, scores,
-                     done, end_token, W, V, K, nchunk, static_cast<const BeamPartial*>(stats),
-                     static_cast<const uint64_t*>(lists), out_scores, out_beams, out_tokens,
-                     out_done);
+    launch_dependent(beam_merge_kernel, dim3(static_cast<unsigned>(B)), kBThreads, 0, st, logits,
+                     dtype, batch_stride, beam_stride, scores, done, end_token, W, V, K, nchunk,
+                     static_cast<const BeamPartial*>(stats), static_cast<const uint64_t*>(lists),
+                     Outputs{out_scores, out_beams, out_tokens, out_done});
     check_launch("beam_merge_kernel", st);
   });
 }
