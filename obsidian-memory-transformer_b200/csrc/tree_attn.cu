@@ -659,9 +659,9 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
             }
             mref[nr][j] = a;
             eref[nr][j] = e;
-            // finite: where the largest scores are those of keys with (nearly) no V scale, the
-            // factor may overflow, and times such a scale of 0 it would be a NaN
-            if constexpr (Q8) frow[nr][j] = e == -INFINITY ? 0.0f : ex2_approx(fminf(a - e, 126.0f));
+            // capped: p, at most 2^8, times it stays finite (times a scale of 0 it would else
+            // be a NaN where the largest scores are those of keys with nearly no V scale)
+            if constexpr (Q8) frow[nr][j] = e == -INFINITY ? 0.0f : ex2_approx(fminf(a - e, 119.0f));
           }
       }
       // ---- probabilities, transposed to the B fragment of the value product
@@ -677,11 +677,9 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
             pr[j] = ex2_approx(s - (mref[nr][j] == -INFINITY ? 0.0f : mref[nr][j]));
             l[nr][j] += pr[j];
             if constexpr (Q8) {
-              // p * v's scale, against its own reference: at most 2^15.  The factor only
-              // overflows where p is 0.  A scale NaN makes a NaN of it, whatever p; a row that
-              // does not see the key takes nothing of it.
-              pr[j] = fmaf(pr[j], fminf(vsc[h] * frow[nr][j], 3.0e38f),
-                           vsc[h] != vsc[h] ? vsc[h] : 0.0f);
+              // p * v's scale, against its own reference: at most 2^15.  A scale NaN makes
+              // a NaN of it, whatever p; a row that does not see the key takes nothing of it.
+              pr[j] = pr[j] * frow[nr][j] * vsc[h];
               if (tail && s == -INFINITY) pr[j] = 0.0f;
             }
           }
