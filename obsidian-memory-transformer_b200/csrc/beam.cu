@@ -149,8 +149,8 @@ struct BeamPartial {
 // and five CTAs share an SM: their loads, exponentials and filters overlap.
 template <class T, int PER>
 __global__ void __launch_bounds__(kBThreads, 5)
-    beam_chunk_kernel(const T* __restrict__ logits, int64_t ldb, int64_t ldw,
-                      const float* __restrict__ scores, const uint8_t* __restrict__ done, int end,
+    beam_chunk_kernel(const T* logits, int64_t ldb, int64_t ldw,
+                      const float* scores, const uint8_t* done, int end,
                       int W, int V, int K, int nchunk, int groups, BeamPartial* __restrict__ stats,
                       uint64_t* __restrict__ lists) {
   constexpr int N = 16 / sizeof(T);  // logits per vector
@@ -464,7 +464,7 @@ __device__ __noinline__ void order_ties(const void* logits, ltm_dtype dtype, int
 // one.  Loops stay rolled: for one request the code's own fetch is most of the time.
 __global__ void __launch_bounds__(kBThreads)
     beam_merge_kernel(const void* logits, ltm_dtype dtype, int64_t ldb, int64_t ldw,
-                      const float* __restrict__ scores, const uint8_t* __restrict__ done, int end,
+                      const float* scores, const uint8_t* done, int end,
                       int W, int V, int K, int nchunk, const BeamPartial* stats,
                       const uint64_t* lists,
                       const __grid_constant__ Outputs out) {

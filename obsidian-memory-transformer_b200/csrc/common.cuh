@@ -262,7 +262,10 @@ void allow_smem(K kernel, int bytes) {
 // it on the stream: its CTAs may be scheduled once every CTA of the kernel before has
 // called grid_release or ended, which hides the launch (and what it does before the
 // wait: it must not touch memory that earlier kernels write, unless they are
-// complete when the kernel before releases).
+// complete when the kernel before releases).  What others write is read by plain loads:
+// the read-only path (__ldg, ld.global.nc, const __restrict__ pointers, of which the compiler
+// makes it) is for memory that nobody writes while the kernel lives, and this one lives
+// while the kernel before it still writes.
 template <class... P, class... A>
 void launch_dependent(void (*kernel)(P...), dim3 grid, int block, size_t smem, cudaStream_t stream,
                       A... args) {

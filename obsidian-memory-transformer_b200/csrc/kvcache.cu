@@ -211,10 +211,10 @@ __device__ __forceinline__ void magnitudes(const uint4 (&raw)[NP], int g, float 
 // neighbouring heads of the same tokens: the reads cover whole projection rows.
 template <class T, int D, bool Q8>
 __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 ? 4 : 2)
-    cache_append_kernel(const T* __restrict__ k, RowStrides sk, const T* __restrict__ v,
+    cache_append_kernel(const T* k, RowStrides sk, const T* v,
                         RowStrides sv, void* __restrict__ kc, void* __restrict__ vc,
                         float* __restrict__ ks, float* __restrict__ vs, int64_t P,
-                        const int* __restrict__ lens, const int* __restrict__ num_tokens, int Tn,
+                        const int* lens, const int* num_tokens, int Tn,
                         int heads, int tgroups, int* err) {
   constexpr int N = 16 / sizeof(T);   // values per piece
   constexpr int NP = kVals / N;       // pieces per lane
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 ? 4 : 2)
     const uint4* at = reinterpret_cast<const uint4*>(src + t * st) + gl;
 #pragma unroll
     for (int q = 0; q < NP; ++q)
-      raw[j][q] = t < n ? __ldg(at + q * G) : make_uint4(0, 0, 0, 0);
+      raw[j][q] = t < n ? at[q * G] : make_uint4(0, 0, 0, 0);
   }
   const int64_t row0 = (static_cast<int64_t>(b) * heads + h) * P + len;
 #pragma unroll
@@ -321,8 +321,8 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 ? 4 : 2)
 // 16-bit cache, that it holds of a row.
 template <class O, int D, bool Q8>
 __global__ void __launch_bounds__(kWarps * 32)
-    cache_read_kernel(const void* __restrict__ cache, const float* __restrict__ scale, int64_t P,
-                      const int* __restrict__ first, const int* __restrict__ lens, int heads,
+    cache_read_kernel(const void* cache, const float* scale, int64_t P,
+                      const int* first, const int* lens, int heads,
                       int n, O* __restrict__ out) {
   constexpr int V = 16 / sizeof(O);
   using Raw = std::conditional_t<!Q8, uint4, std::conditional_t<V == 8, uint2, uint32_t>>;
@@ -347,10 +347,10 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int64_t p = p0 + i;
     const bool live = i < n && p >= 0 && p < end;
     const int64_t row = bh * P + p;
-    raw[j] = live ? __ldg(reinterpret_cast<const Raw*>(static_cast<const uint8_t*>(cache) +
-                                                       row * D * (Q8 ? 1 : 2)) + gl)
+    raw[j] = live ? reinterpret_cast<const Raw*>(static_cast<const uint8_t*>(cache) +
+                                                 row * D * (Q8 ? 1 : 2))[gl]
                   : Raw{};
-    s[j] = Q8 && live ? __ldg(scale + row) : 0.0f;
+    s[j] = Q8 && live ? scale[row] : 0.0f;
   }
 #pragma unroll
   for (int j = 0; j < kReadFly; ++j) {
@@ -402,8 +402,8 @@ __device__ __forceinline__ void reorder_columns(uint8_t* base, int64_t beam_byte
 
 template <int WMAX>
 __global__ void __launch_bounds__(256)
-    cache_reorder_kernel(const __grid_constant__ ReorderParams p, const int* __restrict__ beams,
-                         const int* __restrict__ first, const int* __restrict__ lens, int W,
+    cache_reorder_kernel(const __grid_constant__ ReorderParams p, const int* beams,
+                         const int* first, const int* lens, int W,
                          int heads, int64_t P, int parts, int* err) {
   __shared__ int src[WMAX];
   grid_wait();

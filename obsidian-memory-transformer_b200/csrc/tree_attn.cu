@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(32 * (MmaSmem<D, Q8, NR>::kWarps + 1), 1)
     float sc_next[kAhead];
     auto load_scale = [&](int t) -> float {
       const int key = (sp.tile + t) * S::kKeys + wk + (lane & 15);
-      return key < keys ? __ldg((lane < 16 ? p.ks : p.vs) + head * p.P + key) : 0.0f;
+      return key < keys ? (lane < 16 ? p.ks : p.vs)[head * p.P + key] : 0.0f;
     };
     if constexpr (Q8)
 #pragma unroll
@@ -1119,7 +1119,7 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
           const int rr = sp.rb * N + r, t = over_g(p, rr);
           const T* qp = static_cast<const T*>(p.q) + sp.b * p.qb + t * p.qt +
                         (static_cast<int64_t>(sp.h) * p.G + (rr - t * p.G)) * p.qh;
-          v[i] = r < sp.rows ? __ldg(reinterpret_cast<const uint4*>(qp) + x)
+          v[i] = r < sp.rows ? reinterpret_cast<const uint4*>(qp)[x]
                              : make_uint4(0, 0, 0, 0);
         }
         if ((sp.tile + nt) * kTcTile > sp.len)
@@ -1162,8 +1162,8 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
       auto load_scales = [&](int t, int slot) {
         const int key = (sp.tile + t) * kTcTile + kt;
         const bool in = key < sp.len + sp.n;
-        ks_next[slot] = in ? __ldg(p.ks + head * p.P + key) : 0.0f;
-        vs_next[slot] = in ? __ldg(p.vs + head * p.P + key) : 0.0f;
+        ks_next[slot] = in ? p.ks[head * p.P + key] : 0.0f;
+        vs_next[slot] = in ? p.vs[head * p.P + key] : 0.0f;
       };
       if constexpr (Q8) {
         load_scales(0, 0);
