@@ -1,9 +1,11 @@
 """Build recipe of libltm_b200.so: every csrc/*.cu compiled for sm_100a with
 nvcc and linked into ltm_b200/libltm_b200.so (in-tree, so it travels with the
 repository snapshot), and of ltm_b200/_torch_ops.so, the tensor-level callers of
-its per-token operators (binding/torch_ops.cpp, g++ against PyTorch's headers).
+its per-token operators (binding/torch_ops.cpp, g++ against PyTorch's headers; left
+out, with a message, where there is no PyTorch: the C ABI does not need it).
 Incremental: an object is rebuilt when its source or any header under csrc/ or
-include/ is newer.
+include/ is newer, _torch_ops.so also when it was built for another PyTorch or
+Python (_build/torch_ops.for).
 
     python obsidian-memory-transformer_b200/build.py [--force] [-j N]
 """
@@ -11,6 +13,8 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -24,6 +28,7 @@ BUILD = PKG / "_build"
 LIB = PKG / "ltm_b200" / "libltm_b200.so"
 OPS_SRC = PKG / "binding" / "torch_ops.cpp"
 OPS = PKG / "ltm_b200" / "_torch_ops.so"
+OPS_FOR = BUILD / "torch_ops.for"  # what OPS was built for
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -54,17 +59,37 @@ def _compile(src: Path, obj: Path, verbose: bool) -> tuple[Path, str]:
     return obj, r.stdout + r.stderr
 
 
-def build_torch_ops(force: bool = False) -> Path:
-    """The CPython module of tensor-level callers; links to libltm_b200.so beside it."""
+def cuda_include() -> Path:
+    """Headers of the CUDA toolkit that nvcc() belongs to."""
+    return Path(shutil.which(nvcc()) or nvcc()).resolve().parents[1] / "include"
+
+
+def torch_here() -> tuple[str, str] | None:
+    """Version and place of the installed PyTorch, without importing it."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        return None
+    return importlib.metadata.version("torch"), spec.origin
+
+
+def build_torch_ops(force: bool = False) -> Path | None:
+    """The CPython module of tensor-level callers; links to libltm_b200.so beside it.
+    None, with a message, where there is no PyTorch."""
+    found = torch_here()
+    if found is None:
+        print(f"{OPS.name} is not built: no PyTorch here (the C ABI library does not need it)",
+              file=sys.stderr)
+        return None
+    wanted = "\n".join([*found, sys.version, str(cuda_include())])
     newest = max(p.stat().st_mtime for p in (OPS_SRC, ROOT / "include" / "ltm_b200.h"))
-    if not force and OPS.exists() and OPS.stat().st_mtime >= newest:
+    if (not force and OPS.exists() and OPS.stat().st_mtime >= newest and OPS_FOR.exists()
+            and OPS_FOR.read_text() == wanted):
         return OPS
     import sysconfig
     import torch
     from torch.utils import cpp_extension
+    inc = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], str(cuda_include())]
     torch_lib = Path(torch.__file__).resolve().parent / "lib"
-    inc = cpp_extension.include_paths() + [sysconfig.get_paths()["include"],
-                                           "/usr/local/cuda/include"]
     tmp = OPS.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
            "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
@@ -75,6 +100,8 @@ def build_torch_ops(force: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {OPS_SRC.name}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, OPS)
+    OPS_FOR.parent.mkdir(exist_ok=True)
+    OPS_FOR.write_text(wanted)
     return OPS
 
 
