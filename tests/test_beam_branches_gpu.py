@@ -24,10 +24,10 @@ def rows(B, W, V, dt, seed, off=1):
 # rows x chunks of 8192 must pass four times the SMs for 16384 logits a CTA
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
 @pytest.mark.parametrize("V", [8193, 16385, 32001])
-@pytest.mark.parametrize("off", [0, 1, 5])
-def test_many_rows(ltm, dt, V, off):
+@pytest.mark.parametrize("off,K", [(0, 16), (1, 16), (5, 16), (1, 17), (3, 64)])
+def test_many_rows(ltm, dt, V, off, K):
     import torch
-    W, K = 8, 16
+    W = 8
     B = 4 * torch.cuda.get_device_properties(0).multi_processor_count // (W * ((V + 8191) // 8192)) + 1
     x, scores, done = rows(B, W, V, dt, V + off, off)
     check(ltm, x, scores, K)
