@@ -321,6 +321,11 @@ LTM_API ltm_status ltm_kv_cache_read(const void* cache, const float* scale, ltm_
  * sequence, get zeros.  What the cache holds at positions that a token does not
  * see never reaches its output, NaN and infinities included.  o does not overlap
  * the caches.
+ * Scores, their maxima and sums, and the output until its one rounding are fp32; the
+ * probabilities are rounded to 16 bits for the value product: to dtype over a 16-bit
+ * cache (bf16: 2^-8, f16: 2^-11 relative to each), to f16 over an int8 cache.  Where more
+ * than 64 rows (T * num_heads / kv_heads) share a 16-bit cached head, the sums are those of
+ * the rounded probabilities.
  * workspace: device memory of ltm_tree_attention_workspace bytes, 16-byte
  * aligned, that nothing else uses until the call's work is done. */
 LTM_API ltm_status ltm_tree_attention_workspace(int B, int T, int num_heads, int kv_heads,
@@ -342,9 +347,14 @@ LTM_API ltm_status ltm_tree_attention(const void* q, const int64_t* q_strides, c
  * beam that does not exist).  done (uint8 [B, W] or NULL): a finished beam
  * continues as itself only, its end_token keeping its score and every other
  * token -inf.  A NaN logit or score counts as -inf, a logit +inf as its type's
- * largest value.  Outputs [B, K]: totals (evaluated in 64 bits, stored as fp32), the beam
+ * largest value.  Outputs [B, K]: totals (stored as fp32), the beam
  * and the token of each, and with done whether the continuation is finished (its
  * beam was, or the token is end_token).  W <= 32, K <= 64.
+ * A row's sum of exponentials and its logarithm are taken in fp32 (within 5e-6), the
+ * totals added up and compared in 64 bits: continuations of different beams whose totals
+ * differ by less than 1e-5 may come in the other order.  Within a beam the order is that
+ * of the logits; with a score or a logit beyond 2^24, those whose totals are one number
+ * in 64 bits count as equal.
  * workspace: device memory of ltm_beam_select_workspace bytes, 8-byte aligned. */
 LTM_API ltm_status ltm_beam_select_workspace(int B, int W, int V, int K, size_t* bytes);
 LTM_API ltm_status ltm_beam_select(const void* logits, ltm_dtype dtype, int64_t batch_stride,

@@ -13,7 +13,8 @@
 // list that the persistent CTAs (one per SM) share out evenly; a CTA that ends or
 // starts inside a head leaves a partial (max, sum, output) there, and
 // tree_combine_kernel merges them, one warp per query row.  Every cached byte is
-// read once for a block of rows; that read is the bound.  Only tiles that reach
+// read once for a block of rows (up to 128 rows, 64 over int8 caches; more rows are more
+// blocks, and each goes through the cache again); that read is the bound.  Only tiles that reach
 // past the context look at the mask: a 64-bit ancestor set per token, found by
 // pointer doubling.
 //
@@ -837,7 +838,9 @@ struct TcSmem {
   static constexpr int kCodes = Q8 ? kTcTile * D : 0;        // K or V tile of codes
   static constexpr int kSlots8 = !Q8 ? 0 : D == 64 ? 8 : kFour ? 3 : 4;
   static constexpr int kOffCodes = kOffRing + kSlots * kTile;
-  static_assert(kSlots * kTile + kSlots8 * kCodes <= kLeft && kSlots >= 3, "ring");
+  static_assert(kSlots * kTile + kSlots8 * kCodes <= kLeft, "the rings fit");
+  // the softmax warps wait for V tiles in a sequence's last tiles only (see there)
+  static_assert(kSlots >= 3, "the load before a tile's V load in its slot has completed by then");
   static constexpr int kOffOnes = kOffCodes + kSlots8 * kCodes;
   static constexpr int kOffMax = kOffOnes + kOnes;  // [2][4][N] maxima / sums
   static constexpr int kOffRef = kOffMax + 8 * N * 4;        // [6][N] per row, see the kernel
@@ -1217,6 +1220,10 @@ __global__ void __launch_bounds__(TcSmem<D, N, Q8>::kThreads, 1)
           }
         };
         if (!Q8 && tail && got && sw < 4) {  // this thread's V row, once it has landed
+          // A wait tells a phase from the next only: this one, of load 2 it + 1, is right if load
+          // 2 it + 1 - NS of the same slot has completed.  S(it) has been waited for; it was
+          // issued after S(it - 1) and O(it - 2), which waited for the loads up to 2 it except V's
+          // of tile it - 1, 2 it - 1: any but NS = 2.
           const int slot = 2 * it + 1;
           got = wait_warp(full + slot % NS, (slot / NS) & 1);
           if (got && at >= 0) {

@@ -527,7 +527,9 @@ def tree_attention(q, k_cache, v_cache, cache_lens, parents=None, k_scale=None, 
     kv_heads); caches of q's type, or int8 with fp32 scales; the drafted tokens
     have been appended (kv_cache_append).  parents: int32 [B, T], -1 for a root;
     None for a chain.  num_tokens: int32 [B], how many of the T tokens a sequence
-    has (the others get zeros).  Returns [B, T, heads, head_dim]."""
+    has (the others get zeros).  The probabilities are rounded to q's type for the value
+    product (int8 caches: to f16), everything else is fp32 until the output's rounding.
+    Returns [B, T, heads, head_dim]."""
     return (_ops_module or _ops()).tree_attention(q, k_cache, v_cache, cache_lens, parents, k_scale,
                                                   v_scale, num_tokens, out, stream)
 
@@ -539,7 +541,8 @@ def beam_select(logits, scores, num_out: int | None = None, done=None, end_token
     that does not exist) -> (scores [B, K] fp32, beams [B, K] int32, tokens [B, K]
     int32) of the K = num_out (W when None) best continuations, best first.  With
     `done` (bool [B, W]) finished beams continue as themselves with `end_token`
-    and a fourth output [B, K] bool says which continuations are finished."""
+    and a fourth output [B, K] bool says which continuations are finished.  Log-sums are
+    fp32: totals of different beams within 1e-5 may come in the other order."""
     return (_ops_module or _ops()).beam_select(logits, scores, num_out, done, end_token, stream)
 
 
