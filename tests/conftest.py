@@ -19,6 +19,18 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a B200 (sm_100a) GPU")
 
 
+def pytest_collection_modifyitems(items):
+    """The reference's own kernels are compiled where its sources are (oracle/ref_kernels.py)
+    and are not part of the repository: without them their live runs cannot be made (the
+    fixture that they once wrote is still compared with the oracle on the CPU)."""
+    built = list((ROOT / "oracle" / "_ref").glob("libref_kernels*.so"))
+    for item in items:
+        if "libs" in getattr(item, "fixturenames", ()) and not built:
+            item.add_marker(pytest.mark.skip(
+                reason="oracle/_ref holds no libref_kernels*.so: python oracle/ref_kernels.py builds "
+                       "them on a machine with the reference's sources"))
+
+
 @pytest.fixture(scope="session")
 def orc():
     from oracle import oracle
