@@ -412,9 +412,9 @@ __device__ void ties_by_index(const T* logits, int64_t ldw, const Rows& r, const
                               int64_t k0, int W, int V, int K, int end) {
   __shared__ int s_found[kBThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  auto total = [&](int w, int x) {
-    return total_bits(r, w, r.done[w] && x != end
-                                ? kNegInf : ordered(logit_value<T>(to_f32(logits[w * ldw + x]))));
+  auto total = [&](int w, int x) {  // (a finished beam's end token whatever its logit)
+    if (r.done[w]) return total_bits(r, w, x == end ? ordered(0.0f) : kNegInf);
+    return total_bits(r, w, ordered(logit_value<T>(to_f32(logits[w * ldw + x]))));
   };
   __syncthreads();  // the outputs are written
   const uint64_t tk = total(o.beams[k0 + K - 1], o.tokens[k0 + K - 1]);

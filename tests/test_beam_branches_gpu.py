@@ -96,6 +96,24 @@ def test_totals_that_64_bits_cannot_tell_apart(ltm, dt, V, K):
     check_inf(ltm, x, torch.zeros((6, 1), device="cuda"), K)
 
 
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+@pytest.mark.parametrize("low", [-1e9, -3.4028234663852886e38])
+def test_far_scores_beside_finished_beams(ltm, dt, low):
+    """Finished beams, whose end token is masked among their logits, between beams of far
+    scores with few tokens left."""
+    import torch
+    B, W, V, K, end = 24, 7, 8193, 14, 3212
+    g = torch.Generator().manual_seed(6)
+    x = (10 * torch.randn((B, W, V), generator=g)).to(torch_dtype(dt)).cuda()
+    x[(torch.rand(x.shape, generator=g) < 0.999).cuda()] = float("-inf")
+    x[:, :, end] = float("-inf")
+    scores = -20 * torch.rand((B, W), generator=g).cuda()
+    scores[:, 1:] = low
+    done = (torch.rand((B, W), generator=g) < 0.3).cuda()
+    check(ltm, x, scores, K, done, end)
+    check(ltm, x, scores, K)
+
+
 def check_inf(ltm, x, scores, K):
     """+inf counts as the type's largest value."""
     import torch
