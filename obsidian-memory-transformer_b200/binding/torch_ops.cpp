@@ -303,6 +303,9 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
       bad("out must have q's shape and type");
     if (given != nullptr) {
       apart(*given, {&kc, &vc, ks, vs}, "out must not overlap the caches");
+      bool itself = given->data_ptr() == q.data_ptr();
+      for (int i = 0; i < 4; ++i) itself &= q.size(i) == 1 || q.stride(i) == given->stride(i);
+      if (!itself) apart(*given, {&q}, "out must be q itself or not overlap it");
       if (at::has_internal_overlap(*given) == at::MemOverlap::Yes)
         bad("elements of out share memory");
     }
