@@ -19,12 +19,12 @@
 // aside), because nearly equal totals of different beams decide the order, and filters
 // and ranks them the same way; within a row the order is that of the logits.
 //
-// Measured: 64 requests x 8 beams x 32000 bf16 logits, K = 16, 22.7 us (chunks 18, merge 7
+// Measured: 64 requests x 8 beams x 32000 bf16 logits, K = 16, 22.5 us (chunks 18, merge 8
 // partly under them): the 33 MB take 5 us to read, the chunks are bound by their
 // instructions (65% of the issue slots; 20 a logit, half of them a chunk's fixed part:
 // maxima of groups, candidates, ranks) and their barriers.  With the logits in registers,
-// three CTAs per SM, it took 26.5 us.  One request of 4 beams: 8.5 us, of which the host
-// needs most to queue two kernels (6.4 us in a captured graph).
+// three CTAs per SM, it took 26.5 us.  One request of 4 beams: 8.9 us, of which the host
+// needs most to queue two kernels (6.8 us in a captured graph).
 //
 // The reference's generation loop samples on the host
 // (python_bindings/ltm/inference.py:131-260).

@@ -16,10 +16,11 @@
 // src/core/quantization/quantizer.cu:94-142 with a row per token and head.
 //
 // Rows are handled by groups of lanes that hold 16 bytes each, several rows per lane in
-// flight.  Measured (cold caches): the int8 write of 4 x 8192 tokens, 32 heads of 128 dims
-// (bf16), 147 us for 0.81 GB (5.5 TB/s; arithmetic: 11 instructions a value); reading
-// either cache back 62 us for 0.40 GB (6.5 TB/s, the copy bandwidth); the reorder of 32
-// beams' caches 474 us, at the copy bandwidth.
+// flight.  Measured (inputs larger than L2): the int8 write of 4 x 8192 tokens, 32 heads of
+// 128 dims, from bf16 142 to 147 us for 0.81 GB (5.7 TB/s; arithmetic: 11 instructions a value),
+// from f16 134 us (6.1 TB/s), from fp32 232 us for 1.35 GB (5.8 TB/s); into a 16-bit cache 162 us
+// for 1.07 GB (6.6 TB/s, the copy bandwidth); reading the int8 cache back 64 us for 0.41 GB
+// (6.3 TB/s); the reorder of 32 beams' caches 473 us, at the copy bandwidth.
 #include <algorithm>
 #include <type_traits>
 #include <utility>

@@ -28,7 +28,7 @@
 //   accumulator transposed in registers.  Nothing is exchanged until the segment's
 //   end, where the warps' (max, sum, output) are merged in shared memory.  int8 codes
 //   become f16 in registers (exact), with the row's scale applied to the fp32 score (K)
-//   and to the probability (V); those conversions bound the kernel, so int8 caches run
+//   and to the probability (V); those conversions are most of its instructions, so int8 caches run
 //   15 consumer warps up to 8 rows (16 warps with the producer: 128 registers a
 //   thread) and 11 beyond (168), 16-bit ones 8.  A tile is 16 keys for every warp:
 //   each warp waits for every load in turn (a warp that skipped tiles could take a
@@ -40,16 +40,20 @@
 //   test, its scales and the clean-up of rows past the end are its own.  int8 codes
 //   become f16 tiles in shared memory first.
 //
-// Measured (bf16 queries, calls back to back).  Read-bound: one row per head of 128 dims
-// over a 16-bit cache, 16 x 32 heads x 8192 to 16384 positions, 0.46 ms for 3.2 GB (6.9
-// TB/s); int8, 64 x 32 heads x 4096 to 8192, 0.51 ms for 3.3 GB, 0.60 once the clock has
-// dropped under load (5.6 TB/s).  The int8 conversions bound 9 to 16 rows (8 x 32
-// heads x 16384 positions of 128 dims 0.26 ms, 4.1 TB/s).  tree_tc_kernel reads a 16-bit
-// tile of 128 positions in 0.7 us (64 dims) or 1.4 us (128 dims); with 32, 64 and 128 rows it
-// takes 0.98, 1.26 and 1.84 us for 64 dims, 1.40, 1.45 and 2.2 us for 128: up to 64 rows of
-// 128 dims are read-bound, the others bound by the softmax's latencies (exponentials,
-// votes, barriers).  int8: 1.25 and 1.66 us for 32 and 64 rows of 64 dims, 1.53 and 2.45
-// us for 128.  A segment's start and end cost 7 to 9 us (half of it queries, masks and the
+// Measured (bf16 queries, calls back to back; the second of two figures once the clock has
+// dropped under load).  Read-bound: one row per head of 128 dims over a 16-bit cache, 16 x
+// 32 heads x 8192 to 16384 positions, 0.47 ms for 3.2 GB (6.9 TB/s); int8, 64 x 32 heads x 4096
+// to 8192, 0.52 to 0.61 ms for 3.3 GB (5.5 to 6.4 TB/s).  9 to 16 int8 rows of 128 dims: 8 x 32
+// heads x 16384 positions 0.25 to 0.29 ms, where DRAM (45%) and issue slots (51%) both
+// wait for the chain of a warp's tile: conversions, products, exponentials.
+// Time of a 128-position tile, CTA by CTA, over 8 x 32 heads x 16384 positions in us (to read:
+// 0.74 for 64 dims, 1.48 for 128; int8 0.39 and 0.76):
+//   rows            16    32    64   128
+//   64 dims       0.77  1.00  1.33  1.90   up to 16 rows read-bound, then by the softmax's
+//   128 dims      1.38  1.46  1.64   2.7   latencies (exponentials, votes, barriers)
+//   64 dims int8  0.80  1.28  1.82   3.6   (two blocks of 64 rows) latencies and, with
+//   128 dims int8 1.23  1.54  2.53   5.0   64 rows of 128 dims, three slots of f16 tiles
+// A segment's start and end cost 7 to 9 us (half of it queries, masks and the
 // tail's clean-up; 13 before those were overlapped and rid of divisions).
 //
 // In both, a row's reference maximum is only raised when a score exceeds it by more
