@@ -400,13 +400,18 @@ __device__ __forceinline__ void write_out(const Outputs& o, const Rows& r, int64
   if (o.done) o.done[k] = r.done[w] || tok == end;
 }
 
+constexpr float kFar = 16777216.0f;  // 2^24: steps of 2^-28
+__device__ __forceinline__ bool far_out(const Rows& r, int w) {
+  const float x = fmaxf(fabsf(r.max[w]), fabsf(static_cast<float>(r.score[w])));
+  return x >= kFar && x < INFINITY && !r.done[w];
+}
+
 // For a request with a row so far out that 64 bits may give different logits one total (a
 // score of fp32's lowest value, say, or a logit of +inf): a chunk's list, ordered by the
 // logits, then may lack continuations of a total that it holds.  Only those equal to the
 // K-th total matter (of greater ones there are fewer than K, so they are all in the lists),
 // and of those the lowest indices are the request's: the outputs from k0 + c on, c the number
 // of greater totals, are written anew from the logits, beam after beam.  By the whole CTA.
-constexpr float kFar = 16777216.0f;  // 2^24: steps of 2^-28
 template <class T>
 __device__ void ties_by_index(const T* logits, int64_t ldw, const Rows& r, const Outputs& o,
                               int64_t k0, int W, int V, int K, int end) {
@@ -419,15 +424,32 @@ __device__ void ties_by_index(const T* logits, int64_t ldw, const Rows& r, const
   __syncthreads();  // the outputs are written
   const uint64_t tk = total(o.beams[k0 + K - 1], o.tokens[k0 + K - 1]);
   if (tk == ordered64(-INFINITY)) return;  // equal logits (-inf) only
+  // no row far out that reaches the K-th total: as with beams that have lost already
+  if (!__syncthreads_or(tid < W && far_out(r, tid) &&
+                        total_bits(r, tid, ordered(r.max[tid])) >= tk))
+    return;
   int at = __syncthreads_count(tid < K && total(o.beams[k0 + tid], o.tokens[k0 + tid]) > tk);
 #pragma unroll 1
   for (int w = 0; w < W && at < K; ++w) {
     if (!(r.score[w] > -INFINITY)) continue;
     if (!r.done[w] && (r.max[w] == -INFINITY || total_bits(r, w, ordered(r.max[w])) < tk)) continue;
+    const int n = r.done[w] ? end + 1 : V;
 #pragma unroll 1
-    for (int i0 = r.done[w] ? end : 0; i0 < (r.done[w] ? end + 1 : V) && at < K; i0 += kBThreads) {
+    for (int i0 = r.done[w] ? end : 0; i0 < n && at < K; i0 += kBThreads) {
+      // most of a row holds none: 16 tokens a thread until there is one
+      while (!r.done[w] && i0 + 16 * kBThreads <= n) {
+        T y[16];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) y[x] = logits[w * ldw + i0 + x * kBThreads + tid];
+        bool any = false;
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          any |= total_bits(r, w, ordered(logit_value<T>(to_f32(y[x])))) == tk;
+        if (__syncthreads_or(any)) break;
+        i0 += 16 * kBThreads;
+      }
       const int i = i0 + tid;
-      const bool hit = i < V && total(w, i) == tk;
+      const bool hit = i < n && total(w, i) == tk;
       const uint32_t hits = __ballot_sync(0xffffffffu, hit);
       if (lane == 0) s_found[warp] = __popc(hits);
       __syncthreads();
@@ -508,8 +530,7 @@ __global__ void __launch_bounds__(kBThreads)
     if (lane == 0) {
       rows.max[w] = m;
       rows.lse[w] = static_cast<double>(logf(sum));
-      const float out = fmaxf(fabsf(m), fabsf(static_cast<float>(rows.score[w])));
-      if (out >= kFar && out < INFINITY && !rows.done[w]) s_far = 1;
+      if (far_out(rows, w)) s_far = 1;
     }
   }
   __syncthreads();
