@@ -320,7 +320,8 @@ LTM_API ltm_status ltm_kv_cache_read(const void* cache, const float* scale, ltm_
  * caches serve both.  Tokens t >= num_tokens[b], and those of a skipped
  * sequence, get zeros.  What the cache holds at positions that a token does not
  * see never reaches its output, NaN and infinities included.  o does not overlap
- * the caches; it may be q (with q's strides), and overlaps it in no other way.
+ * the caches; it may be q (with q's strides), and with more than 512 sequences, which
+ * are several launches, overlaps it in no other way.
  * Scores, their maxima and sums, and the output until its one rounding are fp32; the
  * probabilities are rounded to 16 bits for the value product: to dtype over a 16-bit
  * cache (bf16: 2^-8, f16: 2^-11 relative to each), to f16 over an int8 cache.  Where more

@@ -148,10 +148,9 @@ struct BeamPartial {
 // and five CTAs share an SM: their loads, exponentials and filters overlap.
 template <class T, int PER>
 __global__ void __launch_bounds__(kBThreads, 5)
-    beam_chunk_kernel(const T* logits, int64_t ldb, int64_t ldw,
-                      const float* scores, const uint8_t* done, int end,
-                      int W, int V, int K, int nchunk, int groups, BeamPartial* __restrict__ stats,
-                      uint64_t* __restrict__ lists) {
+    beam_chunk_kernel(const T* logits, int64_t ldb, int64_t ldw, const float* scores,
+                      const uint8_t* done, int end, int W, int V, int K, int nchunk, int groups,
+                      BeamPartial* __restrict__ stats, uint64_t* __restrict__ lists) {
   constexpr int N = 16 / sizeof(T);  // logits per vector
   constexpr int NV = PER / N;        // vectors per thread
   constexpr int kChunk = kBThreads * PER, kVecs = kBThreads * NV;
@@ -384,12 +383,12 @@ __device__ __forceinline__ uint64_t total_bits(const Rows& r, int w, uint32_t u)
   return ordered64(t);
 }
 
-// Writes continuation f = beam * V + token with the total t as the k-th of its request.
-struct Outputs {
+struct Outputs {  // [B, K]
   float* scores;
   int *beams, *tokens;
   uint8_t* done;
 };
+// Output k: continuation f = beam * V + token of total t (ordered bits).
 __device__ __forceinline__ void write_out(const Outputs& o, const Rows& r, int64_t k, uint64_t t,
                                           uint32_t f, int V, int end) {
   const int w = static_cast<int>(f / static_cast<uint32_t>(V));
@@ -485,9 +484,8 @@ __device__ __noinline__ void order_ties(const void* logits, ltm_dtype dtype, int
 // one.  Loops stay rolled: for one request the code's own fetch is most of the time.
 __global__ void __launch_bounds__(kBThreads)
     beam_merge_kernel(const void* logits, ltm_dtype dtype, int64_t ldb, int64_t ldw,
-                      const float* scores, const uint8_t* done, int end,
-                      int W, int V, int K, int nchunk, const BeamPartial* stats,
-                      const uint64_t* lists,
+                      const float* scores, const uint8_t* done, int end, int W, int V, int K,
+                      int nchunk, const BeamPartial* stats, const uint64_t* lists,
                       const __grid_constant__ Outputs out) {
   __shared__ Rows rows;
   __shared__ int s_far;  // a row is far out

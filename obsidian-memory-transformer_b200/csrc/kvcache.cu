@@ -212,11 +212,10 @@ __device__ __forceinline__ void magnitudes(const uint4 (&raw)[NP], int g, float 
 // neighbouring heads of the same tokens: the reads cover whole projection rows.
 template <class T, int D, bool Q8>
 __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 ? 4 : 2)
-    cache_append_kernel(const T* k, RowStrides sk, const T* v,
-                        RowStrides sv, void* __restrict__ kc, void* __restrict__ vc,
-                        float* __restrict__ ks, float* __restrict__ vs, int64_t P,
-                        const int* lens, const int* num_tokens, int Tn,
-                        int heads, int tgroups, int* err) {
+    cache_append_kernel(const T* k, RowStrides sk, const T* v, RowStrides sv,
+                        void* __restrict__ kc, void* __restrict__ vc, float* __restrict__ ks,
+                        float* __restrict__ vs, int64_t P, const int* lens, const int* num_tokens,
+                        int Tn, int heads, int tgroups, int* err) {
   constexpr int N = 16 / sizeof(T);   // values per piece
   constexpr int NP = kVals / N;       // pieces per lane
   constexpr int G = D / kVals;        // lanes per row
@@ -322,9 +321,8 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 ? 4 : 2)
 // 16-bit cache, that it holds of a row.
 template <class O, int D, bool Q8>
 __global__ void __launch_bounds__(kWarps * 32)
-    cache_read_kernel(const void* cache, const float* scale, int64_t P,
-                      const int* first, const int* lens, int heads,
-                      int n, O* __restrict__ out) {
+    cache_read_kernel(const void* cache, const float* scale, int64_t P, const int* first,
+                      const int* lens, int heads, int n, O* __restrict__ out) {
   constexpr int V = 16 / sizeof(O);
   using Raw = std::conditional_t<!Q8, uint4, std::conditional_t<V == 8, uint2, uint32_t>>;
   constexpr int G = D / V;

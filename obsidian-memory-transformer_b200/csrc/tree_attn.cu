@@ -14,8 +14,8 @@
 // starts inside a head leaves a partial (max, sum, output) there, and
 // tree_combine_kernel merges them, one warp per query row.  Every cached byte is
 // read once for a block of rows (up to 128 rows, 64 over int8 caches; more rows are more
-// blocks, and each goes through the cache again); that read is the bound.  Only tiles that reach
-// past the context look at the mask: a 64-bit ancestor set per token, found by
+// blocks, and each goes through the cache again); that read is the bound.  Only tiles that
+// reach past the context look at the mask: a 64-bit ancestor set per token, found by
 // pointer doubling.
 //
 // Two kernels contract the tiles, by the rows G * T that share a cached head:
@@ -28,9 +28,9 @@
 //   accumulator transposed in registers.  Nothing is exchanged until the segment's
 //   end, where the warps' (max, sum, output) are merged in shared memory.  int8 codes
 //   become f16 in registers (exact), with the row's scale applied to the fp32 score (K)
-//   and to the probability (V); those conversions are most of its instructions, so int8 caches run
-//   15 consumer warps up to 8 rows (16 warps with the producer: 128 registers a
-//   thread) and 11 beyond (168), 16-bit ones 8.  A tile is 16 keys for every warp:
+//   and to the probability (V); those conversions are most of its instructions, so
+//   int8 caches run 15 consumer warps up to 8 rows (16 warps with the producer: 128
+//   registers a thread) and 11 beyond (168), 16-bit ones 8.  A tile is 16 keys for every warp:
 //   each warp waits for every load in turn (a warp that skipped tiles could take a
 //   barrier's phase for the one before).
 // * tree_tc_kernel, more rows: tcgen05, keys as the 128 lanes:
@@ -58,9 +58,10 @@
 //
 // In both, a row's reference maximum is only raised when a score exceeds it by more
 // than 2^8.  Weights that go to the tensor core as f16 are held 2^7 higher (Raise), so that
-// the many small ones of a long context stay above its smallest numbers.  A non-finite value of a drafted token must not
-// reach the tokens that do not see it (0 * inf): it is taken out of the tile, and
-// the combine kernel adds it to the rows that do.
+// the many small ones of a long context stay above its smallest numbers.  A non-finite
+// value of a drafted token must not reach the tokens that do not see it (0 * inf): it is
+// taken out of the tile, and the combine kernel adds it to the rows that do; over int8
+// caches, whose non-finite rows have the scale NaN, their weights become NaN instead.
 //
 // The reference has no counterpart: its cache manager is a stub
 // (python_bindings/src/main.cpp:101-135).
