@@ -66,3 +66,28 @@ def test_output_dropped_while_the_current_stream_reads_it(ltm, what):
         torch.cuda.synchronize()
         assert torch.equal(copy, want)
         del junk
+
+
+@pytest.mark.parametrize("what", ["read", "tree", "beam"])
+def test_captured_on_a_branch(ltm, what):
+    """A call on a stream that joined a capture, replayed while the inputs stay; outputs of
+    two calls do not share memory."""
+    import torch
+    call, _ = _calls(ltm)[what]
+    want = call(None).clone()
+    other = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        here = torch.cuda.current_stream()
+        other.wait_stream(here)
+        a = call(other)
+        b = call(None)
+        here.wait_stream(other)
+        c = a.clone()
+        d = call(None)
+    for _ in range(3):
+        for x in (a, b, c, d):
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, want) for x in (a, b, c, d))
