@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 2 ? 4 : 2)
 template <class O, int D, bool Q8>
 __global__ void __launch_bounds__(kWarps * 32)
     cache_read_kernel(const void* cache, const float* scale, int64_t P, const int* first,
-                      const int* lens, int heads, int n, O* __restrict__ out) {
+                      const int* lens, int heads, int n, int start, O* __restrict__ out) {
   constexpr int V = 16 / sizeof(O);
   using Raw = std::conditional_t<!Q8, uint4, std::conditional_t<V == 8, uint2, uint32_t>>;
   constexpr int G = D / V;
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   grid_release();
   const int lane = threadIdx.x & 31;
   const int bh = blockIdx.x;
-  const int i0 = (blockIdx.y * kWarps + (threadIdx.x >> 5)) * ROWS;
+  const int64_t i0 = start + static_cast<int64_t>(blockIdx.y * kWarps + (threadIdx.x >> 5)) * ROWS;
   if (i0 >= n) return;
   const int b = bh / heads;
   const int64_t p0 = first ? first[b] : 0;
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   float s[kReadFly];
 #pragma unroll
   for (int j = 0; j < kReadFly; ++j) {
-    const int i = i0 + j * RP + sub;
+    const int64_t i = i0 + j * RP + sub;
     const int64_t p = p0 + i;
     const bool live = i < n && p >= 0 && p < end;
     const int64_t row = bh * P + p;
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 #pragma unroll
   for (int j = 0; j < kReadFly; ++j) {
-    const int i = i0 + j * RP + sub;
+    const int64_t i = i0 + j * RP + sub;
     if (i >= n) continue;
     O* dst = out + (static_cast<int64_t>(bh) * n + i) * D + gl * V;
     if constexpr (Q8) {
@@ -539,18 +539,22 @@ extern "C" ltm_status ltm_kv_cache_read(const void* cache, const float* scale, l
     LTM_REQUIRE(((reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
                 "the cache and the output must be 16-byte aligned");
     const int rows = 32 / (head_dim * static_cast<int>(dtype_size(out_dtype)) / 16) * kReadFly * kWarps;  // per CTA
-    const int gy = (n + rows - 1) / rows;
-    LTM_REQUIRE(static_cast<int64_t>(B) * kv_heads < (1ll << 31) && gy < (1 << 16), "too many rows");
-    const dim3 grid(static_cast<unsigned>(B) * kv_heads, static_cast<unsigned>(gy));
+    LTM_REQUIRE(static_cast<int64_t>(B) * kv_heads < (1ll << 31), "too many rows");
+    constexpr int64_t kMostBlocks = 65535;  // of a launch, in y
     const cudaStream_t st = as_stream(stream);
     dispatch_dtype(out_dtype, [&](auto tag) {
       using O = decltype(tag);
       by_head_dim(head_dim, [&](auto d_c) {
         constexpr int D = decltype(d_c)::value;
         auto go = [&](auto q_c) {
-          launch_dependent(cache_read_kernel<O, D, decltype(q_c)::value>, grid, kWarps * 32, 0, st,
-                           cache, scale, max_positions, first, cache_lens, kv_heads, n,
-                           static_cast<O*>(out));
+          for (int64_t start = 0; start < n; start += kMostBlocks * rows) {
+            const int64_t gy = std::min<int64_t>((n - start + rows - 1) / rows, kMostBlocks);
+            launch_dependent(cache_read_kernel<O, D, decltype(q_c)::value>,
+                             dim3(static_cast<unsigned>(B) * kv_heads, static_cast<unsigned>(gy)),
+                             kWarps * 32, 0, st, cache, scale, max_positions, first, cache_lens,
+                             kv_heads, n, static_cast<int>(start), static_cast<O*>(out));
+            check_launch("cache_read_kernel", st);
+          }
         };
         if constexpr (std::is_same<O, float>::value) {
           go(std::true_type{});
@@ -560,7 +564,6 @@ extern "C" ltm_status ltm_kv_cache_read(const void* cache, const float* scale, l
         }
       });
     });
-    check_launch("cache_read_kernel", st);
   });
 }
 

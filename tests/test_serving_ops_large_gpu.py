@@ -107,3 +107,15 @@ def test_reorder(ltm):
         assert torch.equal(x[:, :, far], y)
         assert not x[:, :, hi:].any() and not x[:, :, lo - 1000:lo].any()
     assert ltm.device_error() == 0
+
+
+def test_read_of_a_very_long_sequence(ltm):
+    """More positions than one launch takes (65535 blocks of 64)."""
+    n = 65535 * 64 + 100
+    c = torch.zeros((1, 1, n, D), dtype=torch.int8, device="cuda")
+    c[0, 0, :, 0] = torch.arange(n, device="cuda") % 127
+    c[0, 0, :, 1] = torch.arange(n, device="cuda") // 65536
+    s = torch.ones((1, 1, n), device="cuda")
+    got = ltm.kv_cache_read(c, s, n, first=i32(3), cache_lens=i32(n - 5))
+    assert torch.equal(got[0, 0, :n - 8], c[0, 0, 3:n - 5].float())
+    assert not got[0, 0, n - 8:].any()
